@@ -13,7 +13,9 @@ from .config import MoEConfig
 LIB_PATH = Path(__file__).resolve().parent / "libeva_moe.so"
 
 EVA_OK, EVA_ERR_INVALID, EVA_ERR_CUDA, EVA_ERR_WORKSPACE = 0, 1, 2, 3
-STATUS_BAD_EXPERT, STATUS_TIMEOUT, STATUS_CAPACITY = 1, 2, 4
+STATUS_BAD_EXPERT, STATUS_TIMEOUT, STATUS_CAPACITY, STATUS_BAD_BATCH = 1, 2, 4, 8
+DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
+KV_PAGE, KV_BLOCK = 64, 16
 ACT_CLAMP_AFTER, ACT_CLAMP_BEFORE = 0, 1
 
 # every symbol include/eva_moe.h declares
@@ -23,7 +25,8 @@ EXPORTS = ("eva_moe_workspace_bytes", "eva_moe_clear_status", "eva_moe_read_stat
            "eva_ep_dispatch", "eva_ep_combine", "eva_ep_arena_layout", "eva_peer_alloc", "eva_peer_open",
            "eva_peer_close", "eva_peer_free", "eva_ep_dispatch_peers", "eva_ep_wait_rows", "eva_ep_signal_partials",
            "eva_ep_combine_peers", "eva_rmsnorm_residual", "eva_moe_experts_window", "eva_decode_microbench",
-           "eva_tc_selftest", "eva_pool_plan", "eva_pool_copy", "eva_host_mapped")
+           "eva_tc_selftest", "eva_pool_plan", "eva_pool_copy", "eva_host_mapped", "eva_rotary", "eva_kv_append",
+           "eva_kv_attend_workspace", "eva_kv_attend")
 EP_MAX_WORLD = 32
 NOALLOC_SCRATCH_BYTES = 16 << 20
 
@@ -63,6 +66,24 @@ class EvaEpPeers(ctypes.Structure):
                 ("reserved", ctypes.c_int32), ("off_x", ctypes.c_uint64), ("off_sel", ctypes.c_uint64),
                 ("off_rw", ctypes.c_uint64), ("off_part", ctypes.c_uint64), ("bytes", ctypes.c_uint64),
                 ("arena", ctypes.c_void_p * EP_MAX_WORLD), ("owner", ctypes.c_void_p), ("local_id", ctypes.c_void_p)]
+
+
+class EvaRotary(ctypes.Structure):
+    _fields_ = [("dim", ctypes.c_int32), ("offset", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("inverse", ctypes.c_int32), ("mscale", ctypes.c_float), ("reserved", ctypes.c_int32),
+                ("turns", ctypes.c_void_p)]
+
+
+class EvaKvCache(ctypes.Structure):
+    _fields_ = [("pages", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("key_dim", ctypes.c_int32),
+                ("value_dim", ctypes.c_int32), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("status", ctypes.c_void_p)]
+
+
+class EvaKvBatch(ctypes.Structure):
+    _fields_ = [("seqs", ctypes.c_int32), ("tokens", ctypes.c_int32), ("max_q", ctypes.c_int32),
+                ("max_pages", ctypes.c_int32), ("table_stride", ctypes.c_int64), ("q_start", ctypes.c_void_p),
+                ("seq_lens", ctypes.c_void_p), ("table", ctypes.c_void_p)]
 
 
 _lib = None
@@ -136,6 +157,15 @@ def load(build_if_missing: bool = True):
     L.eva_pool_copy.argtypes = [P(EvaExpertPool), vp, i32, vp, vp]
     L.eva_host_mapped.restype = ctypes.c_int
     L.eva_host_mapped.argtypes = [vp]
+    i64, f32 = ctypes.c_int64, ctypes.c_float
+    L.eva_rotary.restype = ctypes.c_int
+    L.eva_rotary.argtypes = [P(EvaRotary), vp, i32, i32, i32, i32, i64, i64, vp, i32, vp, i64, i64, vp]
+    L.eva_kv_append.restype = ctypes.c_int
+    L.eva_kv_append.argtypes = [P(EvaKvCache), P(EvaKvBatch), P(EvaRotary), vp, i64, i64, vp, i64, i64, i32, vp]
+    L.eva_kv_attend_workspace.restype = sz
+    L.eva_kv_attend_workspace.argtypes = [P(EvaKvCache), P(EvaKvBatch), i32]
+    L.eva_kv_attend.restype = ctypes.c_int
+    L.eva_kv_attend.argtypes = [P(EvaKvCache), P(EvaKvBatch), vp, i32, i32, i64, i64, f32, i32, vp, sz, vp, vp]
     L.eva_moe_arch.restype = i32
     L.eva_moe_arch.argtypes = []
     _lib = L

@@ -1,0 +1,345 @@
+"""Attention between the MoE layers: rotary positions, a paged 8-bit key/value cache, and causal attention over it.
+
+* `Rotary` rotates part of each head by its token's position (interleaved or half layout, linear, NTK or YaRN scaling).
+* `PagedKVCache` holds one layer's keys and values as e4m3 codes with a power-of-two scale for each 16 tokens and head;
+  `append` rotates, quantises and writes new tokens, `attend` reads them.
+* `PagedBatch` names the sequences of a step: which token rows, how long, and which pages.
+* `PagedAttention` is the attention half of a layer (projections around the three), which `MoEStack` calls.
+
+The reference's attention (runtime/ds41/model.py:566-937 `Attention`) reads a 4-bit compressed cache through an index;
+this is plain causal attention, for layers of DeepSeek shape without that index. Everything runs on the caller's current
+CUDA stream and never synchronises the host, so it can be captured in a CUDA graph and replayed; outputs and
+workspaces come from torch's allocator for each call.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+
+_F16, _BF16, _F32, _I32, _I64 = torch.float16, torch.bfloat16, torch.float32, torch.int32, torch.int64
+_E4M3, _E8M0, _U8 = torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.uint8
+_DTYPE = {_F16: _lib.DTYPE_F16, _BF16: _lib.DTYPE_BF16, _F32: _lib.DTYPE_F32}
+PAGE, BLOCK = _lib.KV_PAGE, _lib.KV_BLOCK
+HEAD_DIMS = ((64, 64), (128, 128), (192, 128))
+_INT32_MAX = 2**31 - 1
+
+
+def _device(device) -> torch.device:
+    device = torch.device(device)
+    if device.type != "cuda" or not torch.cuda.is_available():
+        raise RuntimeError("the attention operators require a CUDA device; there is no CPU fallback")
+    return torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
+
+
+def _on(device):
+    """The library launches on the current device: make it the tensors'."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _rows(t, name, device, dtypes, heads=None, dim=None):
+    if not isinstance(t, torch.Tensor) or t.device != device or t.ndim != 3 or t.dtype not in dtypes:
+        raise ValueError(f"{name} must be [tokens, heads, dim] of {', '.join(map(str, dtypes))} on {device}")
+    if (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim):
+        raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {dim}]")
+    return t
+
+
+def _strides(t):
+    """Token and head stride in elements; 0 where there is nothing to step to."""
+    return (t.stride(0) if t.shape[0] > 1 else 0), (t.stride(1) if t.shape[1] > 1 else 0)
+
+
+class Rotary:
+    """Rotation of `dim` dimensions of a head from `offset` on by position * frequency_i, i < dim / 2.
+
+    layout: "half" pairs dimension i with i + dim / 2, "interleaved" 2i with 2i + 1. Frequencies are
+    base^(-2i / dim), changed by `scaling`: "linear" divides positions by `factor`; "ntk" raises the base to
+    base * factor^(dim / (dim - 2)); "yarn" divides the frequencies that turn less than beta_slow times in
+    original_len positions by `factor`, keeps those above beta_fast, goes linearly between, and scales the result by
+    0.1 ln(factor) + 1. mscale replaces that scale. Angles are exact modulo a turn at any position."""
+
+    def __init__(self, dim, *, base=10000.0, layout="interleaved", offset=0, scaling="none", factor=1.0,
+                 original_len=4096, beta_fast=32.0, beta_slow=1.0, mscale=None, device="cuda"):
+        self.inv_freq, scale = rotary_frequencies(dim, base=base, scaling=scaling, factor=factor,
+                                                  original_len=original_len, beta_fast=beta_fast, beta_slow=beta_slow)
+        if layout not in ("half", "interleaved"):
+            raise ValueError("layout must be 'half' or 'interleaved'")
+        if type(offset) is not int or offset < 0 or offset % 2:
+            raise ValueError("offset must be an even nonnegative int")
+        mscale = scale if mscale is None else mscale
+        if not isinstance(mscale, (int, float)) or not math.isfinite(mscale):
+            raise ValueError("mscale must be a finite number")
+        self.dim, self.offset, self.layout, self.mscale = dim, offset, layout, float(mscale)
+        self.device = _device(device)
+        self.lib = _lib.load()
+        self.turns = torch.tensor(turns_of(self.inv_freq), dtype=_I64, device=self.device)
+        args = (dim, offset, int(layout == "interleaved"))
+        self._c = _lib.EvaRotary(*args, 0, self.mscale, 0, self.turns.data_ptr())
+        self._c_inverse = _lib.EvaRotary(*args, 1, self.mscale, 0, self.turns.data_ptr())
+
+    def apply(self, x, positions, *, inverse=False, out=None):
+        """x [tokens, heads, head_dim] (BF16, Half or Float; last dimension contiguous) rotated by positions (int32 or
+        int64 [tokens]); inverse rotates back by the same scale, as the gradient does. out: x itself, or a tensor that does not
+        overlap it; default a new one."""
+        _rows(x, "x", self.device, (_BF16, _F16, _F32))
+        tokens, heads, head_dim = x.shape
+        if self.offset + self.dim > head_dim:
+            raise ValueError(f"x's heads have {head_dim} dimensions, the rotation ends at {self.offset + self.dim}")
+        if heads < 1:
+            raise ValueError("x has no heads")
+        if (not isinstance(positions, torch.Tensor) or positions.device != self.device or positions.ndim != 1
+                or positions.shape[0] != tokens or positions.dtype not in (_I32, _I64) or not positions.is_contiguous()):
+            raise ValueError(f"positions must be contiguous int32 or int64 [{tokens}] on {self.device}")
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=self.device)
+        elif out is not x:
+            _rows(out, "out", self.device, (x.dtype,), heads, head_dim)
+            if out.shape[0] != tokens:
+                raise ValueError("out must have x's shape")
+            if any(st == 0 and n > 1 for n, st in zip(out.shape, out.stride())):
+                raise ValueError("out must not overlap itself")
+            if out.data_ptr() == x.data_ptr() and out.stride() == x.stride() and tokens:
+                pass   # the same memory: in place
+            elif _overlap(x, out):
+                raise ValueError("out must be x itself or not overlap it")
+        if tokens == 0:
+            return out
+        src = self._movable(x, out is x)
+        dst = out if self._movable(out, True) is out else None
+        if src is None or dst is None:
+            raise ValueError("a tensor written to needs a contiguous last dimension and, with interleaved pairs, aligned ones")
+        if src is not x and out.data_ptr() == x.data_ptr():
+            raise ValueError("in place, x needs a contiguous last dimension and, with interleaved pairs, aligned ones")
+        (xt, xh), (ot, oh) = _strides(src), _strides(dst)
+        with _on(self.device):
+            rc = self.lib.eva_rotary(ctypes.byref(self._c_inverse if inverse else self._c), src.data_ptr(), _DTYPE[x.dtype],
+                                     tokens, heads, head_dim, xt, xh, positions.data_ptr(), int(positions.dtype == _I64),
+                                     dst.data_ptr(), ot, oh, torch.cuda.current_stream(self.device).cuda_stream)
+        _lib.check(rc, "eva_rotary")
+        return out
+
+    def _movable(self, t, must):
+        """t, or a contiguous copy of it (None where it must be t itself), as the kernel moves it: whole elements side by side,
+        interleaved pairs at addresses that are multiples of a pair."""
+        pair = self.layout == "interleaved"
+        st, sh = _strides(t)
+        ok = t.stride(2) == 1 or t.shape[2] == 1
+        if ok and pair:
+            ok = t.data_ptr() % (2 * t.element_size()) == 0 and st % 2 == 0 and sh % 2 == 0 and t.shape[2] % 2 == 0
+        if ok:
+            return t
+        if must or (pair and t.shape[2] % 2):
+            return None
+        return t.clone(memory_format=torch.contiguous_format)
+
+
+def _span(t):
+    n = t.element_size()
+    return t.data_ptr(), t.data_ptr() + n * (1 + sum((s - 1) * st for s, st in zip(t.shape, t.stride())))
+
+
+def _overlap(a, b):
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
+def rotary_frequencies(dim, *, base=10000.0, scaling="none", factor=1.0, original_len=4096, beta_fast=32.0, beta_slow=1.0):
+    """(angle per position of each pair, scale of the rotated part), as Python floats."""
+    if type(dim) is not int or dim < 2 or dim % 2:
+        raise ValueError("dim must be an even positive int")
+    if scaling not in ("none", "linear", "ntk", "yarn"):
+        raise ValueError("scaling must be 'none', 'linear', 'ntk' or 'yarn'")
+    if not (math.isfinite(base) and base > 1.0 and math.isfinite(factor) and factor >= 1.0):
+        raise ValueError("base must be above 1 and factor at least 1")
+    if scaling == "ntk":
+        if dim < 4:
+            raise ValueError("ntk scaling needs dim >= 4")
+        base = base * factor ** (dim / (dim - 2))
+    freq = [base ** (-2.0 * i / dim) for i in range(dim // 2)]
+    if scaling == "linear":
+        return [f / factor for f in freq], 1.0
+    if scaling != "yarn":
+        return freq, 1.0
+    if not (original_len >= 1 and beta_fast >= beta_slow > 0):
+        raise ValueError("yarn needs original_len >= 1 and beta_fast >= beta_slow > 0")
+
+    def pair_turning(times):   # the (fractional) pair that makes so many turns in original_len positions
+        return dim * math.log(original_len / (times * 2 * math.pi)) / (2 * math.log(base))
+
+    low = max(math.floor(pair_turning(beta_fast)), 0)
+    high = min(math.ceil(pair_turning(beta_slow)), dim - 1)
+    width = max(high - low, 0.001)
+    out = []
+    for i, f in enumerate(freq):
+        slow = min(max((i - low) / width, 0.0), 1.0)
+        out.append(f / factor * slow + f * (1.0 - slow))
+    return out, 0.1 * math.log(factor) + 1.0
+
+
+def turns_of(inv_freq):
+    """Frequencies as fractions of a turn times 2^64, modulo 2^64, as int64 values (the same bits)."""
+    out = []
+    for f in inv_freq:
+        t = f / (2 * math.pi)
+        t = int((t - math.floor(t)) * 2.0**64) % 2**64
+        out.append(t - 2**64 if t >= 2**63 else t)
+    return out
+
+
+class PagedBatch:
+    """The sequences of one step. q_start: int32 [seqs + 1], sequence b has token rows q_start[b] .. q_start[b + 1] - 1 of the
+    step's tensors; they are the last ones of its seq_lens[b] tokens (int32 [seqs], new ones included), and token t of it
+    lies in page table[b, t // 64] (int32 [seqs, pages], contiguous rows). max_q: the most rows of a sequence.
+
+    The tensors stay the caller's: a captured step is replayed with new contents in them (max_q and the table's width
+    bound what they may hold). A padding sequence has length 0 (its rows come out zero, nothing is appended). What does
+    not fit (page ids outside the cache, lengths beyond the table, rows out of order) sets STATUS_BAD_BATCH in the cache's
+    status and is left out. A page that two sequences of a batch append to is the caller's error: its contents are then undefined."""
+
+    def __init__(self, q_start, seq_lens, table, max_q):
+        for name, t, nd in (("q_start", q_start, 1), ("seq_lens", seq_lens, 1), ("table", table, 2)):
+            if not isinstance(t, torch.Tensor) or t.dtype != _I32 or t.ndim != nd or t.device.type != "cuda":
+                raise ValueError(f"{name} must be an int32 CUDA tensor of {nd} dimension(s)")
+            if t.device != q_start.device:
+                raise ValueError("q_start, seq_lens and table must be on one device")
+            if t.numel() > 1 and t.stride(-1) != 1 and t.shape[-1] > 1:
+                raise ValueError(f"{name} must be contiguous in its last dimension")
+        self.seqs = seq_lens.shape[0]
+        if q_start.shape[0] != self.seqs + 1 or table.shape[0] != self.seqs:
+            raise ValueError("q_start must be [seqs + 1] and table [seqs, pages]")
+        if type(max_q) is not int or not 0 <= max_q <= 1 << 28:
+            raise ValueError("max_q must be a nonnegative int")
+        if self.seqs > 1 << 24 or table.shape[1] > 1 << 24 or (self.seqs and table.shape[1] < 1):
+            raise ValueError("at most 2^24 sequences, and 1 to 2^24 pages of one")
+        self.q_start, self.seq_lens, self.table, self.max_q = q_start, seq_lens, table, max_q
+        self.device = q_start.device
+        stride = table.stride(0) if self.seqs > 1 else table.shape[1]
+        if stride < 0 or (self.seqs > 1 and stride < table.shape[1]):
+            raise ValueError("table rows must not overlap")
+        self._c = _lib.EvaKvBatch(self.seqs, 0, max_q, table.shape[1], stride, q_start.data_ptr(), seq_lens.data_ptr(),
+                                  table.data_ptr())
+
+    def _for(self, tokens):
+        if tokens > _INT32_MAX:
+            raise ValueError("too many token rows")
+        c = self._c
+        return _lib.EvaKvBatch(c.seqs, tokens, c.max_q, c.max_pages, c.table_stride, c.q_start, c.seq_lens, c.table)
+
+
+class PagedKVCache:
+    """One layer's keys and values in pages of 64 tokens, 8 bits each: codes e4m3, one scale 2^e (E8M0) for each 16 tokens
+    and head. (key_dim, value_dim) is (64, 64), (128, 128) or (192, 128).
+
+    k [pages, kv_heads, 64, key_dim], v [pages, kv_heads, value_dim, 64] (a dimension's tokens side by side), k_scale and
+    v_scale [pages, kv_heads, 4]; existing contiguous tensors may be given (float8 or uint8; scale bytes 1 .. 253)."""
+
+    def __init__(self, pages, kv_heads, key_dim, value_dim=None, *, device="cuda", k=None, v=None, k_scale=None, v_scale=None):
+        value_dim = key_dim if value_dim is None else value_dim
+        if (key_dim, value_dim) not in HEAD_DIMS:
+            raise ValueError(f"(key_dim, value_dim) must be one of {HEAD_DIMS}")
+        if type(pages) is not int or type(kv_heads) is not int or not 1 <= pages <= _INT32_MAX or not 1 <= kv_heads <= 65535:
+            raise ValueError("pages must be a positive int and kv_heads one in 1..65535")
+        self.device = _device(device)
+        self.lib = _lib.load()
+        self.pages, self.kv_heads, self.key_dim, self.value_dim = pages, kv_heads, key_dim, value_dim
+        self.k = self._buffer(k, (pages, kv_heads, PAGE, key_dim), _E4M3, "k")
+        self.v = self._buffer(v, (pages, kv_heads, value_dim, PAGE), _E4M3, "v")
+        self.k_scale = self._buffer(k_scale, (pages, kv_heads, PAGE // BLOCK), _E8M0, "k_scale")
+        self.v_scale = self._buffer(v_scale, (pages, kv_heads, PAGE // BLOCK), _E8M0, "v_scale")
+        self._status = torch.zeros(1, dtype=_I32, device=self.device)
+        self._c = _lib.EvaKvCache(pages, kv_heads, key_dim, value_dim, self.k.data_ptr(), self.v.data_ptr(),
+                                  self.k_scale.data_ptr(), self.v_scale.data_ptr(), self._status.data_ptr())
+        self._ref = ctypes.byref(self._c)
+
+    def _buffer(self, t, shape, dtype, name):
+        if t is None:
+            return torch.zeros(shape, dtype=_U8, device=self.device).view(dtype)
+        if (not isinstance(t, torch.Tensor) or t.device != self.device or tuple(t.shape) != shape or t.dtype not in (dtype, _U8)
+                or not t.is_contiguous() or t.data_ptr() % 16):
+            raise ValueError(f"{name} must be a contiguous {dtype} or uint8 {list(shape)} on {self.device}, 16-byte aligned")
+        return t.view(dtype)
+
+    def _batch(self, batch, tokens):
+        if not isinstance(batch, PagedBatch) or batch.device != self.device:
+            raise ValueError(f"batch must be a PagedBatch on {self.device}")
+        return batch._for(tokens)
+
+    def append(self, k, v, batch, *, rotary=None):
+        """Write the batch's new tokens: k [tokens, kv_heads, key_dim] rotated by each token's position in its sequence, and
+        v [tokens, kv_heads, value_dim] (BF16 or Half, any token and head strides), quantised. A block's scale is the smallest
+        power of two that fits its tokens; one that a later token raises has its older codes rescaled. A token with a
+        non-finite element gets a NaN key: the rows that see it become NaN, and no others."""
+        _rows(k, "k", self.device, (_BF16, _F16), self.kv_heads, self.key_dim)
+        _rows(v, "v", self.device, (k.dtype,), self.kv_heads, self.value_dim)
+        if v.shape[0] != k.shape[0]:
+            raise ValueError("k and v must have the same token rows")
+        if rotary is not None:
+            if not isinstance(rotary, Rotary) or rotary.device != self.device:
+                raise ValueError(f"rotary must be a Rotary on {self.device}")
+            if rotary.offset + rotary.dim > self.key_dim:
+                raise ValueError(f"the rotation ends at {rotary.offset + rotary.dim}, keys have {self.key_dim} dimensions")
+        b = self._batch(batch, k.shape[0])
+        k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (k, v))
+        (kt, kh), (vt, vh) = _strides(k), _strides(v)
+        with _on(self.device):
+            rc = self.lib.eva_kv_append(self._ref, ctypes.byref(b), None if rotary is None else ctypes.byref(rotary._c),
+                                        k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _DTYPE[k.dtype],
+                                        torch.cuda.current_stream(self.device).cuda_stream)
+        _lib.check(rc, "eva_kv_append")
+
+    def attend(self, q, batch, *, scale=None, window=0, out=None):
+        """softmax(scale q k^T) v of q [tokens, heads, key_dim] (BF16 or Half, already rotated) over the batch's sequences,
+        new tokens included: a row sees the tokens up to its own position, with window > 0 the last `window` of them.
+        heads is a multiple of kv_heads. Returns [tokens, heads, value_dim] of q's type; rows that see nothing are zero, rows behind
+        the last sequence are left as they were (in out; a new tensor has no values there)."""
+        _rows(q, "q", self.device, (_BF16, _F16), None, self.key_dim)
+        tokens, heads = q.shape[0], q.shape[1]
+        if heads < 1 or heads % self.kv_heads:
+            raise ValueError(f"heads must be a multiple of {self.kv_heads}")
+        if type(window) is not int or not 0 <= window <= _INT32_MAX:
+            raise ValueError("window must be a nonnegative int")
+        scale = self.key_dim ** -0.5 if scale is None else scale
+        if not isinstance(scale, (int, float)) or not 0 <= scale <= 3e38:
+            raise ValueError("scale must be a finite nonnegative number")
+        b = self._batch(batch, tokens)
+        st, sh = _strides(q)
+        if q.stride(2) != 1 or st % 8 or sh % 8 or q.data_ptr() % 16:
+            q = q.clone(memory_format=torch.contiguous_format)
+            st, sh = _strides(q)
+        if out is None:
+            out = torch.empty(tokens, heads, self.value_dim, dtype=q.dtype, device=self.device)
+        elif (not isinstance(out, torch.Tensor) or out.device != self.device or out.dtype != q.dtype or not out.is_contiguous()
+              or tuple(out.shape) != (tokens, heads, self.value_dim) or out.data_ptr() % 16):
+            raise ValueError(f"out must be a contiguous {q.dtype} [{tokens}, {heads}, {self.value_dim}] on {self.device}, 16-byte aligned")
+        elif _overlap(q, out):
+            raise ValueError("out must not overlap q")
+        with _on(self.device):
+            n = self.lib.eva_kv_attend_workspace(self._ref, ctypes.byref(b), heads)
+            if n == 0:
+                raise ValueError("unsupported batch")
+            ws = torch.empty(n, dtype=_U8, device=self.device)
+            rc = self.lib.eva_kv_attend(self._ref, ctypes.byref(b), q.data_ptr(), _DTYPE[q.dtype], heads, st, sh, float(scale),
+                                        window, ws.data_ptr(), n, out.data_ptr(),
+                                        torch.cuda.current_stream(self.device).cuda_stream)
+        _lib.check(rc, "eva_kv_attend")
+        return out
+
+    def values(self, pages):
+        """The keys [n, kv_heads, 64, key_dim] and values [n, kv_heads, 64, value_dim] that the pages (int64 [n]) hold, as floats."""
+        k = self.k[pages].to(_F32) * self.k_scale[pages].to(_F32).repeat_interleave(BLOCK, -1)[..., None]
+        v = self.v[pages].to(_F32) * self.v_scale[pages].to(_F32).repeat_interleave(BLOCK, -1)[..., None, :]
+        return k, v.transpose(2, 3)
+
+    def status(self) -> int:
+        """The device status bits (reads them back: synchronises the host)."""
+        return int(self._status.item())
+
+    def clear_status(self) -> None:
+        self._status.zero_()

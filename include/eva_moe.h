@@ -44,6 +44,7 @@ extern "C" {
 #define EVA_STATUS_BAD_EXPERT 1   /* a selected expert id is outside [0, n_local) or has a zero pointer */
 #define EVA_STATUS_TIMEOUT 2      /* a bounded device wait gave up (results of that call are invalid) */
 #define EVA_STATUS_CAPACITY 4     /* more rows than the workspace was sized for */
+#define EVA_STATUS_BAD_BATCH 8    /* paged cache: a page id outside the cache, or row starts / lengths outside the batch */
 
 /* router kinds */
 #define EVA_ROUTER_SOFTMAX 0       /* DeepSeek-V2-Lite greedy top-k over softmax probabilities */
@@ -288,6 +289,85 @@ int eva_ep_combine_peers(const EvaEpPeers* p, int32_t M, const int32_t* pos, con
  *   weight: [H] bf16 (weight_is_bf16 = 1) or fp16; h_out: bf16 [M][H] */
 int eva_rmsnorm_residual(int32_t H, int32_t M, float* resid, const float* add, const void* weight,
                          int32_t weight_is_bf16, float eps, void* h_out, void* stream);
+
+/* ---- attention between the MoE layers: rotary positions, paged 8-bit key/value cache ------------------
+ * The reference's attention half of a layer (runtime/ds41/model.py:566-937 `Attention`, rotary tails
+ * runtime/ds41/attn_cuda.py:22) keeps its cache in 4 bits behind an index; these operators give the
+ * layer stack plain causal attention over a paged 8-bit cache. Nothing here synchronises the host. */
+
+/* element types of activations (EVA_DTYPE_F16 and _BF16 are the values of x_is_bf16 above) */
+#define EVA_DTYPE_F16 0
+#define EVA_DTYPE_BF16 1
+#define EVA_DTYPE_F32 2
+
+/* Rotation of `dim` dimensions of a head from `offset` on, in pairs (i, i + dim / 2), or (2i, 2i + 1) when
+ * interleaved: (a, b) -> mscale * (a cos t - b sin t, b cos t + a sin t), t = position * frequency_i.
+ * turns: device uint64 [dim / 2], frequency_i / (2 pi) as a fraction of 2^64: position * turns modulo
+ * 2^64 is the exact fraction of a turn at any position. inverse: t -> -t (the rotation of gradients). */
+typedef struct EvaRotary {
+    int32_t dim, offset;       /* even */
+    int32_t interleaved, inverse;
+    float mscale;
+    int32_t reserved;
+    const uint64_t* turns;
+} EvaRotary;
+
+/* out = x rotated; x, out: [tokens][heads][head_dim] of `dtype` with strides in elements (last dimension
+ * contiguous). out may be x itself (same strides); else they must not overlap. positions: int32 or int64
+ * [tokens]. dim 0 copies. */
+int eva_rotary(const EvaRotary* rotary, const void* x, int32_t dtype, int32_t tokens, int32_t heads, int32_t head_dim,
+               int64_t x_token_stride, int64_t x_head_stride, const void* positions, int32_t positions_i64, void* out,
+               int64_t out_token_stride, int64_t out_head_stride, void* stream);
+
+#define EVA_KV_PAGE 64     /* tokens of a page */
+#define EVA_KV_BLOCK 16    /* tokens that share a scale */
+
+/* Paged cache of one layer: codes are e4m3, scales E8M0 (2^(byte - 127)), one per 16 tokens and head.
+ *   k: [pages][kv_heads][64][key_dim]; v: [pages][kv_heads][value_dim][64] (a dimension's tokens are
+ *   contiguous, as the second matrix product reads them); k_scale, v_scale: [pages][kv_heads][4]
+ * (key_dim, value_dim) is (64, 64), (128, 128) or (192, 128). k, v 16-byte, scales 4-byte aligned.
+ * status: device int32, EVA_STATUS_* bits are OR-ed into it. */
+typedef struct EvaKvCache {
+    int32_t pages, kv_heads, key_dim, value_dim;
+    void* k;
+    void* v;
+    void* k_scale;
+    void* v_scale;
+    int32_t* status;
+} EvaKvCache;
+
+/* A ragged batch: sequence b has token rows q_start[b] .. q_start[b + 1] - 1, which are the last ones of its
+ * seq_lens[b] tokens; its token t lies in page table[b * table_stride + t / 64]. max_q bounds the rows of
+ * one sequence. Rows at negative positions (more rows than tokens: padding) have no token. Row starts out
+ * of order or beyond `tokens`, more than max_q rows, lengths beyond max_pages pages and page ids outside the
+ * cache set EVA_STATUS_BAD_BATCH; what they name is neither read nor written. */
+typedef struct EvaKvBatch {
+    int32_t seqs, tokens, max_q, max_pages;
+    int64_t table_stride;
+    const int32_t* q_start;     /* device int32 [seqs + 1] */
+    const int32_t* seq_lens;    /* device int32 [seqs] */
+    const int32_t* table;       /* device int32 [seqs][table_stride] */
+} EvaKvBatch;
+
+/* Append: the new tokens' keys (rotated by their positions when rotary is not NULL) and values, quantised, into
+ * the pages. A block of 16 tokens has the smallest power of two that brings all its values into e4m3's range;
+ * when a later token raises it, the block's older codes are rescaled. A token of whose key or value an element
+ * is not finite gets a NaN key (its values: 0 there), so that exactly the rows that see it become NaN. Everything
+ * but the blocks' codes and scales stays as it was. No page may be appended to by two sequences of one call.
+ * k: [tokens][kv_heads][key_dim], v: [tokens][kv_heads][value_dim], F16 or BF16, strides in elements. */
+int eva_kv_append(const EvaKvCache* cache, const EvaKvBatch* batch, const EvaRotary* rotary, const void* k,
+                  int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                  int64_t v_head_stride, int32_t dtype, void* stream);
+
+/* Attention of the batch's rows over their sequences: row at position p sees tokens 0 .. p, with window > 0
+ * only the last `window` of them; out = softmax(scale q k^T) v, zero where nothing is seen. q: [tokens][heads]
+ * [key_dim], heads a multiple of kv_heads (query head h reads head h / (heads / kv_heads)); out: contiguous
+ * [tokens][heads][value_dim] of q's type (F16 or BF16). Rows behind the last sequence stay as they were.
+ * workspace: eva_kv_attend_workspace() bytes, 16-byte aligned, not shared by calls that may overlap. */
+size_t eva_kv_attend_workspace(const EvaKvCache* cache, const EvaKvBatch* batch, int32_t heads);
+int eva_kv_attend(const EvaKvCache* cache, const EvaKvBatch* batch, const void* q, int32_t dtype, int32_t heads,
+                  int64_t q_token_stride, int64_t q_head_stride, float scale, int32_t window, void* workspace,
+                  size_t workspace_bytes, void* out, void* stream);
 
 /* Library identification: sm arch the kernels were built for (100 for sm_100a). */
 int32_t eva_moe_arch(void);

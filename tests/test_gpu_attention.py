@@ -1,0 +1,515 @@
+"""Attention operators on a B200 against their 64-bit forms: rotary positions, the append into the paged 8-bit cache,
+attention over it, and the three together. Needs a GPU."""
+import math
+
+import pytest
+import torch
+
+from eva_b200 import _lib
+from eva_b200.attention import PagedBatch, PagedKVCache, Rotary
+from oracle import attention as A
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+# ---- rotary ---------------------------------------------------------------------------------------------------
+
+def _check_rotation(x, pos, rot, got, inverse=False):
+    """Angle: 2^-25 half turns (conversion of the fraction) is 1e-7; cosine and sine 1e-7 more, products and sum 1.2e-7 of
+    |a| + |b|; then the output's own rounding, half a step of its type. Far out the 64-bit angle itself is rounded: the
+    oracle's product by 2^-53 of it, the kernel's fraction of a turn by the division by 2 pi and that constant, 2^-53 each."""
+    ref = A.rotate(x.cpu(), pos.cpu(), rot.inv_freq, rot.mscale, rot.layout, rot.offset, inverse)
+    size = x.cpu().double().abs()
+    lo, hi = rot.offset, rot.offset + rot.dim
+    pair = size[..., lo:hi]
+    if rot.layout == "half":
+        both = (pair[..., :rot.dim // 2] + pair[..., rot.dim // 2:]).repeat(1, 1, 2)
+    else:
+        both = (pair[..., 0::2] + pair[..., 1::2]).repeat_interleave(2, -1)
+    tol = torch.zeros_like(ref)
+    far = float(pos.abs().max()) * max(rot.inv_freq) * 3 * 2.0**-53
+    tol[..., lo:hi] = (3.5e-7 + far) * abs(rot.mscale) * both + torch.finfo(x.dtype).eps / 2 * ref[..., lo:hi].abs() \
+        + torch.finfo(x.dtype).smallest_normal
+    err = (got.cpu().double() - ref).abs()
+    worst = float((err - tol).max())
+    assert worst <= 0, worst
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("tokens,heads,dim,rot,offset", [(1, 1, 64, 64, 0), (3, 5, 80, 40, 8), (70, 16, 192, 64, 128),
+                                                         (257, 3, 102, 6, 34), (9, 33, 128, 128, 0)])
+def test_rotary_matches_64_bits(layout, dtype, tokens, heads, dim, rot, offset):
+    g = torch.Generator(device=DEV).manual_seed(tokens)
+    x = torch.randn(tokens, heads, dim, device=DEV, generator=g).to(dtype)
+    pos = torch.randint(0, 1 << 21, (tokens,), device=DEV, generator=g)
+    r = Rotary(rot, layout=layout, offset=offset)
+    out = r.apply(x, pos)
+    _check_rotation(x, pos, r, out)
+    assert torch.equal(r.apply(x, pos.to(torch.int32)), out)
+    y = x.clone()
+    assert r.apply(y, pos, out=y) is y and torch.equal(y, out)
+    _check_rotation(x, pos, r, r.apply(x, pos, inverse=True), inverse=True)
+
+
+@pytest.mark.parametrize("scaling,kw", [("linear", dict(factor=8.0)), ("ntk", dict(factor=4.0)),
+                                        ("yarn", dict(factor=40.0)), ("yarn", dict(factor=40.0, mscale=1.0))])
+def test_rotary_scalings_at_far_positions(scaling, kw):
+    r = Rotary(64, layout="interleaved", offset=64, scaling=scaling, **kw)
+    x = torch.randn(40, 4, 128, device=DEV)
+    pos = torch.randint(2**31 - 1000, 2**33, (40,), device=DEV)
+    pos[0] = -5
+    _check_rotation(x, pos, r, r.apply(x, pos))
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rotary_strides_and_unaligned_rows(layout):
+    """Slices of a wider projection, heads and tokens exchanged, a last dimension that is not contiguous, odd offsets."""
+    r = Rotary(32, layout=layout, offset=2)
+    pos = torch.arange(7, 18, device=DEV)
+    wide = torch.randn(11, 500, device=DEV).to(BF16)
+    for x in (wide[:, 3:3 + 6 * 48].unflatten(1, (6, 48)), wide[:, :6 * 48].unflatten(1, (6, 48)),
+              wide[:, :288].unflatten(1, (6, 48)).transpose(0, 1).contiguous().transpose(0, 1),
+              wide[:, :288].unflatten(1, (48, 6)).transpose(1, 2), wide[:, None, 1:49], wide[:, None, :48].expand(11, 4, 48)):
+        _check_rotation(x, pos, r, r.apply(x, pos))
+    out = torch.zeros(11, 6, 64, device=DEV, dtype=BF16)
+    x = wide[:, :288].unflatten(1, (6, 48))
+    r.apply(x, pos, out=out[..., 8:56])
+    _check_rotation(x, pos, r, out[..., 8:56])
+    assert not out[..., :8].any() and not out[..., 56:].any()
+
+
+def test_rotary_inverse_is_the_gradient():
+    """<w, R x> is linear in x: its gradient R^T w is the inverse rotation; against differences, exact but for rounding."""
+    r = Rotary(48, layout="half", offset=4, scaling="yarn", factor=4.0)
+    x, w = (torch.randn(5, 3, 64, device=DEV) for _ in range(2))
+    pos = torch.tensor([0, 1, 77, 4096, 300000], device=DEV)
+    grad = r.apply(w, pos, inverse=True)
+    for t, h, d in ((0, 0, 0), (1, 2, 4), (2, 1, 28), (4, 2, 51), (3, 0, 52), (4, 1, 63)):
+        e = torch.zeros_like(x)
+        e[t, h, d] = 1.0
+        diff = float((w.double() * (r.apply(x + e, pos).double() - r.apply(x - e, pos).double())).sum() / 2)
+        # x +- e and the rotation are rounded: 64 terms, each within 3.5e-7 * 2 * 5
+        assert abs(diff - float(grad[t, h, d])) < 5e-5, (t, h, d)
+
+
+def test_rotary_of_nothing():
+    r = Rotary(32, layout="half")
+    x = torch.empty(0, 4, 64, device=DEV)
+    assert r.apply(x, torch.empty(0, dtype=torch.int64, device=DEV)).shape == (0, 4, 64)
+
+
+# ---- paged cache ----------------------------------------------------------------------------------------------
+
+class Setup:
+    """A cache full of old bytes (NaN codes among them), a shuffled page table and a ragged batch."""
+
+    def __init__(self, dims, kv_heads, new, lens, seed=0, spare=2, rows_behind=0):
+        self.g = torch.Generator().manual_seed(seed)
+        dk, dv = dims
+        each = [-(-n // A.PAGE) for n in lens]
+        pages = sum(each) + spare
+        order = torch.randperm(pages, generator=self.g).tolist()
+        self.table = []
+        for n in each:
+            self.table.append(order[:n])
+            order = order[n:]
+        self.unused = order
+        width = max(each + [1])
+        self.new, self.lens = list(new), list(lens)
+        self.start = [0]
+        for n in new:
+            self.start.append(self.start[-1] + n)
+        self.T = self.start[-1] + rows_behind
+        byte = lambda *s: torch.randint(0, 256, s, generator=self.g, dtype=torch.uint8)   # noqa: E731
+        self.host = {"k": byte(pages, kv_heads, 64, dk).view(A.E4M3), "v": byte(pages, kv_heads, dv, 64).view(A.E4M3),
+                     "ks": torch.randint(-12, 2, (pages, kv_heads, 4), generator=self.g),
+                     "vs": torch.randint(-12, 2, (pages, kv_heads, 4), generator=self.g)}
+        t = torch.full((len(lens), width), -1, dtype=torch.int32)
+        for b, p in enumerate(self.table):
+            t[b, :len(p)] = torch.tensor(p, dtype=torch.int32)
+        self.cache = PagedKVCache(pages, kv_heads, dk, dv, k=self.host["k"].to(DEV), v=self.host["v"].to(DEV),
+                                  k_scale=self.bytes_of("ks"), v_scale=self.bytes_of("vs"))
+        self.batch = PagedBatch(torch.tensor(self.start, dtype=torch.int32, device=DEV),
+                                torch.tensor(lens, dtype=torch.int32, device=DEV), t.to(DEV), max([*new, 0]))
+
+    def bytes_of(self, name):
+        return (self.host[name] + 127).to(torch.uint8).to(DEV)
+
+    def fill(self, scale=1.0):
+        """Every token of the sequences gets a finite key and value (what an append before would have left)."""
+        for name, sn in (("k", "ks"), ("v", "vs")):
+            for b, n in enumerate(self.lens):
+                for i, p in enumerate(self.table[b]):
+                    m = min(64, n - 64 * i)
+                    c = self.host[name][p] if name == "k" else self.host[name][p].transpose(1, 2)
+                    vals = (torch.randn(c.shape[0], m, c.shape[2], generator=self.g) * 120).clamp(-448, 448)
+                    c.view(torch.uint8)[:, :m] = vals.to(A.E4M3).view(torch.uint8)
+                    self.host[sn][p] = torch.randint(-9, -5, self.host[sn][p].shape, generator=self.g)
+            getattr(self.cache, name).view(torch.uint8).copy_(self.host[name].view(torch.uint8))
+            getattr(self.cache, name + "_scale").view(torch.uint8).copy_((self.host[sn] + 127).to(torch.uint8))
+        return self
+
+    def rows(self, heads, dim, dtype, scale=1.0):
+        return (torch.randn(self.T, heads, dim, generator=self.g) * scale).to(dtype)
+
+
+DIMS = [(64, 64), (128, 128), (192, 128)]
+# new tokens and lengths: one token, block and page borders, an empty sequence, a padding row, contexts that end inside blocks
+BATCHES = [([1], [1]), ([1, 1, 1, 1], [16, 17, 64, 65]), ([5, 0, 1, 33], [5, 70, 0, 130]), ([130], [130]),
+           ([64, 1, 15], [100, 49, 300]), ([3, 20], [2, 20])]
+
+
+def _same_bytes(got, want, name):
+    g, w = got.cpu().view(torch.uint8), want.view(torch.uint8)
+    nan = ((g & 0x7f) == 0x7f) & ((w & 0x7f) == 0x7f)
+    assert bool(((g == w) | nan).all()), (name, int(((g != w) & ~nan).sum()))
+
+
+@pytest.mark.parametrize("dims", DIMS)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("new,lens", BATCHES)
+def test_append_without_rotation_is_exact(dims, dtype, new, lens):
+    s = Setup(dims, 3, new, lens, seed=len(lens))
+    k, v = s.rows(3, dims[0], dtype, 3.0), s.rows(3, dims[1], dtype, 0.02)
+    s.cache.append(k.to(DEV), v.to(DEV), s.batch)
+    A.append(s.host, k.double(), v.double(), s.start, s.lens, s.table)
+    for name in ("k", "v"):
+        _same_bytes(getattr(s.cache, name), s.host[name], name)
+        assert torch.equal(getattr(s.cache, name + "_scale").view(torch.uint8), s.bytes_of(name + "s"))
+    assert s.cache.status() == 0
+
+
+@pytest.mark.parametrize("dims,layout,rot,offset", [((64, 64), "half", 64, 0), ((128, 128), "interleaved", 44, 84),
+                                                    ((128, 128), "half", 128, 0), ((192, 128), "interleaved", 64, 128),
+                                                    ((192, 128), "half", 30, 2)])
+def test_append_rotates_by_the_position_in_the_sequence(dims, layout, rot, offset):
+    """Angle error 1e-7 and the fast functions' 5e-7 before the rounding to e4m3 (half a step: 2^-4 of the value, or
+    2^-10 of the scale below its normal range); the scale is the exact one unless the largest key lies within that of a power of two."""
+    new, lens = [40, 1, 7], [40, 100, 200007]
+    s = Setup(dims, 2, new, lens, seed=rot)
+    r = Rotary(rot, layout=layout, offset=offset, scaling="yarn", factor=8.0)
+    k, v = s.rows(2, dims[0], BF16, 2.0), s.rows(2, dims[1], BF16)
+    pos = torch.cat([torch.arange(n - m, n) for m, n in zip(new, lens)])
+    kr = A.rotate(k, pos, r.inv_freq, r.mscale, layout, offset)
+    ek, ev = A.append(s.host, kr, v.double(), s.start, s.lens, s.table)
+    s.cache.append(k.to(DEV), v.to(DEV), s.batch, rotary=r)
+    _same_bytes(s.cache.v, s.host["v"], "v")
+    codes, e = s.cache.k.cpu().float(), s.cache.k_scale.cpu().view(torch.uint8).int() - 127
+    for (p, h, t), want in ek.items():
+        two = 2.0 ** int(e[p, h, t // 16])
+        tol = want.abs() * 2.0**-4 + two * 2.0**-10 + 1e-6 * r.mscale * k.abs().max().double()
+        assert bool(((codes[p, h, t].double() * two - want).abs() <= tol).all())
+        assert abs(int(e[p, h, t // 16]) - int(s.host["ks"][p, h, t // 16])) <= 1
+    moved = (e != s.host["ks"].int()).float().mean()
+    assert float(moved) < 0.01
+
+
+def test_append_step_by_step_equals_one_append():
+    """The scale of a block does not depend on how its tokens arrive; codes may differ only where a rescaled one is subnormal."""
+    n = 150
+    a, b = Setup((128, 128), 2, [n], [n], seed=5), Setup((128, 128), 2, [n], [n], seed=5)
+    k, v = a.rows(2, 128, BF16), a.rows(2, 128, BF16)
+    k *= torch.rand(n, 1, 1, generator=a.g).to(BF16) * 30
+    a.cache.append(k.to(DEV), v.to(DEV), a.batch)
+    at = 0
+    for step in (1, 1, 13, 2, 40, 7, 1, 16, 16, 53):
+        i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)   # noqa: E731
+        batch = PagedBatch(i32(0, step), i32(at + step), b.batch.table, step)
+        b.cache.append(k[at:at + step].to(DEV), v[at:at + step].to(DEV), batch)
+        at += step
+    assert at == n
+    pages = torch.tensor(a.table[0], device=DEV)
+    for name in ("k_scale", "v_scale"):
+        assert torch.equal(getattr(a.cache, name).view(torch.uint8)[pages, :], getattr(b.cache, name).view(torch.uint8)[pages, :])
+    for x, y, sc in zip(a.cache.values(pages), b.cache.values(pages), (a.cache.k_scale, a.cache.v_scale)):
+        x, y = x.transpose(1, 2).flatten(0, 1)[:n], y.transpose(1, 2).flatten(0, 1)[:n]
+        step = sc[pages].float().repeat_interleave(16, -1).transpose(1, 2).flatten(0, 1)[:n, :, None] * 2.0**-9
+        assert bool(((x - y).abs() <= step).all())
+
+
+def test_append_of_values_that_are_not_finite():
+    """Such a token gets a NaN key; its block's other tokens and scales are as if it were not there, and so are its finite values."""
+    s = Setup((64, 64), 2, [40], [70], seed=2)
+    k, v = s.rows(2, 64, BF16), s.rows(2, 64, BF16)
+    k[3, 0, 5], k[9, 1, 63], v[20, 0, 1], v[21, 1, 0] = math.inf, math.nan, -math.inf, math.nan
+    s.cache.append(k.to(DEV), v.to(DEV), s.batch)
+    A.append(s.host, k.double(), v.double(), s.start, s.lens, s.table)
+    for name in ("k", "v"):
+        _same_bytes(getattr(s.cache, name), s.host[name], name)
+        assert torch.equal(getattr(s.cache, name + "_scale").view(torch.uint8), s.bytes_of(name + "s"))
+    nan = s.cache.k.float().isnan()
+    assert bool(nan[s.table[0][0], 0, 30 + 3].all()) and bool(nan[s.table[0][0], 1, 30 + 9].all())
+
+
+def test_append_extremes_of_the_range():
+    """Zero blocks, the smallest and the largest values of the input types."""
+    for dtype, big, tiny in ((BF16, 3.0e38, 1e-38), (F16, 65504.0, 6e-8)):
+        s = Setup((64, 64), 1, [64], [64], seed=3)
+        k, v = s.rows(1, 64, dtype), s.rows(1, 64, dtype)
+        k[:16], k[16:32], k[32:48] = 0.0, big, tiny
+        v[:16], v[16:32], v[32:48] = tiny, 0.0, -big
+        s.cache.append(k.to(DEV), v.to(DEV), s.batch)
+        A.append(s.host, k.double(), v.double(), s.start, s.lens, s.table)
+        for name in ("k", "v"):
+            _same_bytes(getattr(s.cache, name), s.host[name], name)
+
+
+# ---- attention ------------------------------------------------------------------------------------------------
+
+def _check_attention(s, q, out, scale, window=0, rows=None):
+    """Scores: key_dim products accumulated in 32 bits with truncation, 2^-23 of the sum of their sizes each at most; a query in
+    8-bit parts drops 2^-18 of its largest element; weights rounded to 16 bits (2^-11) and the output to its type."""
+    ref, mean_abs, size, loud = A.attend(s.host, q.cpu(), s.start, s.lens, s.table, scale, window)
+    delta = q.shape[2] * 2.0**-23 * size + 2.0**-18 * loud + 2.0**-20
+    tol = torch.finfo(q.dtype).eps / 2 * ref.abs() + mean_abs * (2.0**-11 + 2 * delta) + torch.finfo(q.dtype).smallest_normal
+    got = out.cpu().double()
+    n = s.start[-1]
+    err = (got - ref)[:n].abs()
+    nan = ref[:n].isnan()
+    assert torch.equal(got[:n].isnan(), nan)
+    assert bool((err <= tol[:n])[~nan].all()), float((err - tol[:n])[~nan].max())
+
+
+HEADS = [(1, 1), (4, 2), (6, 2), (8, 1), (15, 3)]
+
+
+@pytest.mark.parametrize("dims", DIMS)
+@pytest.mark.parametrize("heads,kv_heads", HEADS)
+@pytest.mark.parametrize("new,lens", BATCHES)
+def test_attention_matches_64_bits(dims, heads, kv_heads, new, lens):
+    s = Setup(dims, kv_heads, new, lens, seed=heads).fill()
+    q = s.rows(heads, dims[0], BF16 if heads % 2 else F16, 2.0).to(DEV)
+    _check_attention(s, q, s.cache.attend(q, s.batch), dims[0] ** -0.5)
+    assert s.cache.status() == 0
+
+
+@pytest.mark.parametrize("window", [1, 16, 50, 64, 129, 1000])
+@pytest.mark.parametrize("new,lens", [([1, 1, 1], [10, 129, 700]), ([90, 3], [300, 40]), ([200], [200])])
+def test_attention_within_a_window(window, new, lens):
+    s = Setup((128, 128), 2, new, lens, seed=window).fill()
+    q = s.rows(6, 128, BF16, 2.0).to(DEV)
+    _check_attention(s, q, s.cache.attend(q, s.batch, window=window, scale=0.2), 0.2, window)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("new,lens", [([1, 1], [3000, 77]), ([7], [1025]), ([150, 40], [1500, 40])])
+def test_attention_over_longer_caches(dtype, new, lens):
+    s = Setup((128, 128), 2, new, lens, seed=11).fill()
+    q = s.rows(8, 128, dtype, 3.0).to(DEV)
+    _check_attention(s, q, s.cache.attend(q, s.batch), 128 ** -0.5)
+
+
+@pytest.mark.parametrize("new,lens", [([1], [500]), ([100], [100])])
+@pytest.mark.parametrize("size", [1e-30, 1e-3, 1e4, 1e30])
+def test_attention_of_very_large_and_small_queries(size, new, lens):
+    """Softmax over equal scores, and over scores so far apart that one token has all the weight."""
+    s = Setup((64, 64), 1, new, lens, seed=4).fill()
+    q = s.rows(2, 64, BF16, size).to(DEV)
+    out = s.cache.attend(q, s.batch)
+    if size <= 1e-3:
+        _check_attention(s, q, out, 0.125)
+    else:
+        ref, _, _, _ = A.attend(s.host, q.cpu(), s.start, s.lens, s.table, 0.125)
+        # the largest score wins unless two lie within the scores' own error: bound by the values' range
+        assert bool(out.isfinite().all()) and float((out.cpu().double() - ref).abs().median()) < 2.0**-8
+
+
+def test_attention_keeps_rows_behind_the_last_sequence():
+    for new, lens in (([1, 1], [30, 40]), ([70, 20], [100, 20])):
+        s = Setup((64, 64), 2, new, lens, rows_behind=5).fill()
+        q = s.rows(4, 64, BF16).to(DEV)
+        out = torch.full((s.T, 4, 64), 7.0, dtype=BF16, device=DEV)
+        assert s.cache.attend(q, s.batch, out=out) is out
+        assert bool((out[s.start[-1]:] == 7).all())
+        _check_attention(s, q, out, 0.125)
+
+
+@pytest.mark.parametrize("new,lens", [([1], [90]), ([90], [90])])
+def test_a_nan_key_reaches_exactly_the_rows_that_see_it(new, lens):
+    s = Setup((128, 128), 2, new, lens).fill()
+    for t in (80, 89):
+        s.host["k"].view(torch.uint8)[s.table[0][t // 64], 1, t % 64] = 0x7f
+    s.cache.k.view(torch.uint8).copy_(s.host["k"].view(torch.uint8))
+    q = s.rows(4, 128, BF16).to(DEV)
+    out = s.cache.attend(q, s.batch)
+    _check_attention(s, q, out, 128 ** -0.5)
+    if new[0] > 1:
+        assert not out[:80].isnan().any() and bool(out[80:, 2:].isnan().all()) and not out[:, :2].isnan().any()
+
+
+@pytest.mark.parametrize("new,lens", [([1, 1], [90, 90]), ([90, 30], [90, 70])])
+def test_queries_that_are_not_finite_stay_in_their_rows(new, lens):
+    s = Setup((64, 64), 2, new, lens).fill()
+    q = s.rows(4, 64, BF16)
+    q[0, 1, 3], q[s.start[1], 2, 0] = math.nan, math.inf
+    out = s.cache.attend(q.to(DEV), s.batch)
+    assert bool(out[0, 1].isnan().all()) and bool(out[s.start[1], 2].isnan().all())
+    assert int(out.isnan().sum()) == 2 * 64
+
+
+def test_attention_strided_queries():
+    s = Setup((128, 128), 2, [20, 1], [100, 30]).fill()
+    wide = torch.randn(s.T, 900, device=DEV).to(BF16)
+    for q in (wide[:, :512].unflatten(1, (4, 128)), wide[:, 4:516].unflatten(1, (4, 128)),
+              wide[:, :512].unflatten(1, (128, 4)).transpose(1, 2), wide[:, None, :128].expand(s.T, 4, 128)):
+        _check_attention(s, q, s.cache.attend(q, s.batch), 128 ** -0.5)
+
+
+def test_repeated_calls_give_the_same_bits():
+    for new, lens in (([1] * 9, [50, 3000, 7, 700, 64, 1, 129, 2000, 333]), ([300, 70], [2000, 70])):
+        s = Setup((128, 128), 2, new, lens).fill()
+        q = s.rows(8, 128, BF16).to(DEV)
+        first = s.cache.attend(q, s.batch)
+        for _ in range(3):
+            assert torch.equal(first, s.cache.attend(q, s.batch))
+
+
+# ---- the three together, streams, graphs, refusals ------------------------------------------------------------
+
+@pytest.mark.parametrize("dims,layout", [((128, 128), "half"), ((192, 128), "interleaved")])
+def test_a_conversation_of_prompt_and_steps(dims, layout):
+    """Append and attend a prompt, a second piece, then single tokens, as one cache would be used."""
+    total, kvh, heads = 150, 2, 6
+    s = Setup(dims, kvh, [total], [total], seed=8)
+    rot = 64
+    r = Rotary(rot, layout=layout, offset=dims[0] - rot)
+    k, v, q = s.rows(kvh, dims[0], BF16), s.rows(kvh, dims[1], BF16), s.rows(heads, dims[0], BF16, 2.0)
+    pos = torch.arange(total)
+    qr = r.apply(q.to(DEV), pos.to(DEV))
+    at = 0
+    for n in (70, 37, 1, 1, 2, 1):
+        i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)   # noqa: E731
+        batch = PagedBatch(i32(0, n), i32(at + n), s.batch.table, n)
+        s.cache.append(k[at:at + n].to(DEV), v[at:at + n].to(DEV), batch, rotary=r)
+        out = s.cache.attend(qr[at:at + n], batch)
+        # the oracle reads the codes that the cache holds: the append has its own tests
+        for name, sn in (("k", "ks"), ("v", "vs")):
+            s.host[name] = getattr(s.cache, name).cpu()
+            s.host[sn] = getattr(s.cache, name + "_scale").cpu().view(torch.uint8).int() - 127
+        s.start, s.lens = [0, n], [at + n]
+        _check_attention(s, qr[at:at + n], out, dims[0] ** -0.5)
+        at += n
+    assert s.cache.status() == 0
+
+
+def test_graph_replay_with_new_contents():
+    """A captured step of padded batch size: rotate, append, attend; replayed as lengths grow, one slot empty."""
+    lens = [63, 0, 130]
+    a, b = Setup((64, 64), 2, [1, 1, 1], [l + 8 for l in lens], seed=6), Setup((64, 64), 2, [1, 1, 1], [l + 8 for l in lens], seed=6)
+    a.fill(), b.fill()
+    r = Rotary(64, layout="half")
+    buf = [torch.zeros(3, h, 64, dtype=BF16, device=DEV) for h in (4, 2, 2)]
+    pos = torch.zeros(3, dtype=torch.int64, device=DEV)
+
+    def step(s):
+        q = r.apply(buf[0], pos)
+        s.cache.append(buf[1], buf[2], s.batch, rotary=r)
+        return s.cache.attend(q, s.batch)
+
+    zero = torch.zeros(3, dtype=torch.int32, device=DEV)
+    a.batch.seq_lens.copy_(zero)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(a)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(a)
+    for i in range(1, 5):
+        now = torch.tensor([lens[0] + i, 0, lens[2] + i], dtype=torch.int32, device=DEV)
+        for s in (a, b):
+            s.batch.seq_lens.copy_(now)
+        pos.copy_((now - 1).clamp(min=0))
+        for t in buf:
+            t.normal_()
+        graph.replay()
+        want = step(b)
+        assert torch.equal(out, want) and not out[1].any()
+        assert torch.equal(a.cache.k.view(torch.uint8), b.cache.k.view(torch.uint8))
+        assert torch.equal(a.cache.v.view(torch.uint8), b.cache.v.view(torch.uint8))
+    assert a.cache.status() == 0
+
+
+def test_two_streams_at_once():
+    """Two attentions over one cache on two streams: their workspaces are their own."""
+    s = Setup((128, 128), 2, [1] * 6, [4000, 3000, 20, 700, 1, 2500]).fill()
+    q1, q2 = (s.rows(8, 128, BF16).to(DEV) for _ in range(2))
+    want = [s.cache.attend(q, s.batch) for q in (q1, q2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i, q in enumerate((q1, q2)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(s.cache.attend(q, s.batch))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+@pytest.mark.parametrize("new,lens", [([1, 1], [100, 200]), ([70, 40], [100, 200])])
+def test_a_batch_that_does_not_fit_is_flagged_and_left_out(new, lens):
+    """Page ids outside the cache, lengths beyond the table and row starts beyond the rows are bounded before any access
+    (the index arithmetic has host tests): a status bit, no fault, and the other sequences' results stand."""
+    s = Setup((64, 64), 2, new, lens).fill()
+    q = s.rows(4, 64, BF16).to(DEV)
+    good = s.cache.attend(q, s.batch)
+    before = s.cache.k.view(torch.uint8).clone()
+    k = torch.zeros(s.T, 2, 64, dtype=BF16, device=DEV)
+    for broken in ("page", "negative", "length", "rows", "order"):
+        t, sl, qs = s.batch.table.clone(), s.batch.seq_lens.clone(), s.batch.q_start.clone()
+        if broken == "page":
+            t[1, :] = s.cache.pages
+        elif broken == "negative":
+            t[1, :] = -7
+        elif broken == "length":
+            sl[1] = t.shape[1] * 64 + 1
+        elif broken == "rows":
+            qs[2] = s.T + 1
+        else:
+            qs[2] = qs[1] - 1
+        bad = PagedBatch(qs, sl, t, max(new))
+        out = s.cache.attend(q, bad)
+        assert s.cache.status() == _lib.STATUS_BAD_BATCH, broken
+        assert torch.equal(out[:s.start[1]], good[:s.start[1]]), broken
+        s.cache.clear_status()
+        sl[0] = 0
+        s.cache.append(k, k, PagedBatch(qs, sl, t, max(new)))
+        assert s.cache.status() == _lib.STATUS_BAD_BATCH, broken
+        assert torch.equal(before, s.cache.k.view(torch.uint8)), broken
+        s.cache.clear_status()
+
+
+def test_refusals():
+    s = Setup((64, 64), 2, [1, 1], [10, 20]).fill()
+    q, k = s.rows(4, 64, BF16).to(DEV), s.rows(2, 64, BF16).to(DEV)
+    r = Rotary(64, layout="half")
+    bad = [
+        lambda: PagedKVCache(4, 2, 96), lambda: PagedKVCache(0, 2, 64), lambda: PagedKVCache(4, 2, 128, 64),
+        lambda: PagedKVCache(4, 2, 64, k=torch.zeros(4, 2, 64, 64, device=DEV)),
+        lambda: s.cache.attend(q.float(), s.batch), lambda: s.cache.attend(q[:, :3], s.batch),
+        lambda: s.cache.attend(q[..., :32], s.batch), lambda: s.cache.attend(q.cpu(), s.batch),
+        lambda: s.cache.attend(q, s.batch, window=-1), lambda: s.cache.attend(q, s.batch, window=1.5),
+        lambda: s.cache.attend(q, s.batch, scale=math.nan), lambda: s.cache.attend(q, s.batch, scale=-1.0),
+        lambda: s.cache.attend(q, None), lambda: s.cache.attend(q, s.batch, out=q),
+        lambda: s.cache.attend(q, s.batch, out=torch.empty(2, 4, 64, device=DEV)),
+        lambda: s.cache.append(k, k.half(), s.batch), lambda: s.cache.append(k[:1], k, s.batch),
+        lambda: s.cache.append(q, q, s.batch), lambda: s.cache.append(k, k, s.batch, rotary=Rotary(128)),
+        lambda: s.cache.append(k, k, s.batch, rotary=3),
+        lambda: PagedBatch(s.batch.q_start, s.batch.seq_lens, s.batch.table[:1], 1),
+        lambda: PagedBatch(s.batch.q_start.long(), s.batch.seq_lens, s.batch.table, 1),
+        lambda: PagedBatch(s.batch.q_start.cpu(), s.batch.seq_lens, s.batch.table, 1),
+        lambda: PagedBatch(s.batch.q_start, s.batch.seq_lens, s.batch.table, -1),
+        lambda: r.apply(q, torch.zeros(2, device=DEV)), lambda: r.apply(q, torch.zeros(3, dtype=torch.int64, device=DEV)),
+        lambda: r.apply(q[..., :32], torch.zeros(2, dtype=torch.int64, device=DEV)),
+        lambda: r.apply(q, torch.zeros(2, dtype=torch.int64, device=DEV), out=q[:, :, :].transpose(0, 1)),
+        lambda: r.apply(q.double(), torch.zeros(2, dtype=torch.int64, device=DEV)),
+        lambda: r.apply(q, torch.zeros(2, dtype=torch.int64, device=DEV), out=q[:1].expand(2, 4, 64)),
+    ]
+    for i, f in enumerate(bad):
+        with pytest.raises(ValueError):
+            f()
+            pytest.fail(f"case {i} was accepted")
