@@ -1,0 +1,49 @@
+// Shared by the attention kernels over the paged cache.
+#pragma once
+
+#include "kv.cuh"
+
+namespace eva {
+
+constexpr int COMBINE_THREADS = 512;
+
+struct AttendArgs {
+    EvaKvCache c;
+    EvaKvBatch b;
+    const void* q;
+    void* out;
+    int64_t qt, qh;        // strides of q, elements
+    int heads, group, window;
+    float scale;           // times log2(e): the softmax's exponentials are powers of two
+    int part_rows;         // rows of a partial sum
+    int4* heads_of;        // [pieces]: item that begins in a piece and goes on {sequence, head, last piece}, -1: none
+    float* part;           // [pieces][2] partial sums
+};
+
+template <typename T> __device__ __forceinline__ float2 two_floats(uint32_t bits);
+template <> __device__ __forceinline__ float2 two_floats<__nv_bfloat16>(uint32_t bits)
+{
+    return make_float2(__uint_as_float(bits << 16), __uint_as_float(bits & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 two_floats<__half>(uint32_t bits)
+{
+    return __half22float2(*reinterpret_cast<const __half2*>(&bits));
+}
+
+template <typename T> __device__ __forceinline__ uint32_t two_bits(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t two_bits<__nv_bfloat16>(float lo, float hi)
+{
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t two_bits<__half>(float lo, float hi)
+{
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <typename T> __device__ __forceinline__ T one_of(float v);
+template <> __device__ __forceinline__ __nv_bfloat16 one_of(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half one_of(float v) { return __float2half_rn(v); }
+
+}  // namespace eva
