@@ -15,8 +15,9 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libeva_moe.so"
 SOURCES = ["capi.cu", "routing.cu", "router_tc.cu", "experts.cu", "prefill.cu", "noalloc.cu", "ep.cu", "stack.cu",
-           "decode_bench.cu", "residency.cu", "rotary.cu", "kv_append.cu", "kv_attend.cu"]
-HEADERS = ["common.cuh", "internal.h", "tc.cuh", "decode_tc.cuh", "kv.cuh"]
+           "decode_bench.cu", "residency.cu", "rotary.cu", "kv_append.cu", "kv_attend.cu",
+           "kv_prompt.cu"]
+HEADERS = ["common.cuh", "internal.h", "tc.cuh", "decode_tc.cuh", "kv.cuh", "kv_attend.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -47,27 +47,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// two e4m3 codes (the low 16 bits) as two halves, exact
-__device__ __forceinline__ uint32_t e4m3_halves(uint32_t two)
-{
-    uint32_t r;
-    asm("{\n .reg .b16 lo;\n cvt.u16.u32 lo, %1;\n cvt.rn.f16x2.e4m3x2 %0, lo;\n}\n" : "=r"(r) : "r"(two));
-    return r;
-}
-
-__device__ __forceinline__ uint32_t half2_bits(float lo, float hi)
-{
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // Tiles of one head of a sequence: the pages from the first token that its first row sees to its last one. A sequence with
 // rows but no token has one (empty) tile, so that its rows are written.
 __device__ __forceinline__ int dec_tiles(const KvSeq& s, int window, int* first)
@@ -478,87 +457,6 @@ template <typename T> static cudaError_t decode_typed(const AttendArgs& p, int p
     return decode_launch<192, 128, T>(p, pieces, st);
 }
 
-constexpr int ATT_WARPS = 4;
-
-__device__ __forceinline__ float e4m3_up(uint32_t byte)
-{
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
-}
-
-template <int DK, int DV, typename T>
-__global__ void __launch_bounds__(ATT_WARPS * 32) kv_attend_kernel(const AttendArgs p)
-{
-    __shared__ float qs[ATT_WARPS][DK];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t w = static_cast<int64_t>(blockIdx.x) * ATT_WARPS + warp;
-    const int64_t bi = w / p.heads;
-    const int head = static_cast<int>(w - bi * p.heads), kvh = head / p.group;
-    const int b = static_cast<int>(bi / p.b.max_q), i = static_cast<int>(bi - static_cast<int64_t>(b) * p.b.max_q);
-    if (b >= p.b.seqs) return;
-    const KvSeq s = kv_seq(p.b, b, p.c.status);
-    if (i >= s.n) return;
-    const int64_t row = s.row0 + i;
-    for (int d = lane; d < DK; d += 32) {
-        const int64_t at = row * p.qt + head * p.qh + d;
-        qs[warp][d] = static_cast<float>(static_cast<const T*>(p.q)[at]);
-    }
-    __syncwarp();
-    const int pos = s.ctx + i, end = pos + 1, begin = p.window > 0 ? max(0, end - p.window) : 0;
-    float m = -INFINITY, l = 0.0f, o[DV / 32] = {};
-    for (int t0 = begin & ~31; t0 < end; t0 += 32) {
-        const int page = kv_page(p.c, p.b, b, t0 / KV_PAGE, p.c.status);
-        if (page < 0) continue;
-        const int64_t ph = static_cast<int64_t>(page) * p.c.kv_heads + kvh;
-        const int t = t0 + lane, in = t0 % KV_PAGE;
-        const uint8_t* kr = static_cast<const uint8_t*>(p.c.k) + (ph * KV_PAGE + in + lane) * DK;
-        const uint8_t* ksc = static_cast<const uint8_t*>(p.c.k_scale) + ph * KV_PAGE_BLOCKS + in / KV_BLOCK;
-        const uint8_t* vsc = static_cast<const uint8_t*>(p.c.v_scale) + ph * KV_PAGE_BLOCKS + in / KV_BLOCK;
-        float x = 0.0f;
-        for (int d = 0; d < DK; ++d) x = fmaf(qs[warp][d], e4m3_up(kr[d]), x);
-        x *= kv_scale(ksc[lane / KV_BLOCK]) * p.scale;
-        const bool seen = t >= begin && t < end;
-        x = seen ? x : -INFINITY;
-        float mx = x;
-#pragma unroll
-        for (int sft = 16; sft > 0; sft >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sft));
-        const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.0f : mn, down = exp2f(m - ref);
-        const float e = seen ? exp2f(x - ref) : 0.0f;
-        m = mn;
-        l = l * down + e;
-        const float ev = e * kv_scale(vsc[lane / KV_BLOCK]);
-        const uint8_t* vr = static_cast<const uint8_t*>(p.c.v) + ph * KV_PAGE * DV + in;
-#pragma unroll
-        for (int j = 0; j < DV / 32; ++j) o[j] *= down;
-        for (int u = 0; u < 32; ++u) {
-            const float pu = __shfl_sync(0xffffffffu, ev, u);
-            if (t0 + u < begin || t0 + u >= end) continue;
-#pragma unroll
-            for (int j = 0; j < DV / 32; ++j) o[j] = fmaf(pu, e4m3_up(vr[(lane + 32 * j) * KV_PAGE + u]), o[j]);
-        }
-    }
-#pragma unroll
-    for (int sft = 16; sft > 0; sft >>= 1) l += __shfl_xor_sync(0xffffffffu, l, sft);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-    for (int j = 0; j < DV / 32; ++j) {
-        const int64_t at = (row * p.heads + head) * DV + lane + 32 * j;
-        static_cast<T*>(p.out)[at] = one_of<T>(o[j] * inv);
-    }
-}
-
-
-template <typename T> static cudaError_t simple_typed(const AttendArgs& p, cudaStream_t st)
-{
-    const int64_t warps = static_cast<int64_t>(p.b.seqs) * p.b.max_q * p.heads;
-    const int64_t grid = (warps + ATT_WARPS - 1) / ATT_WARPS;
-    if (grid > 0x7fffffff) return cudaErrorInvalidValue;
-    const unsigned g = static_cast<unsigned>(grid);
-    if (p.c.key_dim == 64) kv_attend_kernel<64, 64, T><<<g, ATT_WARPS * 32, 0, st>>>(p);
-    else if (p.c.key_dim == 128) kv_attend_kernel<128, 128, T><<<g, ATT_WARPS * 32, 0, st>>>(p);
-    else kv_attend_kernel<192, 128, T><<<g, ATT_WARPS * 32, 0, st>>>(p);
-    return cudaGetLastError();
-}
-
 }  // namespace eva
 
 using namespace eva;
@@ -578,7 +476,7 @@ extern "C" size_t eva_kv_attend_workspace(const EvaKvCache* cache, const EvaKvBa
 {
     if (!attend_ok(cache, batch, heads)) return 0;
     const int64_t rows = shared_rows(*cache, *batch, heads);
-    if (rows > DEC_ROWS || rows == 0) return 16;
+    if (rows > DEC_ROWS) return prompt_workspace(cache->value_dim);
     const size_t pieces = static_cast<size_t>(num_sms()) * dec_warps(cache->key_dim, cache->value_dim);
     return pieces * (sizeof(int4) + 2 * sizeof(float) * part_floats(static_cast<int>(rows), cache->value_dim));
 }
@@ -617,7 +515,7 @@ extern "C" int eva_kv_attend(const EvaKvCache* cache, const EvaKvBatch* batch, c
         p.part = reinterpret_cast<float*>(p.heads_of + pieces);
         e = dtype == EVA_DTYPE_BF16 ? decode_typed<__nv_bfloat16>(p, pieces, st) : decode_typed<__half>(p, pieces, st);
     } else {
-        e = dtype == EVA_DTYPE_BF16 ? simple_typed<__nv_bfloat16>(p, st) : simple_typed<__half>(p, st);
+        e = launch_prompt(p, workspace, dtype == EVA_DTYPE_BF16, st);
     }
     return e == cudaSuccess ? EVA_OK : EVA_ERR_CUDA;
 }

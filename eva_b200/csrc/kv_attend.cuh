@@ -46,4 +46,29 @@ template <typename T> __device__ __forceinline__ T one_of(float v);
 template <> __device__ __forceinline__ __nv_bfloat16 one_of(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half one_of(float v) { return __float2half_rn(v); }
 
+// two e4m3 codes (the low 16 bits) as two halves, exact
+__device__ __forceinline__ uint32_t e4m3_halves(uint32_t two)
+{
+    uint32_t r;
+    asm("{\n .reg .b16 lo;\n cvt.u16.u32 lo, %1;\n cvt.rn.f16x2.e4m3x2 %0, lo;\n}\n" : "=r"(r) : "r"(two));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi)
+{
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Many rows (kv_prompt.cu): workspace bytes for a value dimension, and the launch.
+size_t prompt_workspace(int dv);
+cudaError_t launch_prompt(AttendArgs p, void* workspace, bool bf16, cudaStream_t st);
+
 }  // namespace eva
