@@ -26,9 +26,12 @@
 namespace eva {
 
 constexpr int PR_TILE = 128, PR_ROWS = 2 * PR_TILE;       // rows of a tile, of a CTA; tokens of a step
-constexpr int PR_CONV = 4, PR_WARPS = 8 + PR_CONV + 1;    // softmax, converter and MMA warps
+// Four warpgroups: 8 softmax warps, 4 converter warps, the MMA warp (and three idle ones). Registers move to the
+// softmax threads, which hold a row's 128 scores: 2 x 184 + 96 + 48 = 4 x 128, the launch's own.
+constexpr int PR_CONV = 4, PR_MMA = 8 + PR_CONV, PR_WARPS = 16;
+constexpr int PR_REGS_SOFTMAX = 184, PR_REGS_CONV = 96, PR_REGS_MMA = 48;
 constexpr float PR_BIAS = 7.0f, PR_SLACK = 8.0f;
-constexpr int PR_SCALES = 4;                              // steps whose scales are kept
+constexpr int PR_SCALES = 4, PR_SEGS = 4;                 // steps whose scales are kept, segments in flight
 
 template <int DK, int DV> struct PrCfg {
     static constexpr int KC = DK / 64;                    // 64-element chunks of a query or key row
@@ -40,7 +43,7 @@ template <int DK, int DV> struct PrCfg {
 };
 
 struct PrBars {
-    uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sready[2], pready[2], pvdone[2], qfull[2], scfull[PR_SCALES];
+    uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sready[2], pready[2], pvdone[2], qfull[2], scfull[PR_SCALES], segfull[PR_SEGS], segempty[PR_SEGS];
     uint32_t tmem;
 };
 
@@ -76,54 +79,16 @@ constexpr int PR_SPANS = 256;   // runs of sequences whose steps are summed in s
 
 // A piece of the line: where it begins and how many steps it has.
 struct PrPlace {
-    int b, h, qb, off;
-    int64_t left, begin, total;
-    int pieces;
+    int b, h, qb, off, left, pieces;
+    int64_t begin, total;
 };
 
-// Consecutive steps of one row block within a piece.
+
+// Consecutive steps of one row block within a piece; t1 == 0 ends the piece.
 struct PrSeg {
-    int b, h, qb, t0, t1, after;   // steps t0 .. t1 - 1, `after` more in later pieces
-    bool first;                    // holds the row block's first step
-    PrItem item;
-};
-
-struct PrCursor {
-    PrPlace at;
+    int b, h, qb, t0, t1;          // steps t0 .. t1 - 1
+    int first, after, done;        // holds the row block's first step; steps of it in later pieces; of the piece before
     KvSeq s;
-
-    __device__ __forceinline__ bool next(const AttendArgs& p, PrSeg& g)
-    {
-        if (at.left <= 0) return false;
-        g.b = at.b, g.h = at.h, g.qb = at.qb;
-        g.item = pr_item(s, p.group, p.window, at.qb);
-        const int have = g.item.tiles - at.off;
-        const int take = static_cast<int>(min(static_cast<int64_t>(have), at.left));
-        if (take <= 0) {   // lengths changed under the call
-            at.left = 0;
-            return false;
-        }
-        g.t0 = g.item.t0 + at.off;
-        g.t1 = g.t0 + take;
-        g.first = at.off == 0;
-        g.after = have - take;
-        at.left -= take;
-        at.off = 0;
-        if (at.left > 0 && ++at.qb == pr_blocks(s, p.group)) {
-            at.qb = 0;
-            if (++at.h == p.c.kv_heads) {
-                at.h = 0;
-                do {
-                    if (++at.b >= p.b.seqs) {
-                        at.left = 0;
-                        break;
-                    }
-                    s = kv_seq(p.b, at.b, p.c.status);
-                } while (s.n == 0);
-            }
-        }
-        return true;
-    }
 };
 
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16])
@@ -135,15 +100,98 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_st32f(uint32_t taddr, const float (&v)[32])
+// 32 columns into r, valid after tmem_wait_ld() and tied()
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t* r)
 {
-    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// Keeps the uses of r[0 .. 31] behind this point
+__device__ __forceinline__ void tied(uint32_t* r)
+{
+    asm volatile(""
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
+
+// Two 32-bit products and sums in one instruction
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float m, float c)
+{
+    asm("{\n .reg .b64 p, q, r;\n mov.b64 p, {%2, %3};\n mov.b64 q, {%4, %4};\n mov.b64 r, {%5, %5};\n"
+        " fma.rn.f32x2 p, p, q, r;\n mov.b64 {%0, %1}, p;\n}\n"
+        : "=f"(x), "=f"(y)
+        : "f"(a), "f"(b), "f"(m), "f"(c));
+}
+
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b)
+{
+    asm("{\n .reg .b64 p, q;\n mov.b64 p, {%0, %1};\n mov.b64 q, {%2, %3};\n add.rn.f32x2 p, p, q;\n mov.b64 {%0, %1}, p;\n}\n"
+        : "+f"(x), "+f"(y)
+        : "f"(a), "f"(b));
+}
+
+// Largest t = score * scale + exponent over a step's scores r; with MASK over those that are seen (bit i of the words)
+template <bool MASK>
+__device__ __forceinline__ float pr_max(const uint32_t (&r)[128], const float4* sc, float c, int lo, int hi)
+{
+    float mx = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int x = 0; x < 8; ++x) {
+        float b = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(v[16 * k + i]);
-        tmem_st16(taddr + 16 * k, r);
+        for (int i = 0; i < 16; ++i) {
+            const float v = __uint_as_float(r[16 * x + i]);
+            b = fmaxf(b, !MASK || (16 * x + i >= lo && 16 * x + i < hi) ? v : -INFINITY);
+        }
+        mx = fmaxf(mx, fmaf(b, sc[x].x * c, sc[x].y));
     }
+    return mx;
+}
+
+// Weights 2^(t + ref) of a step's scores as fp16 into tensor memory (over the scores); returns their sum, each divided
+// by its value scale. CAREFUL: with the mask, and rounding t as pr_max did.
+template <bool CAREFUL>
+__device__ __forceinline__ float pr_weights(const uint32_t (&r)[128], const float4* sc, float c, float ref, int lo, int hi, uint32_t ts)
+{
+    float l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        uint32_t w[16];
+#pragma unroll
+        for (int x = 2 * k; x < 2 * k + 2; ++x) {
+            const float4 f = sc[x];
+            const float fc = f.x * c, add = f.y + ref;
+            float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+            for (int i = 16 * x; i < 16 * x + 16; i += 2) {
+                float a = __uint_as_float(r[i]), b = __uint_as_float(r[i + 1]);
+                if constexpr (CAREFUL) {
+                    a = i >= lo && i < hi ? fmaf(a, fc, f.y) + ref : -INFINITY;
+                    b = i + 1 >= lo && i + 1 < hi ? fmaf(b, fc, f.y) + ref : -INFINITY;
+                } else {
+                    fma2(a, b, a, b, fc, add);
+                }
+                a = ex2(a);
+                b = ex2(b);
+                add2(s0, s1, a, b);
+                w[i / 2 - 16 * k] = half2_bits(a, b);
+            }
+            l = fmaf(s0 + s1, f.z, l);
+        }
+        tmem_st16(ts + 16 * k, w);
+    }
+    return l;
 }
 
 // 16 codes (16 bytes) as two 16-byte units of halves
@@ -170,6 +218,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
     __shared__ float4 scales[PR_SCALES][8];               // of a step's blocks: key scale, value exponent, 1 / value scale
     __shared__ unsigned long long spans[PR_SPANS];
     __shared__ PrPlace place;
+    __shared__ PrSeg segs[PR_SEGS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint8_t* smem = align1024(smem_raw);
     const uint32_t sq = smem_u32(smem), sk = sq + C::Q, sv = sk + C::KST * C::K;
@@ -187,9 +236,13 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
             mbar_init(&B.qfull[i], 4);
         }
         for (int i = 0; i < PR_SCALES; ++i) mbar_init(&B.scfull[i], 1);
+        for (int i = 0; i < PR_SEGS; ++i) {
+            mbar_init(&B.segfull[i], 1);
+            mbar_init(&B.segempty[i], 8 + PR_CONV + 1);
+        }
         fence_barrier_init();
     }
-    if (warp == PR_WARPS - 1) tmem_alloc(&B.tmem, 512);
+    if (warp == PR_MMA) tmem_alloc(&B.tmem, 512);
     for (int i = threadIdx.x; i < PR_SPANS; i += PR_WARPS * 32) spans[i] = 0;
     __syncthreads();
     // this CTA's piece of the line
@@ -212,7 +265,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
         const int c = blockIdx.x;
         if (c < w.pieces) {
             w.begin = total * c / w.pieces;
-            w.left = total * (c + 1) / w.pieces - w.begin;
+            w.left = static_cast<int>(total * (c + 1) / w.pieces - w.begin);
             int64_t rem = w.begin;
             int i = 0;
             while (i < PR_SPANS - 1 && rem >= static_cast<int64_t>(spans[i]) * heads) rem -= static_cast<int64_t>(spans[i++]) * heads;
@@ -255,207 +308,194 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = B.tmem;
-    PrCursor cur;
-    cur.at = place;
-    cur.s = cur.at.left > 0 ? kv_seq(p.b, cur.at.b, status) : KvSeq{0, 0, 0, 0};
-    PrSeg g;
+    // Segment i of the piece, for every lane of a warp (or the one thread that calls)
+    auto segment = [&](uint32_t i) -> const PrSeg& {
+        mbar_wait(&B.segfull[i % PR_SEGS], (i / PR_SEGS) & 1, status);
+        return segs[i % PR_SEGS];
+    };
 
     if (warp < 8) {
         // ---- softmax: thread = row of tile `tile`
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PR_REGS_SOFTMAX));
         const int tile = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + tile * PR_TILE, to = tmem + lanes + 2 * PR_TILE + tile * DV;
-        uint32_t it = 0;                      // steps so far
-        int4 head = make_int4(-1, 0, 0, 0);   // the row block that begins here and goes on in later pieces
-        int64_t at = cur.at.begin;
-        KvSeq s = cur.s;
-        while (cur.next(p, g)) {
-            const int r = g.qb * PR_ROWS + tile * PR_TILE + row, tok = r / p.group;
-            const bool in = tok < s.n;
-            const int64_t head_row = (static_cast<int64_t>(s.row0) + tok);
-            const int qh = g.h * p.group + (r - tok * p.group);
-            float c;
-            {
-                // the row, scaled by a power of two to [1, 2) at its largest, as fp16
-                const T* q = static_cast<const T*>(p.q) + head_row * p.qt + static_cast<int64_t>(qh) * p.qh;
-                float big = 0.0f;
-                bool odd = false;
-#pragma unroll 4
-                for (int u = 0; u < DK / 8; ++u) {
-                    const uint4 v = in ? *reinterpret_cast<const uint4*>(q + u * 8) : make_uint4(0, 0, 0, 0);
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t it = 0, seg = 0;             // steps and segments so far
+        uint4 raw[DK / 8];                    // the row's query
+        int pos = 0, t0 = 0, t1 = 0;          // position of the row, -1 - pos where it is behind the sequence
+        T* dst = nullptr;                     // its output, or partial sums
+        bool in = false, whole = false;
+        if (threadIdx.x == 0) p.heads_of[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        // takes the next segment's row up (its loads are under way when this returns)
+        auto take = [&]() -> bool {
+            const PrSeg& g = segment(seg);
+            t0 = g.t0;
+            t1 = g.t1;
+            if (t1 == 0) return false;
+            const int r = g.qb * PR_ROWS + tile * PR_TILE + row, tok = r / p.group, qh = g.h * p.group + (r - tok * p.group);
+            in = tok < g.s.n;
+            pos = g.s.ctx + tok;
+            whole = g.first && g.after == 0;
+            const int64_t qrow = static_cast<int64_t>(g.s.row0) + tok;
+            if (whole)
+                dst = static_cast<T*>(p.out) + (qrow * p.heads + qh) * DV;
+            else
+                dst = reinterpret_cast<T*>(p.part + (static_cast<int64_t>(blockIdx.x) * 2 + g.first) * PR_ROWS * (DV + 2));
+            if (threadIdx.x == 0 && g.first && g.after > 0)
+                p.heads_of[blockIdx.x] =
+                    make_int4(g.b, g.h, g.qb,
+                              static_cast<int>(((place.begin + g.done + (t1 - t0) + g.after) * place.pieces - 1) / place.total));
+            const T* q = static_cast<const T*>(p.q) + qrow * p.qt + static_cast<int64_t>(qh) * p.qh;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 f = two_floats<T>(w[e]);
-                        big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
-                        odd |= f.x != f.x || f.y != f.y;
-                    }
-                }
-                odd |= big == INFINITY;
-                const int e2 = min(max(static_cast<int>(__float_as_uint(big) >> 23), 1), 252);
-                const float down = __uint_as_float(static_cast<uint32_t>(254 - e2) << 23);
-                c = odd ? __uint_as_float(0x7fc00000u) : p.scale * __uint_as_float(static_cast<uint32_t>(e2) << 23);
-#pragma unroll 4
-                for (int u = 0; u < DK / 8; ++u) {
-                    const uint4 v = in ? *reinterpret_cast<const uint4*>(q + u * 8) : make_uint4(0, 0, 0, 0);
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                    uint32_t o[4];
+            for (int u = 0; u < DK / 8; ++u) raw[u] = in ? *reinterpret_cast<const uint4*>(q + u * 8) : make_uint4(0, 0, 0, 0);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&B.segempty[seg % PR_SEGS]);
+            ++seg;
+            return true;
+        };
+        bool more = take();
+        while (more) {
+            // the row, scaled by a power of two to [1, 2) at its largest, as fp16
+            float c, big = 0.0f;
+            bool odd = false;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 f = two_floats<T>(w[e]);
-                        o[e] = half2_bits(f.x * down, f.y * down);
-                    }
-                    st_shared16(sq + (tile * C::KC + u / 8) * C::CHUNK + sw128(row, u % 8), make_uint4(o[0], o[1], o[2], o[3]));
+            for (int u = 0; u < DK / 8; ++u) {
+                const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 f = two_floats<T>(w[e]);
+                    big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+                    odd |= f.x != f.x || f.y != f.y;
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&B.qfull[tile]);
             }
+            odd |= big == INFINITY;
+            const int e2 = min(max(static_cast<int>(__float_as_uint(big) >> 23), 1), 252);
+            const float down = __uint_as_float(static_cast<uint32_t>(254 - e2) << 23);
+            c = odd ? __uint_as_float(0x7fc00000u) : p.scale * __uint_as_float(static_cast<uint32_t>(e2) << 23);
+#pragma unroll
+            for (int u = 0; u < DK / 8; ++u) {
+                const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+                uint32_t o[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 f = two_floats<T>(w[e]);
+                    o[e] = half2_bits(f.x * down, f.y * down);
+                }
+                st_shared16(sq + (tile * C::KC + u / 8) * C::CHUNK + sw128(row, u % 8), make_uint4(o[0], o[1], o[2], o[3]));
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&B.qfull[tile]);
             // rows without a token see nothing; rows behind the sequence are not written and need no mask
-            const int hi = in ? s.ctx + tok + 1 : 0x7fffffff;
-            const int lo = in && p.window > 0 ? hi - p.window : 0;
+            const int hi = in ? pos + 1 : 0x7fffffff, lo = in && p.window > 0 ? max(hi - p.window, 0) : 0;
             const int all_hi = __reduce_min_sync(0xffffffffu, hi), all_lo = __reduce_max_sync(0xffffffffu, lo);
             float m = -INFINITY, l = 0.0f;
-            for (int t = g.t0; t < g.t1; ++t, ++it) {
+            const int first = t0;
+            for (int t = t0; t < t1; ++t, ++it) {
                 const float4* sc = scales[it % PR_SCALES];
                 const int tok0 = t * PR_TILE;
                 const bool part = tok0 + PR_TILE > all_hi || tok0 < all_lo;
                 mbar_wait(&B.scfull[it % PR_SCALES], (it / PR_SCALES) & 1, status);
                 mbar_wait(&B.sready[tile], it & 1, status);
                 tc_fence_after();
-                float mx = -INFINITY;
+                uint32_t v[128];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    float v[32];
-                    tmem_ld32(ts + 32 * k, v);
-                    if (part) {
+                for (int k = 0; k < 4; ++k) tmem_ld32_async(ts + 32 * k, v + 32 * k);
+                tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int tk = tok0 + 32 * k + i;
-                            v[i] = tk >= lo && tk < hi ? v[i] : -INFINITY;
-                        }
-                    }
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        float b = v[16 * x];
-#pragma unroll
-                        for (int i = 1; i < 16; ++i) b = fmaxf(b, v[16 * x + i]);
-                        const float4 f = sc[2 * k + x];
-                        mx = fmaxf(mx, fmaf(b, f.x * c, f.y));
-                    }
-                }
+                for (int k = 0; k < 4; ++k) tied(v + 32 * k);
+                const float mx = part ? pr_max<true>(v, sc, c, lo - tok0, hi - tok0) : pr_max<false>(v, sc, c, 0, 0);
                 const bool grow = mx > m + PR_SLACK || (m == -INFINITY && mx > m);
                 if (__any_sync(0xffffffffu, grow)) {
-                    const float down = grow ? ex2(m - mx) : 1.0f;
+                    const float fall = grow ? ex2(m - mx) : 1.0f;
                     if (grow) m = mx;
-                    l *= down;
-                    if (t > g.t0) {
+                    l *= fall;
+                    if (t > first) {
                         mbar_wait(&B.pvdone[tile], (it - 1) & 1, status);
                         tc_fence_after();
 #pragma unroll 1
-                        for (int k = 0; k < DV; k += 32) {
-                            float v[32];
-                            tmem_ld32(to + k, v);
+                        for (int k = 0; k < DV; k += 16) {
+                            uint32_t o[16];
+                            tmem_ld32x32_x16(to + k, o);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] *= down;
-                            tmem_st32f(to + k, v);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fall);
+                            tmem_st16(to + k, o);
                         }
                     }
                 }
                 const float ref = PR_BIAS - (m == -INFINITY ? 0.0f : m);
                 // far from 0 the rounding of M must be the score's own, else their difference is not small at the largest
                 const bool careful = part || __any_sync(0xffffffffu, m != -INFINITY && fabsf(m) > 4096.0f);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    float v[32];
-                    tmem_ld32(ts + 32 * k, v);
-                    uint32_t w[16];
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const float4 f = sc[2 * k + x];
-                        const float fc = f.x * c, add = f.y + ref;
-                        float sum = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            float a = fmaf(v[16 * x + i], fc, add), b = fmaf(v[16 * x + i + 1], fc, add);
-                            if (careful) {
-                                const int tk = tok0 + 32 * k + 16 * x + i;
-                                a = fmaf(v[16 * x + i], fc, f.y) + ref;
-                                b = fmaf(v[16 * x + i + 1], fc, f.y) + ref;
-                                a = tk >= lo && tk < hi ? a : -INFINITY;
-                                b = tk + 1 >= lo && tk + 1 < hi ? b : -INFINITY;
-                            }
-                            a = ex2(a);
-                            b = ex2(b);
-                            sum += a + b;
-                            w[8 * x + i / 2] = half2_bits(a, b);
-                        }
-                        l = fmaf(sum, f.z, l);
-                    }
-                    tmem_st16(ts + 16 * k, w);
-                }
+                l += careful ? pr_weights<true>(v, sc, c, ref, part ? lo - tok0 : 0, part ? hi - tok0 : PR_TILE, ts)
+                             : pr_weights<false>(v, sc, c, ref, 0, 0, ts);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&B.pready[tile]);
             }
-            // the row block's output, or its partial sums
+            // the row block's output, or its partial sums, while the next query is on its way
+            const bool was_whole = whole, was_in = in;
+            T* out = dst;
+            more = take();
             mbar_wait(&B.pvdone[tile], (it - 1) & 1, status);
             tc_fence_after();
-            const bool whole = g.first && g.after == 0;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            T* out = static_cast<T*>(p.out) + (head_row * p.heads + qh) * DV;
             const int pr = tile * PR_TILE + row;
-            float* part = p.part + (static_cast<int64_t>(blockIdx.x) * 2 + (g.first ? 1 : 0)) * PR_ROWS * (DV + 2);
-            if (!whole && in) {
+            float* part = reinterpret_cast<float*>(out);
+            if (!was_whole && was_in) {
                 part[pr] = m;
                 part[PR_ROWS + pr] = l;
             }
-            float* po = part + 2 * PR_ROWS + static_cast<int64_t>(pr) * DV;
+            float* po = part + 2 * PR_ROWS + pr * DV;
 #pragma unroll 1
             for (int k = 0; k < DV; k += 32) {
                 float v[32];
                 __syncwarp();
                 tmem_ld32(to + k, v);
-                if (in && whole) {
+                if (was_in && was_whole) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 8)
                         *reinterpret_cast<uint4*>(out + k + i) =
                             make_uint4(two_bits<T>(v[i] * inv, v[i + 1] * inv), two_bits<T>(v[i + 2] * inv, v[i + 3] * inv),
                                        two_bits<T>(v[i + 4] * inv, v[i + 5] * inv), two_bits<T>(v[i + 6] * inv, v[i + 7] * inv));
-                } else if (in) {
+                } else if (was_in) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
                         *reinterpret_cast<float4*>(po + k + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                 }
             }
             tc_fence_before();
-            at += g.t1 - g.t0;
-            if (g.first && g.after > 0)
-                head = make_int4(g.b, g.h, g.qb, static_cast<int>(((at + g.after) * cur.at.pieces - 1) / cur.at.total));
-            s = cur.s;
         }
-        if (threadIdx.x == 0) p.heads_of[blockIdx.x] = head;
     } else if (warp < 8 + PR_CONV) {
         // ---- converters: 64-byte quarters of 8 rows per warp and load
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PR_REGS_CONV));
         const int cw = warp - 8, unit = lane & 3, sub = cw * 8 + (lane >> 2);
         uint4 kr[DK / 64][4], vr[2][DV / 32];
         float4 mine = make_float4(1.0f, 0.0f, 1.0f, 0.0f);   // scales of block `lane` of the step (lanes 0 .. 7 of warp 8)
         int pages = -1, pages_at = -64, pages_b = -1;        // lane l: page pages_at + l of sequence pages_b
-        KvSeq s = cur.s;
-        bool more = cur.next(p, g);
-        int t = more ? g.t0 : 0, pg[2] = {-1, -1}, len = s.len;
+        uint32_t seg = 0;
+        int gb = 0, gh = 0, t = 0, t1 = 0, len = 0, pg[2] = {-1, -1};
+        auto take = [&]() -> bool {
+            const PrSeg& g = segment(seg);
+            gb = g.b, gh = g.h, t = g.t0, t1 = g.t1, len = g.s.len;
+            if (t1 == 0) return false;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&B.segempty[seg % PR_SEGS]);
+            ++seg;
+            return true;
+        };
+        bool more = take();
 
         // pages of step t
         auto find = [&]() {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const int i = 2 * t + x;
-                if (g.b != pages_b || i < pages_at || i >= pages_at + 32) {
-                    pages_b = g.b;
+                if (gb != pages_b || i < pages_at || i >= pages_at + 32) {
+                    pages_b = gb;
                     pages_at = i;
                     const int want = i + lane;
-                    pages = static_cast<int64_t>(want) * KV_PAGE < s.len ? kv_page(p.c, p.b, g.b, want, status) : -1;
+                    pages = static_cast<int64_t>(want) * KV_PAGE < len ? kv_page(p.c, p.b, gb, want, status) : -1;
                 }
                 pg[x] = __shfl_sync(0xffffffffu, pages, i - pages_at);
             }
@@ -465,7 +505,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
             for (int k = 0; k < 4; ++k) {
                 const int r = sub + 32 * k, page = pg[k >> 1];   // row r: token r % 64 of page r / 64
                 const uint8_t* src = static_cast<const uint8_t*>(p.c.k) +
-                                     ((static_cast<int64_t>(max(page, 0)) * p.c.kv_heads + g.h) * KV_PAGE + (r & 63)) * DK + unit * 16;
+                                     ((static_cast<int64_t>(max(page, 0)) * p.c.kv_heads + gh) * KV_PAGE + (r & 63)) * DK + unit * 16;
 #pragma unroll
                 for (int ch = 0; ch < DK / 64; ++ch)
                     kr[ch][k] = page >= 0 ? *reinterpret_cast<const uint4*>(src + ch * 64) : make_uint4(0, 0, 0, 0);
@@ -474,7 +514,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
                 const int page = pg[lane >> 2];
                 mine = make_float4(1.0f, -INFINITY, 0.0f, 0.0f);   // no page: no weight
                 if (page >= 0) {
-                    const int64_t i = (static_cast<int64_t>(page) * p.c.kv_heads + g.h) * KV_PAGE_BLOCKS + (lane & 3);
+                    const int64_t i = (static_cast<int64_t>(page) * p.c.kv_heads + gh) * KV_PAGE_BLOCKS + (lane & 3);
                     const uint32_t ks = static_cast<const uint8_t*>(p.c.k_scale)[i];
                     const uint32_t vs = min(max(static_cast<uint32_t>(static_cast<const uint8_t*>(p.c.v_scale)[i]), 1u), 253u);
                     mine = make_float4(kv_scale(ks), static_cast<float>(static_cast<int>(vs) - 127),
@@ -486,7 +526,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const uint8_t* src = static_cast<const uint8_t*>(p.c.v) +
-                                     ((static_cast<int64_t>(max(pg[x], 0)) * p.c.kv_heads + g.h) * DV + sub) * KV_PAGE + unit * 16;
+                                     ((static_cast<int64_t>(max(pg[x], 0)) * p.c.kv_heads + gh) * DV + sub) * KV_PAGE + unit * 16;
 #pragma unroll
                 for (int k = 0; k < DV / 32; ++k)
                     vr[x][k] = pg[x] >= 0 ? *reinterpret_cast<const uint4*>(src + k * 32 * KV_PAGE) : make_uint4(0, 0, 0, 0);
@@ -532,12 +572,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
             __syncwarp();
             if (lane == 0) mbar_arrive(&B.kfull[ks]);
             if (cw == 0 && lane == 0) mbar_arrive(&B.scfull[it % PR_SCALES]);
-            if (++t == g.t1) {
-                s = cur.s;
-                more = cur.next(p, g);
-                t = g.t0;
-                len = s.len;
-            }
+            if (++t == t1) more = take();
             if (more) {
                 find();
                 load_k();
@@ -558,10 +593,12 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
             if (lane == 0) mbar_arrive(&B.vfull[vs]);
             if (more) load_v();
         }
-    } else if (lane == 0) {
-        // ---- MMA issue
+    } else {
+        // ---- MMA issue: one thread
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PR_REGS_MMA));
+        if (warp == PR_MMA && lane == 0) {
         constexpr uint32_t iqk = umma_idesc_f16(PR_TILE, PR_TILE), ipv = umma_idesc_f16(PR_TILE, DV);
-        uint32_t it = 0, segs = 0;
+        uint32_t it = 0, seg = 0;
         auto qk = [&](int tile, uint32_t n) {
             const uint32_t k0 = sk + (n % C::KST) * C::K, q0 = sq + tile * C::KC * C::CHUNK;
 #pragma unroll
@@ -570,10 +607,13 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
                          umma_desc_sw128(k0 + (j >> 2) * C::CHUNK + (j & 3) * 32), iqk, j > 0);
             umma_commit(&B.sready[tile]);
         };
-        while (cur.next(p, g)) {
+        for (;; ++seg) {
+            const PrSeg& g = segment(seg);
             const int n = g.t1 - g.t0;
+            if (g.t1 == 0) break;
+            mbar_arrive(&B.segempty[seg % PR_SEGS]);
             for (int tile = 0; tile < 2; ++tile) {
-                mbar_wait(&B.qfull[tile], segs & 1, status);
+                mbar_wait(&B.qfull[tile], seg & 1, status);
                 if (tile == 0) mbar_wait(&B.kfull[it % C::KST], (it / C::KST) & 1, status);
                 tc_fence_after();
                 qk(tile, it);
@@ -601,13 +641,55 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
                 umma_commit(&B.vempty[it % C::VST]);
                 if (j + 1 < n) umma_commit(&B.kempty[(it + 1) % C::KST]);
             }
-            ++segs;
+        }
+        } else if (warp == PR_MMA + 1 && lane == 0) {
+            // the segments of the piece
+            int b = place.b, h = place.h, qb = place.qb, off = place.off, left = place.left, done = 0;
+            KvSeq s = left > 0 ? kv_seq(p.b, b, status) : KvSeq{0, 0, 0, 0};
+            for (uint32_t i = 0;; ++i) {
+                mbar_wait(&B.segempty[i % PR_SEGS], ((i / PR_SEGS) & 1) ^ 1, status);
+                PrSeg& g = segs[i % PR_SEGS];
+                PrItem item{};
+                int have = 0;
+                if (left > 0) {
+                    item = pr_item(s, p.group, p.window, qb);
+                    have = item.tiles - off;
+                }
+                const int n = min(have, left);
+                if (n <= 0) {   // the end (or lengths that changed under the call)
+                    g.t0 = g.t1 = 0;
+                    mbar_arrive(&B.segfull[i % PR_SEGS]);
+                    break;
+                }
+                g.b = b, g.h = h, g.qb = qb, g.s = s, g.done = done;
+                g.t0 = item.t0 + off;
+                g.t1 = g.t0 + n;
+                g.first = off == 0;
+                g.after = have - n;
+                mbar_arrive(&B.segfull[i % PR_SEGS]);
+                left -= n;
+                done += n;
+                off = 0;
+                if (left > 0 && ++qb == pr_blocks(s, p.group)) {
+                    qb = 0;
+                    if (++h == p.c.kv_heads) {
+                        h = 0;
+                        do {
+                            if (++b >= p.b.seqs) {
+                                left = 0;
+                                break;
+                            }
+                            s = kv_seq(p.b, b, status);
+                        } while (s.n == 0);
+                    }
+                }
+            }
         }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == PR_WARPS - 1) {
+    if (warp == PR_MMA) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
