@@ -100,6 +100,41 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         : "memory");
 }
 
+// One lane of the (whole) warp
+__device__ __forceinline__ uint32_t elect_one()
+{
+    uint32_t r;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r;
+}
+
+__device__ __forceinline__ void umma_f16_if(uint32_t lead, uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc)
+{
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+        "l"(da), "l"(db), "r"(idesc), "r"(acc), "r"(lead)
+        : "memory");
+}
+
+__device__ __forceinline__ void umma_f16_ta_if(uint32_t lead, uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc,
+                                               uint32_t acc)
+{
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(db), "r"(idesc), "r"(acc), "r"(lead)
+        : "memory");
+}
+
+__device__ __forceinline__ void umma_commit_if(uint32_t lead, uint64_t* bar)
+{
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)), "r"(lead)
+        : "memory");
+}
+
 // 32 columns into r, valid after tmem_wait_ld() and tied()
 __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t* r)
 {
@@ -219,7 +254,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
     __shared__ unsigned long long spans[PR_SPANS];
     __shared__ PrPlace place;
     __shared__ PrSeg segs[PR_SEGS];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform for the compiler
     uint8_t* smem = align1024(smem_raw);
     const uint32_t sq = smem_u32(smem), sk = sq + C::Q, sv = sk + C::KST * C::K;
     int* const status = p.c.status;
@@ -353,8 +388,43 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
             ++seg;
             return true;
         };
-        bool more = take();
-        while (more) {
+        float m = 0.0f, l = 0.0f;
+        for (bool pending = false;; pending = true) {
+            const bool was_whole = whole, was_in = in;
+            T* const out = dst;
+            const bool more = take();
+            if (pending) {
+                // the row block's output, or its partial sums, while the next query is on its way
+                mbar_wait(&B.pvdone[tile], (it - 1) & 1, status);
+                tc_fence_after();
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const int pr = tile * PR_TILE + row;
+                float* part = reinterpret_cast<float*>(out);
+                if (!was_whole && was_in) {
+                    part[pr] = m;
+                    part[PR_ROWS + pr] = l;
+                }
+                float* po = part + 2 * PR_ROWS + pr * DV;
+#pragma unroll 1
+                for (int k = 0; k < DV; k += 32) {
+                    float v[32];
+                    __syncwarp();
+                    tmem_ld32(to + k, v);
+                    if (was_in && was_whole) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8)
+                            *reinterpret_cast<uint4*>(out + k + i) =
+                                make_uint4(two_bits<T>(v[i] * inv, v[i + 1] * inv), two_bits<T>(v[i + 2] * inv, v[i + 3] * inv),
+                                           two_bits<T>(v[i + 4] * inv, v[i + 5] * inv), two_bits<T>(v[i + 6] * inv, v[i + 7] * inv));
+                    } else if (was_in) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<float4*>(po + k + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                    }
+                }
+                tc_fence_before();
+            }
+            if (!more) break;
             // the row, scaled by a power of two to [1, 2) at its largest, as fp16
             float c, big = 0.0f;
             bool odd = false;
@@ -389,7 +459,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
             // rows without a token see nothing; rows behind the sequence are not written and need no mask
             const int hi = in ? pos + 1 : 0x7fffffff, lo = in && p.window > 0 ? max(hi - p.window, 0) : 0;
             const int all_hi = __reduce_min_sync(0xffffffffu, hi), all_lo = __reduce_max_sync(0xffffffffu, lo);
-            float m = -INFINITY, l = 0.0f;
+            m = -INFINITY, l = 0.0f;
             const int first = t0;
             for (int t = t0; t < t1; ++t, ++it) {
                 const float4* sc = scales[it % PR_SCALES];
@@ -433,38 +503,6 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&B.pready[tile]);
             }
-            // the row block's output, or its partial sums, while the next query is on its way
-            const bool was_whole = whole, was_in = in;
-            T* out = dst;
-            more = take();
-            mbar_wait(&B.pvdone[tile], (it - 1) & 1, status);
-            tc_fence_after();
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            const int pr = tile * PR_TILE + row;
-            float* part = reinterpret_cast<float*>(out);
-            if (!was_whole && was_in) {
-                part[pr] = m;
-                part[PR_ROWS + pr] = l;
-            }
-            float* po = part + 2 * PR_ROWS + pr * DV;
-#pragma unroll 1
-            for (int k = 0; k < DV; k += 32) {
-                float v[32];
-                __syncwarp();
-                tmem_ld32(to + k, v);
-                if (was_in && was_whole) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 8)
-                        *reinterpret_cast<uint4*>(out + k + i) =
-                            make_uint4(two_bits<T>(v[i] * inv, v[i + 1] * inv), two_bits<T>(v[i + 2] * inv, v[i + 3] * inv),
-                                       two_bits<T>(v[i + 4] * inv, v[i + 5] * inv), two_bits<T>(v[i + 6] * inv, v[i + 7] * inv));
-                } else if (was_in) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<float4*>(po + k + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                }
-            }
-            tc_fence_before();
         }
     } else if (warp < 8 + PR_CONV) {
         // ---- converters: 64-byte quarters of 8 rows per warp and load
@@ -475,17 +513,6 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
         int pages = -1, pages_at = -64, pages_b = -1;        // lane l: page pages_at + l of sequence pages_b
         uint32_t seg = 0;
         int gb = 0, gh = 0, t = 0, t1 = 0, len = 0, pg[2] = {-1, -1};
-        auto take = [&]() -> bool {
-            const PrSeg& g = segment(seg);
-            gb = g.b, gh = g.h, t = g.t0, t1 = g.t1, len = g.s.len;
-            if (t1 == 0) return false;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&B.segempty[seg % PR_SEGS]);
-            ++seg;
-            return true;
-        };
-        bool more = take();
-
         // pages of step t
         auto find = [&]() {
 #pragma unroll
@@ -549,13 +576,42 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
                 }
             }
         };
-        if (more) {
-            find();
-            load_k();
+        for (uint32_t it = 0;; ++it) {
+            // step `it`: keys on their way, then the values of the step before into shared memory, and so on in turn
+            if (it == 0 || ++t == t1) {
+                const PrSeg& g = segment(seg);
+                gb = g.b, gh = g.h, t = g.t0, t1 = g.t1, len = g.s.len;
+                if (t1 != 0) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&B.segempty[seg % PR_SEGS]);
+                    ++seg;
+                }
+            }
+            const bool more = t1 != 0;
+            if (more) {
+                find();
+                load_k();
+            }
+            if (it > 0) {
+                const uint32_t vs = (it - 1) % C::VST;
+                mbar_wait(&B.vempty[vs], (((it - 1) / C::VST) & 1) ^ 1, status);
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int k = 0; k < DV / 32; ++k) {
+                        uint4 a, b;
+                        codes_to_halves(vr[x][k], a, b);
+                        const uint32_t dst = sv + vs * C::V + x * C::VCHUNK;
+                        st_shared16(dst + sw128(sub + 32 * k, 2 * unit), a);
+                        st_shared16(dst + sw128(sub + 32 * k, 2 * unit + 1), b);
+                    }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&B.vfull[vs]);
+            }
+            if (!more) break;
             load_v();
-        }
-        for (uint32_t it = 0; more; ++it) {
-            const uint32_t ks = it % C::KST, vs = it % C::VST;
+            const uint32_t ks = it % C::KST;
             mbar_wait(&B.kempty[ks], ((it / C::KST) & 1) ^ 1, status);
 #pragma unroll
             for (int ch = 0; ch < DK / 64; ++ch)
@@ -572,64 +628,54 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
             __syncwarp();
             if (lane == 0) mbar_arrive(&B.kfull[ks]);
             if (cw == 0 && lane == 0) mbar_arrive(&B.scfull[it % PR_SCALES]);
-            if (++t == t1) more = take();
-            if (more) {
-                find();
-                load_k();
-            }
-            mbar_wait(&B.vempty[vs], ((it / C::VST) & 1) ^ 1, status);
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int k = 0; k < DV / 32; ++k) {
-                    uint4 a, b;
-                    codes_to_halves(vr[x][k], a, b);
-                    const uint32_t dst = sv + vs * C::V + x * C::VCHUNK;
-                    st_shared16(dst + sw128(sub + 32 * k, 2 * unit), a);
-                    st_shared16(dst + sw128(sub + 32 * k, 2 * unit + 1), b);
-                }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&B.vfull[vs]);
-            if (more) load_v();
         }
     } else {
-        // ---- MMA issue: one thread
+        // ---- MMA issue: a whole warp walks through, so that descriptors stay in uniform registers, and one lane issues
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PR_REGS_MMA));
-        if (warp == PR_MMA && lane == 0) {
+        if (warp == PR_MMA) {
+            const uint32_t lead = elect_one();
         constexpr uint32_t iqk = umma_idesc_f16(PR_TILE, PR_TILE), ipv = umma_idesc_f16(PR_TILE, DV);
         uint32_t it = 0, seg = 0;
+        // Rolled loops: this warp runs each product once a step, and straight-line code would come from memory every time.
         auto qk = [&](int tile, uint32_t n) {
-            const uint32_t k0 = sk + (n % C::KST) * C::K, q0 = sq + tile * C::KC * C::CHUNK;
-#pragma unroll
-            for (int j = 0; j < DK / 16; ++j)
-                umma_f16(tmem + tile * PR_TILE, umma_desc_sw128(q0 + (j >> 2) * C::CHUNK + (j & 3) * 32),
-                         umma_desc_sw128(k0 + (j >> 2) * C::CHUNK + (j & 3) * 32), iqk, j > 0);
-            umma_commit(&B.sready[tile]);
+            uint64_t a = umma_desc_sw128(sq + tile * C::KC * C::CHUNK), b = umma_desc_sw128(sk + (n % C::KST) * C::K);
+#pragma unroll 1
+            for (int j = 0; j < DK / 16; ++j) {
+                umma_f16_if(lead, tmem + tile * PR_TILE, a, b, iqk, j > 0);
+                const uint32_t up = (j & 3) == 3 ? (C::CHUNK - 96) >> 4 : 2;   // 32 bytes on, or the next chunk
+                a += up;
+                b += up;
+            }
+            umma_commit_if(lead, &B.sready[tile]);
+        };
+        auto pv = [&](int tile, uint32_t n, bool add) {
+            uint64_t b = umma_desc_sw128(sv + (n % C::VST) * C::V);
+#pragma unroll 1
+            for (int k = 0; k < PR_TILE / 16; ++k) {
+                umma_f16_ta_if(lead, tmem + 2 * PR_TILE + tile * DV, tmem + tile * PR_TILE + k * 8, b, ipv, add || k > 0);
+                b += (k & 3) == 3 ? (C::VCHUNK - 96) >> 4 : 2;
+            }
+            umma_commit_if(lead, &B.pvdone[tile]);
         };
         for (;; ++seg) {
             const PrSeg& g = segment(seg);
             const int n = g.t1 - g.t0;
             if (g.t1 == 0) break;
-            mbar_arrive(&B.segempty[seg % PR_SEGS]);
+            __syncwarp();
+            if (lead) mbar_arrive(&B.segempty[seg % PR_SEGS]);
             for (int tile = 0; tile < 2; ++tile) {
                 mbar_wait(&B.qfull[tile], seg & 1, status);
                 if (tile == 0) mbar_wait(&B.kfull[it % C::KST], (it / C::KST) & 1, status);
                 tc_fence_after();
                 qk(tile, it);
             }
-            umma_commit(&B.kempty[it % C::KST]);
+            umma_commit_if(lead, &B.kempty[it % C::KST]);
             for (int j = 0; j < n; ++j, ++it) {
                 for (int tile = 0; tile < 2; ++tile) {
                     if (tile == 0) mbar_wait(&B.vfull[it % C::VST], (it / C::VST) & 1, status);
                     mbar_wait(&B.pready[tile], it & 1, status);
                     tc_fence_after();
-                    const uint32_t v0 = sv + (it % C::VST) * C::V;
-#pragma unroll
-                    for (int k = 0; k < PR_TILE / 16; ++k)
-                        umma_f16_ta(tmem + 2 * PR_TILE + tile * DV, tmem + tile * PR_TILE + k * 8,
-                                    umma_desc_sw128(v0 + (k >> 2) * C::VCHUNK + (k & 3) * 32), ipv, j > 0 || k > 0);
-                    umma_commit(&B.pvdone[tile]);
+                    pv(tile, it, j > 0);
                     if (j + 1 < n) {
                         if (tile == 0) {
                             mbar_wait(&B.kfull[(it + 1) % C::KST], ((it + 1) / C::KST) & 1, status);
@@ -638,8 +684,8 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
                         qk(tile, it + 1);
                     }
                 }
-                umma_commit(&B.vempty[it % C::VST]);
-                if (j + 1 < n) umma_commit(&B.kempty[(it + 1) % C::KST]);
+                umma_commit_if(lead, &B.vempty[it % C::VST]);
+                if (j + 1 < n) umma_commit_if(lead, &B.kempty[(it + 1) % C::KST]);
             }
         }
         } else if (warp == PR_MMA + 1 && lane == 0) {
