@@ -5,7 +5,7 @@
 // operand in tensor memory. The two tiles alternate: while the tensor cores multiply for one, eight warps (a thread per row)
 // do the softmax of the other. Tensor memory is full: two S of 128 columns (P, 16-bit, overwrites its own S) and two O.
 //
-// Four more warps turn the cache's codes into fp16 (exact) in the 128-byte swizzled layout, straight from global memory: a page's
+// Bulk copies bring a page's codes as they are; four more warps turn them into fp16 (exact) in the 128-byte swizzled layout: a page's
 // keys are rows of key_dim, its values rows of 64 tokens, so both are K-major operands without a transposition. Converting for
 // two tiles at once halves that work. The scales stay outside, as in the decode kernel: a block's key scale multiplies its
 // scores, its value scale 2^e goes into the exponent t = score + e, and out = sum 2^(t - M) code / sum 2^(t - M) 2^-e.
@@ -38,12 +38,15 @@ template <int DK, int DV> struct PrCfg {
     static constexpr int CHUNK = PR_TILE * 128;           // 128 rows x 128 bytes
     static constexpr int VCHUNK = DV * 128;               // a page of values
     static constexpr int Q = 2 * KC * CHUNK, K = KC * CHUNK, V = 2 * VCHUNK;
-    static constexpr int KST = DK == 192 ? 1 : 2, VST = 2;
-    static constexpr int SMEM = Q + KST * K + VST * V + 1024;
+    static constexpr int RK = 2 * KV_PAGE * DK, RV = 2 * KV_PAGE * DV;   // a step's codes as they are in the cache
+    static constexpr int KST = DK == 192 ? 1 : 2, VST = DK == 192 ? 1 : 2;
+    static constexpr int SMEM = Q + KST * K + VST * V + RK + RV + 1024;
+    static_assert(SMEM <= 227 * 1024 - 1536, "shared memory");
 };
 
 struct PrBars {
     uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sready[2], pready[2], pvdone[2], qfull[2], scfull[PR_SCALES], segfull[PR_SEGS], segempty[PR_SEGS];
+    uint64_t rkfull, rkempty, rvfull, rvempty;
     uint32_t tmem;
 };
 
@@ -236,6 +239,13 @@ __device__ __forceinline__ void codes_to_halves(uint4 c, uint4& lo, uint4& hi)
     hi = make_uint4(e4m3_halves(c.z), e4m3_halves(c.z >> 16), e4m3_halves(c.w), e4m3_halves(c.w >> 16));
 }
 
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
 __device__ __forceinline__ void st_shared16(uint32_t addr, uint4 v)
 {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
@@ -251,12 +261,14 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
     extern __shared__ uint8_t smem_raw[];
     __shared__ PrBars B;
     __shared__ float4 scales[PR_SCALES][8];               // of a step's blocks: key scale, value exponent, 1 / value scale
-    __shared__ unsigned long long spans[PR_SPANS];
     __shared__ PrPlace place;
     __shared__ PrSeg segs[PR_SEGS];
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform for the compiler
     uint8_t* smem = align1024(smem_raw);
     const uint32_t sq = smem_u32(smem), sk = sq + C::Q, sv = sk + C::KST * C::K;
+    uint8_t* const rawk = smem + C::Q + C::KST * C::K + C::VST * C::V;
+    uint8_t* const rawv = rawk + C::RK;
+    unsigned long long* const spans = reinterpret_cast<unsigned long long*>(smem);   // until the first query
     int* const status = p.c.status;
 
     if (threadIdx.x == 0) {
@@ -273,8 +285,12 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
         for (int i = 0; i < PR_SCALES; ++i) mbar_init(&B.scfull[i], 1);
         for (int i = 0; i < PR_SEGS; ++i) {
             mbar_init(&B.segfull[i], 1);
-            mbar_init(&B.segempty[i], 8 + PR_CONV + 1);
+            mbar_init(&B.segempty[i], 8 + PR_CONV + 2);
         }
+        mbar_init(&B.rkfull, 1);
+        mbar_init(&B.rvfull, 1);
+        mbar_init(&B.rkempty, PR_CONV);
+        mbar_init(&B.rvempty, PR_CONV);
         fence_barrier_init();
     }
     if (warp == PR_MMA) tmem_alloc(&B.tmem, 512);
@@ -507,127 +523,84 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
     } else if (warp < 8 + PR_CONV) {
         // ---- converters: 64-byte quarters of 8 rows per warp and load
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PR_REGS_CONV));
-        const int cw = warp - 8, unit = lane & 3, sub = cw * 8 + (lane >> 2);
-        uint4 kr[DK / 64][4], vr[2][DV / 32];
-        float4 mine = make_float4(1.0f, 0.0f, 1.0f, 0.0f);   // scales of block `lane` of the step (lanes 0 .. 7 of warp 8)
-        int pages = -1, pages_at = -64, pages_b = -1;        // lane l: page pages_at + l of sequence pages_b
-        uint32_t seg = 0;
-        int gb = 0, gh = 0, t = 0, t1 = 0, len = 0, pg[2] = {-1, -1};
-        // pages of step t
-        auto find = [&]() {
+        const int unit = lane & 3, sub = (warp - 8) * 8 + (lane >> 2);
+        // Eight lanes read and write 128 bytes without a bank conflict where two rows of a quarter are 64 or 192 bytes apart;
+        // rows of 128 bytes take the one half from the even and the other from the odd row.
+        const int odd = DK == 128 ? sub & 1 : 0;
+        const uint32_t u0 = sw128(sub, 2 * unit), u1 = sw128(sub, 2 * unit + 1);
+        uint32_t it = 0;
+        for (uint32_t seg = 0;; ++seg) {
+            const PrSeg& g = segment(seg);
+            const int t0 = g.t0, t1 = g.t1, len = g.s.len;
+            if (t1 == 0) break;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&B.segempty[seg % PR_SEGS]);
+            for (int t = t0; t < t1; ++t, ++it) {
+                const uint32_t ks = it % C::KST, vs = it % C::VST;
+                mbar_wait(&B.rkfull, it & 1, status);
+                mbar_wait(&B.kempty[ks], ((it / C::KST) & 1) ^ 1, status);
+#pragma unroll 1
+                for (int ch = 0; ch < DK / 64; ++ch) {
+                    const uint32_t src = smem_u32(rawk) + sub * DK + ((ch ^ odd) * 64 + unit * 16);
+                    const uint32_t dst = sk + ks * C::K + (ch ^ odd) * C::CHUNK;
+                    uint4 c[4];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int i = 2 * t + x;
-                if (gb != pages_b || i < pages_at || i >= pages_at + 32) {
-                    pages_b = gb;
-                    pages_at = i;
-                    const int want = i + lane;
-                    pages = static_cast<int64_t>(want) * KV_PAGE < len ? kv_page(p.c, p.b, gb, want, status) : -1;
-                }
-                pg[x] = __shfl_sync(0xffffffffu, pages, i - pages_at);
-            }
-        };
-        auto load_k = [&]() {
+                    for (int k = 0; k < 4; ++k) c[k] = ld_shared16(src + k * 32 * DK);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int r = sub + 32 * k, page = pg[k >> 1];   // row r: token r % 64 of page r / 64
-                const uint8_t* src = static_cast<const uint8_t*>(p.c.k) +
-                                     ((static_cast<int64_t>(max(page, 0)) * p.c.kv_heads + gh) * KV_PAGE + (r & 63)) * DK + unit * 16;
-#pragma unroll
-                for (int ch = 0; ch < DK / 64; ++ch)
-                    kr[ch][k] = page >= 0 ? *reinterpret_cast<const uint4*>(src + ch * 64) : make_uint4(0, 0, 0, 0);
-            }
-            if (cw == 0 && lane < 8) {
-                const int page = pg[lane >> 2];
-                mine = make_float4(1.0f, -INFINITY, 0.0f, 0.0f);   // no page: no weight
-                if (page >= 0) {
-                    const int64_t i = (static_cast<int64_t>(page) * p.c.kv_heads + gh) * KV_PAGE_BLOCKS + (lane & 3);
-                    const uint32_t ks = static_cast<const uint8_t*>(p.c.k_scale)[i];
-                    const uint32_t vs = min(max(static_cast<uint32_t>(static_cast<const uint8_t*>(p.c.v_scale)[i]), 1u), 253u);
-                    mine = make_float4(kv_scale(ks), static_cast<float>(static_cast<int>(vs) - 127),
-                                       __uint_as_float((254u - vs) << 23), 0.0f);
-                }
-            }
-        };
-        auto load_v = [&]() {
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const uint8_t* src = static_cast<const uint8_t*>(p.c.v) +
-                                     ((static_cast<int64_t>(max(pg[x], 0)) * p.c.kv_heads + gh) * DV + sub) * KV_PAGE + unit * 16;
-#pragma unroll
-                for (int k = 0; k < DV / 32; ++k)
-                    vr[x][k] = pg[x] >= 0 ? *reinterpret_cast<const uint4*>(src + k * 32 * KV_PAGE) : make_uint4(0, 0, 0, 0);
-                // behind the sequence's end a page may hold anything, NaN codes too, and 0 x NaN would count
-                const int live = len - (2 * t + x) * KV_PAGE - unit * 16;
-                if (live < 16) {
-                    uint32_t keep[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int n = live - 4 * e;
-                        keep[e] = n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
-                    }
-#pragma unroll
-                    for (int k = 0; k < DV / 32; ++k) {
-                        vr[x][k].x &= keep[0];
-                        vr[x][k].y &= keep[1];
-                        vr[x][k].z &= keep[2];
-                        vr[x][k].w &= keep[3];
+                    for (int k = 0; k < 4; ++k) {
+                        uint4 a, b;
+                        codes_to_halves(c[k], a, b);
+                        st_shared16(dst + k * 32 * 128 + u0, a);
+                        st_shared16(dst + k * 32 * 128 + u1, b);
                     }
                 }
-            }
-        };
-        for (uint32_t it = 0;; ++it) {
-            // step `it`: keys on their way, then the values of the step before into shared memory, and so on in turn
-            if (it == 0 || ++t == t1) {
-                const PrSeg& g = segment(seg);
-                gb = g.b, gh = g.h, t = g.t0, t1 = g.t1, len = g.s.len;
-                if (t1 != 0) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&B.segempty[seg % PR_SEGS]);
-                    ++seg;
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&B.kfull[ks]);
+                    mbar_arrive(&B.rkempty);
                 }
-            }
-            const bool more = t1 != 0;
-            if (more) {
-                find();
-                load_k();
-            }
-            if (it > 0) {
-                const uint32_t vs = (it - 1) % C::VST;
-                mbar_wait(&B.vempty[vs], (((it - 1) / C::VST) & 1) ^ 1, status);
+                mbar_wait(&B.rvfull, it & 1, status);
+                mbar_wait(&B.vempty[vs], ((it / C::VST) & 1) ^ 1, status);
+#pragma unroll 1
+                for (int x = 0; x < 2; ++x) {
+                    const uint32_t src = smem_u32(rawv) + (x * DV + sub) * KV_PAGE + unit * 16;
+                    const uint32_t dst = sv + vs * C::V + x * C::VCHUNK;
+                    uint4 c[DV / 32];
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
+                    for (int k = 0; k < DV / 32; ++k) c[k] = ld_shared16(src + k * 32 * KV_PAGE);
+                    // behind the sequence's end a page may hold anything, NaN codes too, and 0 x NaN would count
+                    const int live = len - (2 * t + x) * KV_PAGE - unit * 16;
+                    if (__any_sync(0xffffffffu, live < 16)) {
+                        uint32_t keep[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int n = live - 4 * e;
+                            keep[e] = n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+                        }
+#pragma unroll
+                        for (int k = 0; k < DV / 32; ++k) {
+                            c[k].x &= keep[0];
+                            c[k].y &= keep[1];
+                            c[k].z &= keep[2];
+                            c[k].w &= keep[3];
+                        }
+                    }
 #pragma unroll
                     for (int k = 0; k < DV / 32; ++k) {
                         uint4 a, b;
-                        codes_to_halves(vr[x][k], a, b);
-                        const uint32_t dst = sv + vs * C::V + x * C::VCHUNK;
-                        st_shared16(dst + sw128(sub + 32 * k, 2 * unit), a);
-                        st_shared16(dst + sw128(sub + 32 * k, 2 * unit + 1), b);
+                        codes_to_halves(c[k], a, b);
+                        st_shared16(dst + k * 32 * 128 + u0, a);
+                        st_shared16(dst + k * 32 * 128 + u1, b);
                     }
+                }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&B.vfull[vs]);
-            }
-            if (!more) break;
-            load_v();
-            const uint32_t ks = it % C::KST;
-            mbar_wait(&B.kempty[ks], ((it / C::KST) & 1) ^ 1, status);
-#pragma unroll
-            for (int ch = 0; ch < DK / 64; ++ch)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    uint4 a, b;
-                    codes_to_halves(kr[ch][k], a, b);
-                    const uint32_t dst = sk + ks * C::K + ch * C::CHUNK;
-                    st_shared16(dst + sw128(sub + 32 * k, 2 * unit), a);
-                    st_shared16(dst + sw128(sub + 32 * k, 2 * unit + 1), b);
+                if (lane == 0) {
+                    mbar_arrive(&B.vfull[vs]);
+                    mbar_arrive(&B.rvempty);
                 }
-            if (cw == 0 && lane < 8) scales[it % PR_SCALES][lane] = mine;
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&B.kfull[ks]);
-            if (cw == 0 && lane == 0) mbar_arrive(&B.scfull[it % PR_SCALES]);
+            }
         }
     } else {
         // ---- MMA issue: a whole warp walks through, so that descriptors stay in uniform registers, and one lane issues
@@ -688,8 +661,85 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
                 if (j + 1 < n) umma_commit_if(lead, &B.kempty[(it + 1) % C::KST]);
             }
         }
+        } else if (warp == PR_MMA + 2) {
+            // ---- copies: a step's pages into shared memory as they are, and its blocks' scales
+            int pages = -1, pages_at = -64, pages_b = -1;   // lane l: page pages_at + l of sequence pages_b
+            uint32_t it = 0;
+            float4 mine = make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
+            for (uint32_t seg = 0;; ++seg) {
+                const PrSeg& g = segment(seg);
+                const int b = g.b, h = g.h, t0 = g.t0, t1 = g.t1, len = g.s.len;
+                if (t1 == 0) break;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&B.segempty[seg % PR_SEGS]);
+                for (int t = t0; t < t1; ++t, ++it) {
+                    int pg[2];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int i = 2 * t + x;
+                        if (b != pages_b || i < pages_at || i >= pages_at + 32) {
+                            pages_b = b;
+                            pages_at = i;
+                            const int want = i + lane;
+                            pages = static_cast<int64_t>(want) * KV_PAGE < len ? kv_page(p.c, p.b, b, want, status) : -1;
+                        }
+                        pg[x] = __shfl_sync(0xffffffffu, pages, i - pages_at);
+                    }
+                    // a page that is not there: codes of zero and no weight
+                    if (lane < 8) {
+                        const int page = pg[lane >> 2];
+                        mine = make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
+                        if (page >= 0) {
+                            const int64_t i = (static_cast<int64_t>(page) * p.c.kv_heads + h) * KV_PAGE_BLOCKS + (lane & 3);
+                            const uint32_t ks = static_cast<const uint8_t*>(p.c.k_scale)[i];
+                            const uint32_t vs = min(max(static_cast<uint32_t>(static_cast<const uint8_t*>(p.c.v_scale)[i]), 1u), 253u);
+                            mine = make_float4(kv_scale(ks), static_cast<float>(static_cast<int>(vs) - 127),
+                                               __uint_as_float((254u - vs) << 23), 0.0f);
+                        }
+                    }
+                    mbar_wait(&B.rkempty, (it & 1) ^ 1, status);
+                    if (pg[0] < 0 || pg[1] < 0) {
+                        for (int x = 0; x < 2; ++x)
+                            if (pg[x] < 0)
+                                for (int i = lane; i < KV_PAGE * DK / 16; i += 32)
+                                    st_shared16(smem_u32(rawk) + x * KV_PAGE * DK + i * 16, make_uint4(0, 0, 0, 0));
+                        __syncwarp();
+                    }
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&B.rkfull, ((pg[0] >= 0) + (pg[1] >= 0)) * KV_PAGE * DK);
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+                            if (pg[x] >= 0)
+                                bulk_g2s(rawk + x * KV_PAGE * DK,
+                                         static_cast<const uint8_t*>(p.c.k) + (static_cast<int64_t>(pg[x]) * p.c.kv_heads + h) * KV_PAGE * DK,
+                                         KV_PAGE * DK, &B.rkfull);
+                    }
+                    __syncwarp();
+                    mbar_wait(&B.rvempty, (it & 1) ^ 1, status);
+                    if (pg[0] < 0 || pg[1] < 0) {
+                        for (int x = 0; x < 2; ++x)
+                            if (pg[x] < 0)
+                                for (int i = lane; i < KV_PAGE * DV / 16; i += 32)
+                                    st_shared16(smem_u32(rawv) + x * KV_PAGE * DV + i * 16, make_uint4(0, 0, 0, 0));
+                        __syncwarp();
+                    }
+                    if (lane < 8) scales[it % PR_SCALES][lane] = mine;
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&B.rvfull, ((pg[0] >= 0) + (pg[1] >= 0)) * KV_PAGE * DV);
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+                            if (pg[x] >= 0)
+                                bulk_g2s(rawv + x * KV_PAGE * DV,
+                                         static_cast<const uint8_t*>(p.c.v) + (static_cast<int64_t>(pg[x]) * p.c.kv_heads + h) * KV_PAGE * DV,
+                                         KV_PAGE * DV, &B.rvfull);
+                        mbar_arrive(&B.scfull[it % PR_SCALES]);
+                    }
+                    __syncwarp();
+                }
+            }
         } else if (warp == PR_MMA + 1 && lane == 0) {
-            // the segments of the piece
+            // ---- the segments of the piece
             int b = place.b, h = place.h, qb = place.qb, off = place.off, left = place.left, done = 0;
             KvSeq s = left > 0 ? kv_seq(p.b, b, status) : KvSeq{0, 0, 0, 0};
             for (uint32_t i = 0;; ++i) {
