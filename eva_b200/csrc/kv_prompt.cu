@@ -25,30 +25,38 @@
 
 namespace eva {
 
-constexpr int PR_TILE = 128, PR_ROWS = 2 * PR_TILE;       // rows of a tile, of a CTA; tokens of a step
-// Four warpgroups: 8 softmax warps, 4 converter warps, the MMA warp (and three idle ones). Registers move to the
-// softmax threads, which hold a row's 128 scores: 2 x 184 + 96 + 48 = 4 x 128, the launch's own.
+constexpr int PR_TILE = 128, PR_ROWS = 2 * PR_TILE;       // rows of a tile, of a CTA
+constexpr int PR_STEP = KV_PAGE;                          // tokens of a step
+// Four warpgroups: 8 softmax warps, 4 converter warps, two that issue the MMAs, one each for
+// the segments and the copies.
 constexpr int PR_CONV = 4, PR_MMA = 8 + PR_CONV, PR_WARPS = 16;
-constexpr int PR_REGS_SOFTMAX = 184, PR_REGS_CONV = 96, PR_REGS_MMA = 48;
 constexpr float PR_BIAS = 7.0f, PR_SLACK = 8.0f;
-constexpr int PR_SCALES = 4, PR_SEGS = 4;                 // steps whose scales are kept, segments in flight
+constexpr int PR_SCALES = 8, PR_SEGS = 4;                 // steps whose scales are kept, segments in flight
 
 template <int DK, int DV> struct PrCfg {
     static constexpr int KC = DK / 64;                    // 64-element chunks of a query or key row
-    static constexpr int CHUNK = PR_TILE * 128;           // 128 rows x 128 bytes
-    static constexpr int VCHUNK = DV * 128;               // a page of values
-    static constexpr int Q = 2 * KC * CHUNK, K = KC * CHUNK, V = 2 * VCHUNK;
-    static constexpr int RK = 2 * KV_PAGE * DK, RV = 2 * KV_PAGE * DV;   // a step's codes as they are in the cache
-    static constexpr int KST = DK == 192 ? 1 : 2, VST = DK == 192 ? 1 : 2;
-    static constexpr int SMEM = Q + KST * K + VST * V + RK + RV + 1024;
-    static_assert(SMEM <= 227 * 1024 - 1536, "shared memory");
+    static constexpr int QCHUNK = PR_TILE * 128, KCHUNK = PR_STEP * 128;   // rows x 128 bytes
+    static constexpr int Q = 2 * KC * QCHUNK, K = KC * KCHUNK, V = DV * 128;
+    static constexpr int RK = PR_STEP * DK, RV = PR_STEP * DV;   // a step's codes as they are in the cache
+    static constexpr int KST = 3, VST = DK == 192 ? 2 : 3, RST = DK == 192 ? 1 : 2;   // stages
+    static constexpr int SMEM = Q + KST * K + VST * V + RST * (RK + RV) + 1024;
+    static_assert(SMEM <= 227 * 1024 - 2048, "shared memory");
 };
 
 struct PrBars {
-    uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sready[2], pready[2], pvdone[2], qfull[2], scfull[PR_SCALES], segfull[PR_SEGS], segempty[PR_SEGS];
-    uint64_t rkfull, rkempty, rvfull, rvempty;
+    uint64_t kfull[3], kempty[3], vfull[3], vempty[3], rkfull[2], rkempty[2], rvfull[2], rvempty[2];
+    uint64_t sready[2][2], pready[2][2], pvdone[2][2], qfull[2];   // [tile][step & 1]
+    uint64_t scfull[PR_SCALES], segfull[PR_SEGS], segempty[PR_SEGS];
     uint32_t tmem;
 };
+
+// mbar_wait with the waiting itself out of line: code that a warp runs once a step has to stay short.
+__device__ __noinline__ void wait_long(uint64_t* bar, uint32_t parity, int* status) { mbar_wait(bar, parity, status); }
+
+__device__ __forceinline__ void wait_on(uint64_t* bar, uint32_t parity, int* status)
+{
+    if (!mbar_try_wait(bar, parity)) wait_long(bar, parity, status);
+}
 
 // Row block qb of a sequence: its rows' tokens, the token range they see and the steps over it.
 struct PrItem {
@@ -61,8 +69,8 @@ __device__ __forceinline__ PrItem pr_item(const KvSeq& s, int group, int window,
     PrItem it;
     it.hi = max(s.ctx + r1 / group + 1, 0);
     it.lo = window > 0 ? max(0, s.ctx + r0 / group + 1 - window) : 0;
-    it.t0 = it.lo / PR_TILE;
-    it.tiles = it.hi > 0 ? (it.hi + PR_TILE - 1) / PR_TILE - it.t0 : 1;
+    it.t0 = it.lo / PR_STEP;
+    it.tiles = it.hi > 0 ? (it.hi + PR_STEP - 1) / PR_STEP - it.t0 : 1;
     return it;
 }
 
@@ -179,32 +187,26 @@ __device__ __forceinline__ void add2(float& x, float& y, float a, float b)
         : "f"(a), "f"(b));
 }
 
-// Largest t = score * scale + exponent over a step's scores r; with MASK over those that are seen (bit i of the words)
-template <bool MASK>
-__device__ __forceinline__ float pr_max(const uint32_t (&r)[128], const float4* sc, float c, int lo, int hi)
+// Largest t = score * scale + exponent of a step's scores
+__device__ __forceinline__ float pr_max(const uint32_t (&r)[64], const float4* sc, float c)
 {
     float mx = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
+    for (int x = 0; x < 4; ++x) {
         float b = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float v = __uint_as_float(r[16 * x + i]);
-            b = fmaxf(b, !MASK || (16 * x + i >= lo && 16 * x + i < hi) ? v : -INFINITY);
-        }
+        for (int i = 0; i < 16; ++i) b = fmaxf(b, __uint_as_float(r[16 * x + i]));
         mx = fmaxf(mx, fmaf(b, sc[x].x * c, sc[x].y));
     }
     return mx;
 }
 
-// Weights 2^(t + ref) of a step's scores as fp16 into tensor memory (over the scores); returns their sum, each divided
-// by its value scale. CAREFUL: with the mask, and rounding t as pr_max did.
-template <bool CAREFUL>
-__device__ __forceinline__ float pr_weights(const uint32_t (&r)[128], const float4* sc, float c, float ref, int lo, int hi, uint32_t ts)
+// Weights 2^(t + ref) as fp16 into tensor memory (over the scores); returns their sum, each divided by its value scale.
+__device__ __forceinline__ float pr_weights(const uint32_t (&r)[64], const float4* sc, float c, float ref, uint32_t ts)
 {
     float l = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 2; ++k) {
         uint32_t w[16];
 #pragma unroll
         for (int x = 2 * k; x < 2 * k + 2; ++x) {
@@ -213,13 +215,8 @@ __device__ __forceinline__ float pr_weights(const uint32_t (&r)[128], const floa
             float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
             for (int i = 16 * x; i < 16 * x + 16; i += 2) {
-                float a = __uint_as_float(r[i]), b = __uint_as_float(r[i + 1]);
-                if constexpr (CAREFUL) {
-                    a = i >= lo && i < hi ? fmaf(a, fc, f.y) + ref : -INFINITY;
-                    b = i + 1 >= lo && i + 1 < hi ? fmaf(b, fc, f.y) + ref : -INFINITY;
-                } else {
-                    fma2(a, b, a, b, fc, add);
-                }
+                float a, b;
+                fma2(a, b, __uint_as_float(r[i]), __uint_as_float(r[i + 1]), fc, add);
                 a = ex2(a);
                 b = ex2(b);
                 add2(s0, s1, a, b);
@@ -228,6 +225,47 @@ __device__ __forceinline__ float pr_weights(const uint32_t (&r)[128], const floa
             l = fmaf(s0 + s1, f.z, l);
         }
         tmem_st16(ts + 16 * k, w);
+    }
+    return l;
+}
+
+// The same two for a step of which a row sees tokens lo .. hi - 1 only, or whose scores lie far from 0, where M must be rounded as
+// t is, else their difference is not small at the largest: 16 columns at a time, since this is seldom run and long code would
+// come from memory.
+__device__ __noinline__ float pr_max_masked(uint32_t ts, const float4* sc, float c, int lo, int hi)
+{
+    float mx = -INFINITY;
+#pragma unroll 1
+    for (int x = 0; x < 4; ++x) {
+        uint32_t r[16];
+        tmem_ld32x32_x16(ts + 16 * x, r);
+        const float fc = sc[x].x * c, add = sc[x].y;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            mx = fmaxf(mx, 16 * x + i >= lo && 16 * x + i < hi ? fmaf(__uint_as_float(r[i]), fc, add) : -INFINITY);
+    }
+    return mx;
+}
+
+__device__ __noinline__ float pr_weights_masked(uint32_t ts, const float4* sc, float c, float ref, int lo, int hi)
+{
+    float l = 0.0f;
+#pragma unroll 1
+    for (int x = 0; x < 4; ++x) {
+        uint32_t r[16], w[8];
+        tmem_ld32x32_x16(ts + 16 * x, r);
+        const float4 f = sc[x];
+        const float fc = f.x * c;
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const float a = 16 * x + i >= lo && 16 * x + i < hi ? ex2(fmaf(__uint_as_float(r[i]), fc, f.y) + ref) : 0.0f;
+            const float b = 16 * x + i + 1 >= lo && 16 * x + i + 1 < hi ? ex2(fmaf(__uint_as_float(r[i + 1]), fc, f.y) + ref) : 0.0f;
+            s += a + b;
+            w[i / 2] = half2_bits(a, b);
+        }
+        l = fmaf(s, f.z, l);
+        tmem_st32x32_x8(ts + 8 * x, w);
     }
     return l;
 }
@@ -260,37 +298,41 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
     using C = PrCfg<DK, DV>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ PrBars B;
-    __shared__ float4 scales[PR_SCALES][8];               // of a step's blocks: key scale, value exponent, 1 / value scale
+    __shared__ float4 scales[PR_SCALES][4];               // of a step's blocks: key scale, value exponent, 1 / value scale
     __shared__ PrPlace place;
     __shared__ PrSeg segs[PR_SEGS];
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform for the compiler
     uint8_t* smem = align1024(smem_raw);
     const uint32_t sq = smem_u32(smem), sk = sq + C::Q, sv = sk + C::KST * C::K;
     uint8_t* const rawk = smem + C::Q + C::KST * C::K + C::VST * C::V;
-    uint8_t* const rawv = rawk + C::RK;
+    uint8_t* const rawv = rawk + C::RST * C::RK;
     unsigned long long* const spans = reinterpret_cast<unsigned long long*>(smem);   // until the first query
     int* const status = p.c.status;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 3; ++i) {
             mbar_init(&B.kfull[i], PR_CONV);
-            mbar_init(&B.kempty[i], 1);
+            mbar_init(&B.kempty[i], 2);
             mbar_init(&B.vfull[i], PR_CONV);
-            mbar_init(&B.vempty[i], 1);
-            mbar_init(&B.sready[i], 1);
-            mbar_init(&B.pready[i], 4);
-            mbar_init(&B.pvdone[i], 1);
+            mbar_init(&B.vempty[i], 2);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&B.rkfull[i], 1);
+            mbar_init(&B.rvfull[i], 1);
+            mbar_init(&B.rkempty[i], PR_CONV);
+            mbar_init(&B.rvempty[i], PR_CONV);
+            for (int j = 0; j < 2; ++j) {
+                mbar_init(&B.sready[i][j], 1);
+                mbar_init(&B.pready[i][j], 4);
+                mbar_init(&B.pvdone[i][j], 1);
+            }
             mbar_init(&B.qfull[i], 4);
         }
         for (int i = 0; i < PR_SCALES; ++i) mbar_init(&B.scfull[i], 1);
         for (int i = 0; i < PR_SEGS; ++i) {
             mbar_init(&B.segfull[i], 1);
-            mbar_init(&B.segempty[i], 8 + PR_CONV + 2);
+            mbar_init(&B.segempty[i], 8 + PR_CONV + 3);
         }
-        mbar_init(&B.rkfull, 1);
-        mbar_init(&B.rvfull, 1);
-        mbar_init(&B.rkempty, PR_CONV);
-        mbar_init(&B.rvempty, PR_CONV);
         fence_barrier_init();
     }
     if (warp == PR_MMA) tmem_alloc(&B.tmem, 512);
@@ -361,143 +403,107 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
     const uint32_t tmem = B.tmem;
     // Segment i of the piece, for every lane of a warp (or the one thread that calls)
     auto segment = [&](uint32_t i) -> const PrSeg& {
-        mbar_wait(&B.segfull[i % PR_SEGS], (i / PR_SEGS) & 1, status);
+        wait_on(&B.segfull[i % PR_SEGS], (i / PR_SEGS) & 1, status);
         return segs[i % PR_SEGS];
     };
 
     if (warp < 8) {
         // ---- softmax: thread = row of tile `tile`
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PR_REGS_SOFTMAX));
         const int tile = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + lanes + tile * PR_TILE, to = tmem + lanes + 2 * PR_TILE + tile * DV;
-        uint32_t it = 0, seg = 0;             // steps and segments so far
-        uint4 raw[DK / 8];                    // the row's query
-        int pos = 0, t0 = 0, t1 = 0;          // position of the row, -1 - pos where it is behind the sequence
-        T* dst = nullptr;                     // its output, or partial sums
-        bool in = false, whole = false;
+        const uint32_t tsc = tmem + lanes + tile * PR_TILE, to = tmem + lanes + 2 * PR_TILE + tile * DV;
+        uint32_t it = 0;                      // steps so far
         if (threadIdx.x == 0) p.heads_of[blockIdx.x] = make_int4(-1, 0, 0, 0);
-        // takes the next segment's row up (its loads are under way when this returns)
-        auto take = [&]() -> bool {
+        for (uint32_t seg = 0;; ++seg) {
             const PrSeg& g = segment(seg);
-            t0 = g.t0;
-            t1 = g.t1;
-            if (t1 == 0) return false;
+            const int t0 = g.t0, t1 = g.t1;
+            if (t1 == 0) break;
             const int r = g.qb * PR_ROWS + tile * PR_TILE + row, tok = r / p.group, qh = g.h * p.group + (r - tok * p.group);
-            in = tok < g.s.n;
-            pos = g.s.ctx + tok;
-            whole = g.first && g.after == 0;
+            const bool in = tok < g.s.n, whole = g.first && g.after == 0;
             const int64_t qrow = static_cast<int64_t>(g.s.row0) + tok;
-            if (whole)
-                dst = static_cast<T*>(p.out) + (qrow * p.heads + qh) * DV;
-            else
-                dst = reinterpret_cast<T*>(p.part + (static_cast<int64_t>(blockIdx.x) * 2 + g.first) * PR_ROWS * (DV + 2));
+            // rows without a token see nothing; rows behind the sequence are not written and need no mask
+            const int hi = in ? g.s.ctx + tok + 1 : 0x7fffffff, lo = in && p.window > 0 ? max(hi - p.window, 0) : 0;
+            // its output, or its piece's partial sums
+            T* const out = static_cast<T*>(p.out) + (qrow * p.heads + qh) * DV;
+            float* const part = p.part + (static_cast<int64_t>(blockIdx.x) * 2 + g.first) * PR_ROWS * (DV + 2);
             if (threadIdx.x == 0 && g.first && g.after > 0)
                 p.heads_of[blockIdx.x] =
                     make_int4(g.b, g.h, g.qb,
                               static_cast<int>(((place.begin + g.done + (t1 - t0) + g.after) * place.pieces - 1) / place.total));
-            const T* q = static_cast<const T*>(p.q) + qrow * p.qt + static_cast<int64_t>(qh) * p.qh;
-#pragma unroll
-            for (int u = 0; u < DK / 8; ++u) raw[u] = in ? *reinterpret_cast<const uint4*>(q + u * 8) : make_uint4(0, 0, 0, 0);
             __syncwarp();
             if (lane == 0) mbar_arrive(&B.segempty[seg % PR_SEGS]);
-            ++seg;
-            return true;
-        };
-        float m = 0.0f, l = 0.0f;
-        for (bool pending = false;; pending = true) {
-            const bool was_whole = whole, was_in = in;
-            T* const out = dst;
-            const bool more = take();
-            if (pending) {
-                // the row block's output, or its partial sums, while the next query is on its way
-                mbar_wait(&B.pvdone[tile], (it - 1) & 1, status);
-                tc_fence_after();
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                const int pr = tile * PR_TILE + row;
-                float* part = reinterpret_cast<float*>(out);
-                if (!was_whole && was_in) {
-                    part[pr] = m;
-                    part[PR_ROWS + pr] = l;
-                }
-                float* po = part + 2 * PR_ROWS + pr * DV;
+            // the row, scaled by a power of two to [1, 2) at its largest, as fp16
+            float c;
+            {
+                const T* q = static_cast<const T*>(p.q) + qrow * p.qt + static_cast<int64_t>(qh) * p.qh;
+                float big = 0.0f;
+                bool odd = false;
 #pragma unroll 1
-                for (int k = 0; k < DV; k += 32) {
-                    float v[32];
-                    __syncwarp();
-                    tmem_ld32(to + k, v);
-                    if (was_in && was_whole) {
+                for (int u = 0; u < DK / 8; u += 8) {
+                    uint4 raw[8];
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8)
-                            *reinterpret_cast<uint4*>(out + k + i) =
-                                make_uint4(two_bits<T>(v[i] * inv, v[i + 1] * inv), two_bits<T>(v[i + 2] * inv, v[i + 3] * inv),
-                                           two_bits<T>(v[i + 4] * inv, v[i + 5] * inv), two_bits<T>(v[i + 6] * inv, v[i + 7] * inv));
-                    } else if (was_in) {
+                    for (int k = 0; k < 8; ++k) raw[k] = in ? *reinterpret_cast<const uint4*>(q + (u + k) * 8) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<float4*>(po + k + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                    for (int k = 0; k < 8; ++k) {
+                        const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 f = two_floats<T>(w[e]);
+                            big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+                            odd |= f.x != f.x || f.y != f.y;
+                        }
                     }
                 }
-                tc_fence_before();
-            }
-            if (!more) break;
-            // the row, scaled by a power of two to [1, 2) at its largest, as fp16
-            float c, big = 0.0f;
-            bool odd = false;
+                odd |= big == INFINITY;
+                const int e2 = min(max(static_cast<int>(__float_as_uint(big) >> 23), 1), 252);
+                const float down = __uint_as_float(static_cast<uint32_t>(254 - e2) << 23);
+                c = odd ? __uint_as_float(0x7fc00000u) : p.scale * __uint_as_float(static_cast<uint32_t>(e2) << 23);
+#pragma unroll 2
+                for (int u = 0; u < DK / 8; ++u) {
+                    const uint4 raw = in ? *reinterpret_cast<const uint4*>(q + u * 8) : make_uint4(0, 0, 0, 0);
+                    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+                    uint32_t o[4];
 #pragma unroll
-            for (int u = 0; u < DK / 8; ++u) {
-                const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 f = two_floats<T>(w[e]);
-                    big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
-                    odd |= f.x != f.x || f.y != f.y;
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 f = two_floats<T>(w[e]);
+                        o[e] = half2_bits(f.x * down, f.y * down);
+                    }
+                    st_shared16(sq + (tile * C::KC + u / 8) * C::QCHUNK + sw128(row, u % 8), make_uint4(o[0], o[1], o[2], o[3]));
                 }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&B.qfull[tile]);
             }
-            odd |= big == INFINITY;
-            const int e2 = min(max(static_cast<int>(__float_as_uint(big) >> 23), 1), 252);
-            const float down = __uint_as_float(static_cast<uint32_t>(254 - e2) << 23);
-            c = odd ? __uint_as_float(0x7fc00000u) : p.scale * __uint_as_float(static_cast<uint32_t>(e2) << 23);
-#pragma unroll
-            for (int u = 0; u < DK / 8; ++u) {
-                const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-                uint32_t o[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 f = two_floats<T>(w[e]);
-                    o[e] = half2_bits(f.x * down, f.y * down);
-                }
-                st_shared16(sq + (tile * C::KC + u / 8) * C::CHUNK + sw128(row, u % 8), make_uint4(o[0], o[1], o[2], o[3]));
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&B.qfull[tile]);
-            // rows without a token see nothing; rows behind the sequence are not written and need no mask
-            const int hi = in ? pos + 1 : 0x7fffffff, lo = in && p.window > 0 ? max(hi - p.window, 0) : 0;
             const int all_hi = __reduce_min_sync(0xffffffffu, hi), all_lo = __reduce_max_sync(0xffffffffu, lo);
-            m = -INFINITY, l = 0.0f;
-            const int first = t0;
+            float m = -INFINITY, l = 0.0f;
+#pragma unroll 1
             for (int t = t0; t < t1; ++t, ++it) {
                 const float4* sc = scales[it % PR_SCALES];
-                const int tok0 = t * PR_TILE;
-                const bool part = tok0 + PR_TILE > all_hi || tok0 < all_lo;
-                mbar_wait(&B.scfull[it % PR_SCALES], (it / PR_SCALES) & 1, status);
-                mbar_wait(&B.sready[tile], it & 1, status);
+                const uint32_t ts = tsc + (it & 1) * PR_STEP;
+                const int tok0 = t * PR_STEP;
+                const bool part_seen = tok0 + PR_STEP > all_hi || tok0 < all_lo;
+                wait_on(&B.scfull[it % PR_SCALES], (it / PR_SCALES) & 1, status);
+                wait_on(&B.sready[tile][it & 1], (it >> 1) & 1, status);
                 tc_fence_after();
-                uint32_t v[128];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) tmem_ld32_async(ts + 32 * k, v + 32 * k);
-                tmem_wait_ld();
-#pragma unroll
-                for (int k = 0; k < 4; ++k) tied(v + 32 * k);
-                const float mx = part ? pr_max<true>(v, sc, c, lo - tok0, hi - tok0) : pr_max<false>(v, sc, c, 0, 0);
+                uint32_t v[64];
+                float mx;
+                if (!part_seen) {
+                    tmem_ld32_async(ts, v);
+                    tmem_ld32_async(ts + 32, v + 32);
+                    tmem_wait_ld();
+                    tied(v);
+                    tied(v + 32);
+                    mx = pr_max(v, sc, c);
+                } else {
+                    mx = pr_max_masked(ts, sc, c, lo - tok0, hi - tok0);
+                }
                 const bool grow = mx > m + PR_SLACK || (m == -INFINITY && mx > m);
                 if (__any_sync(0xffffffffu, grow)) {
                     const float fall = grow ? ex2(m - mx) : 1.0f;
                     if (grow) m = mx;
                     l *= fall;
-                    if (t > first) {
-                        mbar_wait(&B.pvdone[tile], (it - 1) & 1, status);
+                    if (t > t0) {
+                        wait_on(&B.pvdone[tile][(it - 1) & 1], ((it - 1) >> 1) & 1, status);
                         tc_fence_after();
 #pragma unroll 1
                         for (int k = 0; k < DV; k += 16) {
@@ -510,19 +516,47 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
                     }
                 }
                 const float ref = PR_BIAS - (m == -INFINITY ? 0.0f : m);
-                // far from 0 the rounding of M must be the score's own, else their difference is not small at the largest
-                const bool careful = part || __any_sync(0xffffffffu, m != -INFINITY && fabsf(m) > 4096.0f);
-                l += careful ? pr_weights<true>(v, sc, c, ref, part ? lo - tok0 : 0, part ? hi - tok0 : PR_TILE, ts)
-                             : pr_weights<false>(v, sc, c, ref, 0, 0, ts);
+                if (!part_seen && !__any_sync(0xffffffffu, m != -INFINITY && fabsf(m) > 4096.0f))
+                    l += pr_weights(v, sc, c, ref, ts);
+                else
+                    l += pr_weights_masked(ts, sc, c, ref, lo - tok0, hi - tok0);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&B.pready[tile]);
+                if (lane == 0) mbar_arrive(&B.pready[tile][it & 1]);
             }
+            wait_on(&B.pvdone[tile][(it - 1) & 1], ((it - 1) >> 1) & 1, status);
+            tc_fence_after();
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const int pr = tile * PR_TILE + row;
+            if (!whole && in) {
+                part[pr] = m;
+                part[PR_ROWS + pr] = l;
+            }
+#pragma unroll 1
+            for (int k = 0; k < DV; k += 16) {
+                uint32_t v[16];
+                __syncwarp();
+                tmem_ld32x32_x16(to + k, v);
+                if (in && whole) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 8) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            w[e] = two_bits<T>(__uint_as_float(v[i + 2 * e]) * inv, __uint_as_float(v[i + 2 * e + 1]) * inv);
+                        *reinterpret_cast<uint4*>(out + k + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                } else if (in) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4)
+                        *reinterpret_cast<uint4*>(part + 2 * PR_ROWS + pr * DV + k + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                }
+            }
+            tc_fence_before();
         }
     } else if (warp < 8 + PR_CONV) {
         // ---- converters: 64-byte quarters of 8 rows per warp and load
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PR_REGS_CONV));
         const int unit = lane & 3, sub = (warp - 8) * 8 + (lane >> 2);
         // Eight lanes read and write 128 bytes without a bank conflict where two rows of a quarter are 64 or 192 bytes apart;
         // rows of 128 bytes take the one half from the even and the other from the odd row.
@@ -535,42 +569,43 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
             if (t1 == 0) break;
             __syncwarp();
             if (lane == 0) mbar_arrive(&B.segempty[seg % PR_SEGS]);
-            for (int t = t0; t < t1; ++t, ++it) {
-                const uint32_t ks = it % C::KST, vs = it % C::VST;
-                mbar_wait(&B.rkfull, it & 1, status);
-                mbar_wait(&B.kempty[ks], ((it / C::KST) & 1) ^ 1, status);
 #pragma unroll 1
-                for (int ch = 0; ch < DK / 64; ++ch) {
-                    const uint32_t src = smem_u32(rawk) + sub * DK + ((ch ^ odd) * 64 + unit * 16);
-                    const uint32_t dst = sk + ks * C::K + (ch ^ odd) * C::CHUNK;
-                    uint4 c[4];
+            for (int t = t0; t < t1; ++t, ++it) {
+                const uint32_t ks = it % C::KST, vs = it % C::VST, rs = it % C::RST;
+                wait_on(&B.rkfull[rs], (it / C::RST) & 1, status);
+                wait_on(&B.kempty[ks], ((it / C::KST) & 1) ^ 1, status);
+                {
+                    const uint32_t src = smem_u32(rawk) + rs * C::RK + sub * DK + unit * 16, dst = sk + ks * C::K;
+                    uint4 c[C::KC][2];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) c[k] = ld_shared16(src + k * 32 * DK);
+                    for (int ch = 0; ch < C::KC; ++ch)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        uint4 a, b;
-                        codes_to_halves(c[k], a, b);
-                        st_shared16(dst + k * 32 * 128 + u0, a);
-                        st_shared16(dst + k * 32 * 128 + u1, b);
-                    }
+                        for (int k = 0; k < 2; ++k) c[ch][k] = ld_shared16(src + (ch ^ odd) * 64 + k * 32 * DK);
+#pragma unroll
+                    for (int ch = 0; ch < C::KC; ++ch)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            uint4 a, b;
+                            codes_to_halves(c[ch][k], a, b);
+                            st_shared16(dst + (ch ^ odd) * C::KCHUNK + k * 32 * 128 + u0, a);
+                            st_shared16(dst + (ch ^ odd) * C::KCHUNK + k * 32 * 128 + u1, b);
+                        }
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(&B.kfull[ks]);
-                    mbar_arrive(&B.rkempty);
+                    mbar_arrive(&B.rkempty[rs]);
                 }
-                mbar_wait(&B.rvfull, it & 1, status);
-                mbar_wait(&B.vempty[vs], ((it / C::VST) & 1) ^ 1, status);
-#pragma unroll 1
-                for (int x = 0; x < 2; ++x) {
-                    const uint32_t src = smem_u32(rawv) + (x * DV + sub) * KV_PAGE + unit * 16;
-                    const uint32_t dst = sv + vs * C::V + x * C::VCHUNK;
+                wait_on(&B.rvfull[rs], (it / C::RST) & 1, status);
+                wait_on(&B.vempty[vs], ((it / C::VST) & 1) ^ 1, status);
+                {
+                    const uint32_t src = smem_u32(rawv) + rs * C::RV + sub * KV_PAGE + unit * 16, dst = sv + vs * C::V;
                     uint4 c[DV / 32];
 #pragma unroll
                     for (int k = 0; k < DV / 32; ++k) c[k] = ld_shared16(src + k * 32 * KV_PAGE);
                     // behind the sequence's end a page may hold anything, NaN codes too, and 0 x NaN would count
-                    const int live = len - (2 * t + x) * KV_PAGE - unit * 16;
+                    const int live = len - t * PR_STEP - unit * 16;
                     if (__any_sync(0xffffffffu, live < 16)) {
                         uint32_t keep[4];
 #pragma unroll
@@ -598,141 +633,105 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(&B.vfull[vs]);
-                    mbar_arrive(&B.rvempty);
+                    mbar_arrive(&B.rvempty[rs]);
                 }
             }
         }
     } else {
-        // ---- MMA issue: a whole warp walks through, so that descriptors stay in uniform registers, and one lane issues
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PR_REGS_MMA));
-        if (warp == PR_MMA) {
+        if (warp == PR_MMA || warp == PR_MMA + 3) {
+            // ---- MMA issue, a warp for each tile, so that the one's waits do not hold the other's products up. A whole warp walks
+            // through, so that descriptors stay in uniform registers, and one lane issues. Loops stay rolled: each product is
+            // issued once a step, and straight-line code would come from memory every time.
+            constexpr uint32_t iqk = umma_idesc_f16(PR_TILE, PR_STEP), ipv = umma_idesc_f16(PR_TILE, DV);
             const uint32_t lead = elect_one();
-        constexpr uint32_t iqk = umma_idesc_f16(PR_TILE, PR_TILE), ipv = umma_idesc_f16(PR_TILE, DV);
-        uint32_t it = 0, seg = 0;
-        // Rolled loops: this warp runs each product once a step, and straight-line code would come from memory every time.
-        auto qk = [&](int tile, uint32_t n) {
-            uint64_t a = umma_desc_sw128(sq + tile * C::KC * C::CHUNK), b = umma_desc_sw128(sk + (n % C::KST) * C::K);
+            const int tile = warp == PR_MMA ? 0 : 1;
+            const uint32_t ts = tmem + tile * PR_TILE, to = tmem + 2 * PR_TILE + tile * DV;
+            const uint64_t dq = umma_desc_sw128(sq + tile * C::KC * C::QCHUNK);
+            uint32_t it = 0;
+            for (uint32_t seg = 0;; ++seg) {
+                const PrSeg& g = segment(seg);
+                const int n = g.t1 - g.t0;
+                if (g.t1 == 0) break;
+                __syncwarp();
+                if (lead) mbar_arrive(&B.segempty[seg % PR_SEGS]);
+                wait_on(&B.qfull[tile], seg & 1, status);
+                // scores run two steps ahead of the weights' products
+                it -= 2;
 #pragma unroll 1
-            for (int j = 0; j < DK / 16; ++j) {
-                umma_f16_if(lead, tmem + tile * PR_TILE, a, b, iqk, j > 0);
-                const uint32_t up = (j & 3) == 3 ? (C::CHUNK - 96) >> 4 : 2;   // 32 bytes on, or the next chunk
-                a += up;
-                b += up;
-            }
-            umma_commit_if(lead, &B.sready[tile]);
-        };
-        auto pv = [&](int tile, uint32_t n, bool add) {
-            uint64_t b = umma_desc_sw128(sv + (n % C::VST) * C::V);
+                for (int j = -2; j < n; ++j, ++it) {
+                    if (j >= 0) {
+                        wait_on(&B.vfull[it % C::VST], (it / C::VST) & 1, status);
+                        wait_on(&B.pready[tile][it & 1], (it >> 1) & 1, status);
+                        tc_fence_after();
+                        uint64_t b = umma_desc_sw128(sv + (it % C::VST) * C::V);
+                        uint32_t a = ts + (it & 1) * PR_STEP;
 #pragma unroll 1
-            for (int k = 0; k < PR_TILE / 16; ++k) {
-                umma_f16_ta_if(lead, tmem + 2 * PR_TILE + tile * DV, tmem + tile * PR_TILE + k * 8, b, ipv, add || k > 0);
-                b += (k & 3) == 3 ? (C::VCHUNK - 96) >> 4 : 2;
-            }
-            umma_commit_if(lead, &B.pvdone[tile]);
-        };
-        for (;; ++seg) {
-            const PrSeg& g = segment(seg);
-            const int n = g.t1 - g.t0;
-            if (g.t1 == 0) break;
-            __syncwarp();
-            if (lead) mbar_arrive(&B.segempty[seg % PR_SEGS]);
-            for (int tile = 0; tile < 2; ++tile) {
-                mbar_wait(&B.qfull[tile], seg & 1, status);
-                if (tile == 0) mbar_wait(&B.kfull[it % C::KST], (it / C::KST) & 1, status);
-                tc_fence_after();
-                qk(tile, it);
-            }
-            umma_commit_if(lead, &B.kempty[it % C::KST]);
-            for (int j = 0; j < n; ++j, ++it) {
-                for (int tile = 0; tile < 2; ++tile) {
-                    if (tile == 0) mbar_wait(&B.vfull[it % C::VST], (it / C::VST) & 1, status);
-                    mbar_wait(&B.pready[tile], it & 1, status);
-                    tc_fence_after();
-                    pv(tile, it, j > 0);
-                    if (j + 1 < n) {
-                        if (tile == 0) {
-                            mbar_wait(&B.kfull[(it + 1) % C::KST], ((it + 1) / C::KST) & 1, status);
-                            tc_fence_after();
+                        for (int k = 0; k < PR_STEP / 16; ++k, a += 8, b += 2) umma_f16_ta_if(lead, to, a, b, ipv, j > 0 || k > 0);
+                        umma_commit_if(lead, &B.pvdone[tile][it & 1]);
+                        umma_commit_if(lead, &B.vempty[it % C::VST]);
+                    }
+                    if (j + 2 < n) {
+                        const uint32_t ahead = it + 2, ks = ahead % C::KST;
+                        wait_on(&B.kfull[ks], (ahead / C::KST) & 1, status);
+                        tc_fence_after();
+                        uint64_t a = dq, b = umma_desc_sw128(sk + ks * C::K);
+#pragma unroll 1
+                        for (int k = 0; k < DK / 16; ++k) {
+                            umma_f16_if(lead, ts + (it & 1) * PR_STEP, a, b, iqk, k > 0);
+                            a += (k & 3) == 3 ? (C::QCHUNK - 96) >> 4 : 2;   // 32 bytes on, or the next chunk
+                            b += (k & 3) == 3 ? (C::KCHUNK - 96) >> 4 : 2;
                         }
-                        qk(tile, it + 1);
+                        umma_commit_if(lead, &B.sready[tile][it & 1]);
+                        umma_commit_if(lead, &B.kempty[ks]);
                     }
                 }
-                umma_commit_if(lead, &B.vempty[it % C::VST]);
-                if (j + 1 < n) umma_commit_if(lead, &B.kempty[(it + 1) % C::KST]);
             }
-        }
         } else if (warp == PR_MMA + 2) {
-            // ---- copies: a step's pages into shared memory as they are, and its blocks' scales
+            // ---- copies: a step's page into shared memory as it is, and its blocks' scales
             int pages = -1, pages_at = -64, pages_b = -1;   // lane l: page pages_at + l of sequence pages_b
             uint32_t it = 0;
-            float4 mine = make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
             for (uint32_t seg = 0;; ++seg) {
                 const PrSeg& g = segment(seg);
                 const int b = g.b, h = g.h, t0 = g.t0, t1 = g.t1, len = g.s.len;
                 if (t1 == 0) break;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&B.segempty[seg % PR_SEGS]);
+#pragma unroll 1
                 for (int t = t0; t < t1; ++t, ++it) {
-                    int pg[2];
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const int i = 2 * t + x;
-                        if (b != pages_b || i < pages_at || i >= pages_at + 32) {
-                            pages_b = b;
-                            pages_at = i;
-                            const int want = i + lane;
-                            pages = static_cast<int64_t>(want) * KV_PAGE < len ? kv_page(p.c, p.b, b, want, status) : -1;
-                        }
-                        pg[x] = __shfl_sync(0xffffffffu, pages, i - pages_at);
+                    const uint32_t rs = it % C::RST, par = ((it / C::RST) & 1) ^ 1;
+                    if (b != pages_b || t < pages_at || t >= pages_at + 32) {
+                        pages_b = b;
+                        pages_at = t;
+                        const int want = t + lane;
+                        pages = static_cast<int64_t>(want) * KV_PAGE < len ? kv_page(p.c, p.b, b, want, status) : -1;
                     }
-                    // a page that is not there: codes of zero and no weight
-                    if (lane < 8) {
-                        const int page = pg[lane >> 2];
-                        mine = make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
-                        if (page >= 0) {
-                            const int64_t i = (static_cast<int64_t>(page) * p.c.kv_heads + h) * KV_PAGE_BLOCKS + (lane & 3);
-                            const uint32_t ks = static_cast<const uint8_t*>(p.c.k_scale)[i];
-                            const uint32_t vs = min(max(static_cast<uint32_t>(static_cast<const uint8_t*>(p.c.v_scale)[i]), 1u), 253u);
-                            mine = make_float4(kv_scale(ks), static_cast<float>(static_cast<int>(vs) - 127),
-                                               __uint_as_float((254u - vs) << 23), 0.0f);
-                        }
+                    const int page = __shfl_sync(0xffffffffu, pages, t - pages_at);
+                    const int64_t ph = static_cast<int64_t>(max(page, 0)) * p.c.kv_heads + h;
+                    float4 mine = make_float4(1.0f, -INFINITY, 0.0f, 0.0f);   // no page: codes of zero and no weight
+                    if (lane < 4 && page >= 0) {
+                        const uint32_t ks = static_cast<const uint8_t*>(p.c.k_scale)[ph * KV_PAGE_BLOCKS + lane];
+                        const uint32_t vs = static_cast<const uint8_t*>(p.c.v_scale)[ph * KV_PAGE_BLOCKS + lane];
+                        const uint32_t ve = min(max(vs, 1u), 253u);
+                        mine = make_float4(kv_scale(ks), static_cast<float>(static_cast<int>(ve) - 127),
+                                           __uint_as_float((254u - ve) << 23), 0.0f);
                     }
-                    mbar_wait(&B.rkempty, (it & 1) ^ 1, status);
-                    if (pg[0] < 0 || pg[1] < 0) {
-                        for (int x = 0; x < 2; ++x)
-                            if (pg[x] < 0)
-                                for (int i = lane; i < KV_PAGE * DK / 16; i += 32)
-                                    st_shared16(smem_u32(rawk) + x * KV_PAGE * DK + i * 16, make_uint4(0, 0, 0, 0));
+                    wait_on(&B.rkempty[rs], par, status);
+                    if (page < 0) {
+                        for (int i = lane; i < C::RK / 16; i += 32) st_shared16(smem_u32(rawk) + rs * C::RK + i * 16, make_uint4(0, 0, 0, 0));
                         __syncwarp();
                     }
                     if (lane == 0) {
-                        mbar_arrive_expect_tx(&B.rkfull, ((pg[0] >= 0) + (pg[1] >= 0)) * KV_PAGE * DK);
-#pragma unroll
-                        for (int x = 0; x < 2; ++x)
-                            if (pg[x] >= 0)
-                                bulk_g2s(rawk + x * KV_PAGE * DK,
-                                         static_cast<const uint8_t*>(p.c.k) + (static_cast<int64_t>(pg[x]) * p.c.kv_heads + h) * KV_PAGE * DK,
-                                         KV_PAGE * DK, &B.rkfull);
+                        mbar_arrive_expect_tx(&B.rkfull[rs], page >= 0 ? C::RK : 0);
+                        if (page >= 0) bulk_g2s(rawk + rs * C::RK, static_cast<const uint8_t*>(p.c.k) + ph * C::RK, C::RK, &B.rkfull[rs]);
                     }
-                    __syncwarp();
-                    mbar_wait(&B.rvempty, (it & 1) ^ 1, status);
-                    if (pg[0] < 0 || pg[1] < 0) {
-                        for (int x = 0; x < 2; ++x)
-                            if (pg[x] < 0)
-                                for (int i = lane; i < KV_PAGE * DV / 16; i += 32)
-                                    st_shared16(smem_u32(rawv) + x * KV_PAGE * DV + i * 16, make_uint4(0, 0, 0, 0));
-                        __syncwarp();
-                    }
-                    if (lane < 8) scales[it % PR_SCALES][lane] = mine;
+                    wait_on(&B.rvempty[rs], par, status);
+                    if (page < 0)
+                        for (int i = lane; i < C::RV / 16; i += 32) st_shared16(smem_u32(rawv) + rs * C::RV + i * 16, make_uint4(0, 0, 0, 0));
+                    if (lane < 4) scales[it % PR_SCALES][lane] = mine;
                     __syncwarp();
                     if (lane == 0) {
-                        mbar_arrive_expect_tx(&B.rvfull, ((pg[0] >= 0) + (pg[1] >= 0)) * KV_PAGE * DV);
-#pragma unroll
-                        for (int x = 0; x < 2; ++x)
-                            if (pg[x] >= 0)
-                                bulk_g2s(rawv + x * KV_PAGE * DV,
-                                         static_cast<const uint8_t*>(p.c.v) + (static_cast<int64_t>(pg[x]) * p.c.kv_heads + h) * KV_PAGE * DV,
-                                         KV_PAGE * DV, &B.rvfull);
+                        mbar_arrive_expect_tx(&B.rvfull[rs], page >= 0 ? C::RV : 0);
+                        if (page >= 0) bulk_g2s(rawv + rs * C::RV, static_cast<const uint8_t*>(p.c.v) + ph * C::RV, C::RV, &B.rvfull[rs]);
                         mbar_arrive(&B.scfull[it % PR_SCALES]);
                     }
                     __syncwarp();
@@ -743,7 +742,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
             int b = place.b, h = place.h, qb = place.qb, off = place.off, left = place.left, done = 0;
             KvSeq s = left > 0 ? kv_seq(p.b, b, status) : KvSeq{0, 0, 0, 0};
             for (uint32_t i = 0;; ++i) {
-                mbar_wait(&B.segempty[i % PR_SEGS], ((i / PR_SEGS) & 1) ^ 1, status);
+                wait_on(&B.segempty[i % PR_SEGS], ((i / PR_SEGS) & 1) ^ 1, status);
                 PrSeg& g = segs[i % PR_SEGS];
                 PrItem item{};
                 int have = 0;
