@@ -63,7 +63,7 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi)
 __device__ __forceinline__ float ex2(float x)
 {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 

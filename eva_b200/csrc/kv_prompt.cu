@@ -9,8 +9,8 @@
 // keys are rows of key_dim, its values rows of 64 tokens, so both are K-major operands without a transposition. Converting for
 // two tiles at once halves that work. The scales stay outside, as in the decode kernel: a block's key scale multiplies its
 // scores, its value scale 2^e goes into the exponent t = score + e, and out = sum 2^(t - M) code / sum 2^(t - M) 2^-e.
-// M is raised (and O rescaled in tensor memory) only when a row's maximum has grown by more than 2^8: weights are fp16 up to
-// 2^15, 2^7 at M, so that tokens down to 2^-21 of the largest keep 11 bits, and 2^-31 is the smallest.
+// M is raised (and O rescaled in tensor memory) only when a row's maximum has grown by more than 2^12: weights are fp16 up to 2^15,
+// 2^3 at M, so that tokens down to 2^-17 of it keep 11 bits, and 2^-27 is the step below.
 //
 // The (sequence, head, row block, token tile) units of a call form one line that is cut into equal pieces, one per SM, so
 // causal rows of different lengths and ragged batches fill the GPU alike; row blocks cut between pieces leave fp32 partial
@@ -27,10 +27,10 @@ namespace eva {
 
 constexpr int PR_TILE = 128, PR_ROWS = 2 * PR_TILE;       // rows of a tile, of a CTA
 constexpr int PR_STEP = KV_PAGE;                          // tokens of a step
-// Four warpgroups: 8 softmax warps, 4 converter warps, two that issue the MMAs, one each for
-// the segments and the copies.
-constexpr int PR_CONV = 4, PR_MMA = 8 + PR_CONV, PR_WARPS = 16;
-constexpr float PR_BIAS = 7.0f, PR_SLACK = 8.0f;
+// 16 softmax warps (for each tile four for the even and four for the odd steps), 4 converter warps, two that issue the
+// MMAs, one each for the segments and the copies.
+constexpr int PR_SOFT = 16, PR_CONV = 4, PR_MMA = PR_SOFT + PR_CONV, PR_WARPS = PR_MMA + 4;
+constexpr float PR_BIAS = 3.0f, PR_SLACK = 12.0f;         // exponents of a weight at M, and by which it may pass M
 constexpr int PR_SCALES = 8, PR_SEGS = 4;                 // steps whose scales are kept, segments in flight
 
 template <int DK, int DV> struct PrCfg {
@@ -38,24 +38,46 @@ template <int DK, int DV> struct PrCfg {
     static constexpr int QCHUNK = PR_TILE * 128, KCHUNK = PR_STEP * 128;   // rows x 128 bytes
     static constexpr int Q = 2 * KC * QCHUNK, K = KC * KCHUNK, V = DV * 128;
     static constexpr int RK = PR_STEP * DK, RV = PR_STEP * DV;   // a step's codes as they are in the cache
-    static constexpr int KST = 3, VST = DK == 192 ? 2 : 3, RST = DK == 192 ? 1 : 2;   // stages
+    static constexpr int KST = DK == 192 ? 2 : 3, VST = KST, RST = 2;   // stages
     static constexpr int SMEM = Q + KST * K + VST * V + RST * (RK + RV) + 1024;
-    static_assert(SMEM <= 227 * 1024 - 2048, "shared memory");
+    static_assert(SMEM <= 227 * 1024 - 7168, "shared memory");
 };
 
 struct PrBars {
     uint64_t kfull[3], kempty[3], vfull[3], vempty[3], rkfull[2], rkempty[2], rvfull[2], rvempty[2];
     uint64_t sready[2][2], pready[2][2], pvdone[2][2], qfull[2];   // [tile][step & 1]
+    uint64_t mready[2][4][2];                                   // [tile][warp][step & 1]
     uint64_t scfull[PR_SCALES], segfull[PR_SEGS], segempty[PR_SEGS];
     uint32_t tmem;
 };
 
-// mbar_wait with the waiting itself out of line: code that a warp runs once a step has to stay short.
-__device__ __noinline__ void wait_long(uint64_t* bar, uint32_t parity, int* status) { mbar_wait(bar, parity, status); }
+// mbar_wait that sleeps in the barrier unit for up to 100 us a try: many warps wait here at any time, and short tries would
+// fill the queue to shared memory, exponentials and tensor memory that the others work through. The loop for a wait
+// that is not over by then stays out of line.
+__device__ __forceinline__ bool try_wait_long(uint64_t* bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(100000)
+        : "memory");
+    return ok != 0;
+}
+
+__device__ __noinline__ void wait_more(uint64_t* bar, uint32_t parity, int* status)
+{
+    const uint64_t t0 = globaltimer();
+    while (!try_wait_long(bar, parity))
+        if (globaltimer() - t0 > WAIT_LIMIT_NS || (ld_volatile(status) & ST_TIMEOUT)) {
+            atomicOr(status, ST_TIMEOUT);
+            return;
+        }
+}
 
 __device__ __forceinline__ void wait_on(uint64_t* bar, uint32_t parity, int* status)
 {
-    if (!mbar_try_wait(bar, parity)) wait_long(bar, parity, status);
+    if (!try_wait_long(bar, parity)) wait_more(bar, parity, status);
 }
 
 // Row block qb of a sequence: its rows' tokens, the token range they see and the steps over it.
@@ -102,7 +124,7 @@ struct PrSeg {
     KvSeq s;
 };
 
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16])
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r)
 {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
@@ -188,9 +210,15 @@ __device__ __forceinline__ void add2(float& x, float& y, float a, float b)
 }
 
 // Largest t = score * scale + exponent of a step's scores
-__device__ __forceinline__ float pr_max(const uint32_t (&r)[64], const float4* sc, float c)
+__device__ __forceinline__ float pr_max(uint32_t ts, const float4* sc, float c)
 {
     float mx = -INFINITY;
+    uint32_t r[64];
+    tmem_ld32_async(ts, r);
+    tmem_ld32_async(ts + 32, r + 32);
+    tmem_wait_ld();
+    tied(r);
+    tied(r + 32);
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
         float b = -INFINITY;
@@ -202,28 +230,36 @@ __device__ __forceinline__ float pr_max(const uint32_t (&r)[64], const float4* s
 }
 
 // Weights 2^(t + ref) as fp16 into tensor memory (over the scores); returns their sum, each divided by its value scale.
-__device__ __forceinline__ float pr_weights(const uint32_t (&r)[64], const float4* sc, float c, float ref, uint32_t ts)
+__device__ __forceinline__ float pr_weights(uint32_t ts, const float4* sc, float c, float ref)
 {
     float l = 0.0f;
-#pragma unroll
+#pragma unroll 1
     for (int k = 0; k < 2; ++k) {
-        uint32_t w[16];
+        uint32_t r[32], w[16];
+        tmem_ld32_async(ts + 32 * k, r);
+        tmem_wait_ld();
+        tied(r);
+        // A pair's exponentials are issued four pairs before their sum and rounding, which would wait for them.
+        constexpr int AHEAD = 4;
+        float4 f[2] = {sc[2 * k], sc[2 * k + 1]};
+        float sum[2][2] = {};
 #pragma unroll
-        for (int x = 2 * k; x < 2 * k + 2; ++x) {
-            const float4 f = sc[x];
-            const float fc = f.x * c, add = f.y + ref;
-            float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll
-            for (int i = 16 * x; i < 16 * x + 16; i += 2) {
+        for (int i = 0; i < 16 + AHEAD; ++i) {
+            if (i < 16) {
                 float a, b;
-                fma2(a, b, __uint_as_float(r[i]), __uint_as_float(r[i + 1]), fc, add);
-                a = ex2(a);
-                b = ex2(b);
-                add2(s0, s1, a, b);
-                w[i / 2 - 16 * k] = half2_bits(a, b);
+                fma2(a, b, __uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), f[i / 8].x * c, f[i / 8].y + ref);
+                r[2 * i] = __float_as_uint(ex2(a));
+                r[2 * i + 1] = __float_as_uint(ex2(b));
             }
-            l = fmaf(s0 + s1, f.z, l);
+            if (i >= AHEAD) {
+                const int j = i - AHEAD;
+                const float a = __uint_as_float(r[2 * j]), b = __uint_as_float(r[2 * j + 1]);
+                add2(sum[j / 8][0], sum[j / 8][1], a, b);
+                w[j] = half2_bits(a, b);
+            }
         }
+        l = fmaf(sum[0][0] + sum[0][1], f[0].z, l);
+        l = fmaf(sum[1][0] + sum[1][1], f[1].z, l);
         tmem_st16(ts + 16 * k, w);
     }
     return l;
@@ -270,6 +306,22 @@ __device__ __noinline__ float pr_weights_masked(uint32_t ts, const float4* sc, f
     return l;
 }
 
+// A row's output so far, times fall
+template <int DV> __device__ __noinline__ void pr_rescale(uint32_t to, float fall)
+{
+#pragma unroll 1
+    for (int k = 0; k < DV; k += 32) {
+        uint32_t o[32];
+        tmem_ld32_async(to + k, o);
+        tmem_wait_ld();
+        tied(o);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fall);
+        tmem_st16(to + k, o);
+        tmem_st16(to + k + 16, o + 16);
+    }
+}
+
 // 16 codes (16 bytes) as two 16-byte units of halves
 __device__ __forceinline__ void codes_to_halves(uint4 c, uint4& lo, uint4& hi)
 {
@@ -282,6 +334,12 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t addr)
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
     return v;
+}
+
+// 16 bytes from global to shared memory, or zeros
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 
 __device__ __forceinline__ void st_shared16(uint32_t addr, uint4 v)
@@ -301,6 +359,9 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
     __shared__ float4 scales[PR_SCALES][4];               // of a step's blocks: key scale, value exponent, 1 / value scale
     __shared__ PrPlace place;
     __shared__ PrSeg segs[PR_SEGS];
+    __shared__ float qscale[2][PR_TILE];                  // of a row's query: its power of two times the call's scale
+    __shared__ float top[2][PR_TILE];                     // the running M of a tile's rows
+    __shared__ float2 sums[2][2][PR_TILE];                // [tile][step & 1]: M and sum of a row as its steps left them
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform for the compiler
     uint8_t* smem = align1024(smem_raw);
     const uint32_t sq = smem_u32(smem), sk = sq + C::Q, sv = sk + C::KST * C::K;
@@ -325,13 +386,14 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
                 mbar_init(&B.sready[i][j], 1);
                 mbar_init(&B.pready[i][j], 4);
                 mbar_init(&B.pvdone[i][j], 1);
+                for (int k = 0; k < 4; ++k) mbar_init(&B.mready[i][k][j], 1);
             }
-            mbar_init(&B.qfull[i], 4);
+            mbar_init(&B.qfull[i], 8);
         }
         for (int i = 0; i < PR_SCALES; ++i) mbar_init(&B.scfull[i], 1);
         for (int i = 0; i < PR_SEGS; ++i) {
             mbar_init(&B.segfull[i], 1);
-            mbar_init(&B.segempty[i], 8 + PR_CONV + 3);
+            mbar_init(&B.segempty[i], PR_SOFT + PR_CONV + 3);
         }
         fence_barrier_init();
     }
@@ -407,19 +469,21 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
         return segs[i % PR_SEGS];
     };
 
-    if (warp < 8) {
-        // ---- softmax: thread = row of tile `tile`
-        const int tile = warp >> 2, row = (warp & 3) * 32 + lane;
-        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t tsc = tmem + lanes + tile * PR_TILE, to = tmem + lanes + 2 * PR_TILE + tile * DV;
+    if (warp < PR_SOFT) {
+        // ---- softmax: thread = row of tile `tile`, in the steps of one parity. A step's maximum joins the other parity's M of the
+        // step before; all else of consecutive steps overlaps.
+        const int tile = warp >> 3, odd_steps = (warp >> 2) & 1, quad = warp & 3, row = quad * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+        const uint32_t ts = tmem + lanes + tile * PR_TILE + odd_steps * PR_STEP, to = tmem + lanes + 2 * PR_TILE + tile * DV;
         uint32_t it = 0;                      // steps so far
         if (threadIdx.x == 0) p.heads_of[blockIdx.x] = make_int4(-1, 0, 0, 0);
         for (uint32_t seg = 0;; ++seg) {
             const PrSeg& g = segment(seg);
             const int t0 = g.t0, t1 = g.t1;
             if (t1 == 0) break;
-            const int r = g.qb * PR_ROWS + tile * PR_TILE + row, tok = r / p.group, qh = g.h * p.group + (r - tok * p.group);
-            const bool in = tok < g.s.n, whole = g.first && g.after == 0;
+            const int qb = g.qb, h = g.h, rows = g.s.n, row0 = g.s.row0;
+            const int r = qb * PR_ROWS + tile * PR_TILE + row, tok = r / p.group, qh = h * p.group + (r - tok * p.group);
+            const bool in = tok < rows, whole = g.first && g.after == 0;
             const int64_t qrow = static_cast<int64_t>(g.s.row0) + tok;
             // rows without a token see nothing; rows behind the sequence are not written and need no mask
             const int hi = in ? g.s.ctx + tok + 1 : 0x7fffffff, lo = in && p.window > 0 ? max(hi - p.window, 0) : 0;
@@ -432,20 +496,31 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
                               static_cast<int>(((place.begin + g.done + (t1 - t0) + g.after) * place.pieces - 1) / place.total));
             __syncwarp();
             if (lane == 0) mbar_arrive(&B.segempty[seg % PR_SEGS]);
-            // the row, scaled by a power of two to [1, 2) at its largest, as fp16
-            float c;
+            // The 32 rows (16 by each parity's warp), each scaled by a power of two to [1, 2) at its largest, as fp16: eight lanes a row, so that copies and
+            // stores take whole 128-byte lines, four rows at a time; first as they are to their places, then scaled there.
             {
-                const T* q = static_cast<const T*>(p.q) + qrow * p.qt + static_cast<int64_t>(qh) * p.qh;
-                float big = 0.0f;
-                bool odd = false;
+                const int l8 = lane & 7, sub4 = quad * 32 + (lane >> 3);
+                const uint32_t dst = sq + tile * C::KC * C::QCHUNK;
 #pragma unroll 1
-                for (int u = 0; u < DK / 8; u += 8) {
-                    uint4 raw[8];
+                for (int x = 16 * odd_steps; x < 16 * odd_steps + 16; x += 4) {
+                    const int r4 = qb * PR_ROWS + tile * PR_TILE + sub4 + x, tok4 = r4 / p.group;
+                    const T* q = static_cast<const T*>(p.q) + (static_cast<int64_t>(row0) + tok4) * p.qt +
+                                 (static_cast<int64_t>(h) * p.group + (r4 - tok4 * p.group)) * p.qh + l8 * 8;
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) raw[k] = in ? *reinterpret_cast<const uint4*>(q + (u + k) * 8) : make_uint4(0, 0, 0, 0);
+                    for (int j = 0; j < C::KC; ++j) copy16(dst + j * C::QCHUNK + sw128(sub4 + x, l8), tok4 < rows ? q + j * 64 : p.q, tok4 < rows);
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                __syncwarp();
+#pragma unroll 1
+                for (int x = 16 * odd_steps; x < 16 * odd_steps + 16; x += 4) {
+                    uint4 raw[C::KC];
+                    float big = 0.0f;
+                    bool odd = false;
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+                    for (int j = 0; j < C::KC; ++j) raw[j] = ld_shared16(dst + j * C::QCHUNK + sw128(sub4 + x, l8));
+#pragma unroll
+                    for (int j = 0; j < C::KC; ++j) {
+                        const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const float2 f = two_floats<T>(w[e]);
@@ -453,88 +528,88 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
                             odd |= f.x != f.x || f.y != f.y;
                         }
                     }
-                }
-                odd |= big == INFINITY;
-                const int e2 = min(max(static_cast<int>(__float_as_uint(big) >> 23), 1), 252);
-                const float down = __uint_as_float(static_cast<uint32_t>(254 - e2) << 23);
-                c = odd ? __uint_as_float(0x7fc00000u) : p.scale * __uint_as_float(static_cast<uint32_t>(e2) << 23);
-#pragma unroll 2
-                for (int u = 0; u < DK / 8; ++u) {
-                    const uint4 raw = in ? *reinterpret_cast<const uint4*>(q + u * 8) : make_uint4(0, 0, 0, 0);
-                    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-                    uint32_t o[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 f = two_floats<T>(w[e]);
-                        o[e] = half2_bits(f.x * down, f.y * down);
+                    for (int o = 1; o < 8; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                    odd = (__ballot_sync(0xffffffffu, odd) >> (lane & 24) & 0xffu) != 0 || big == INFINITY;
+                    const int e2 = min(max(static_cast<int>(__float_as_uint(big) >> 23), 1), 252);
+                    const float down = __uint_as_float(static_cast<uint32_t>(254 - e2) << 23);
+                    if (l8 == 0)
+                        qscale[tile][sub4 + x] = odd ? __uint_as_float(0x7fc00000u) : p.scale * __uint_as_float(static_cast<uint32_t>(e2) << 23);
+#pragma unroll
+                    for (int j = 0; j < C::KC; ++j) {
+                        const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+                        uint32_t o[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 f = two_floats<T>(w[e]);
+                            o[e] = half2_bits(f.x * down, f.y * down);
+                        }
+                        st_shared16(dst + j * C::QCHUNK + sw128(sub4 + x, l8), make_uint4(o[0], o[1], o[2], o[3]));
                     }
-                    st_shared16(sq + (tile * C::KC + u / 8) * C::QCHUNK + sw128(row, u % 8), make_uint4(o[0], o[1], o[2], o[3]));
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&B.qfull[tile]);
             }
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + tile * 4 + quad) : "memory");
+            const float c = qscale[tile][row];
             const int all_hi = __reduce_min_sync(0xffffffffu, hi), all_lo = __reduce_max_sync(0xffffffffu, lo);
+            const uint32_t first = it, end = it + (t1 - t0);
             float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
-            for (int t = t0; t < t1; ++t, ++it) {
+            for (it += (it ^ odd_steps) & 1; it < end; it += 2) {
                 const float4* sc = scales[it % PR_SCALES];
-                const uint32_t ts = tsc + (it & 1) * PR_STEP;
-                const int tok0 = t * PR_STEP;
+                const int tok0 = (t0 + static_cast<int>(it - first)) * PR_STEP;
                 const bool part_seen = tok0 + PR_STEP > all_hi || tok0 < all_lo;
                 wait_on(&B.scfull[it % PR_SCALES], (it / PR_SCALES) & 1, status);
-                wait_on(&B.sready[tile][it & 1], (it >> 1) & 1, status);
+                wait_on(&B.sready[tile][odd_steps], (it >> 1) & 1, status);
                 tc_fence_after();
-                uint32_t v[64];
-                float mx;
-                if (!part_seen) {
-                    tmem_ld32_async(ts, v);
-                    tmem_ld32_async(ts + 32, v + 32);
-                    tmem_wait_ld();
-                    tied(v);
-                    tied(v + 32);
-                    mx = pr_max(v, sc, c);
-                } else {
-                    mx = pr_max_masked(ts, sc, c, lo - tok0, hi - tok0);
+                const float mx = part_seen ? pr_max_masked(ts, sc, c, lo - tok0, hi - tok0) : pr_max(ts, sc, c);
+                float was = -INFINITY;
+                if (it > first) {
+                    wait_on(&B.mready[tile][quad][odd_steps ^ 1], ((it - 1) >> 1) & 1, status);
+                    was = top[tile][row];
                 }
-                const bool grow = mx > m + PR_SLACK || (m == -INFINITY && mx > m);
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float fall = grow ? ex2(m - mx) : 1.0f;
-                    if (grow) m = mx;
-                    l *= fall;
-                    if (t > t0) {
-                        wait_on(&B.pvdone[tile][(it - 1) & 1], ((it - 1) >> 1) & 1, status);
-                        tc_fence_after();
-#pragma unroll 1
-                        for (int k = 0; k < DV; k += 16) {
-                            uint32_t o[16];
-                            tmem_ld32x32_x16(to + k, o);
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fall);
-                            tmem_st16(to + k, o);
-                        }
-                    }
+                const bool grow = mx > was + PR_SLACK || (was == -INFINITY && mx > was);
+                const float now = grow ? mx : was;
+                top[tile][row] = now;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&B.mready[tile][quad][odd_steps]);
+                if (it > first && __any_sync(0xffffffffu, grow)) {
+                    const float fall = grow ? ex2(was - now) : 1.0f;
+                    wait_on(&B.pvdone[tile][odd_steps ^ 1], ((it - 1) >> 1) & 1, status);
+                    tc_fence_after();
+                    pr_rescale<DV>(to, fall);
                 }
+                if (m != now) l *= m == -INFINITY ? 1.0f : ex2(m - now);   // (a sum that is not 0 there is NaN, and stays it)
+                m = now;
                 const float ref = PR_BIAS - (m == -INFINITY ? 0.0f : m);
                 if (!part_seen && !__any_sync(0xffffffffu, m != -INFINITY && fabsf(m) > 4096.0f))
-                    l += pr_weights(v, sc, c, ref, ts);
+                    l += pr_weights(ts, sc, c, ref);
                 else
                     l += pr_weights_masked(ts, sc, c, ref, lo - tok0, hi - tok0);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&B.pready[tile][it & 1]);
+                if (lane == 0) mbar_arrive(&B.pready[tile][odd_steps]);
             }
+            it = end;
+            // both parities' sums, then half of the output each
+            sums[tile][odd_steps][row] = make_float2(m, l);
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + tile * 4 + quad) : "memory");
+            const float2 s0 = sums[tile][0][row], s1 = sums[tile][1][row];
+            m = fmaxf(s0.x, s1.x);
+            l = s0.y * (s0.x == -INFINITY ? 1.0f : ex2(s0.x - m)) + s1.y * (s1.x == -INFINITY ? 1.0f : ex2(s1.x - m));
             wait_on(&B.pvdone[tile][(it - 1) & 1], ((it - 1) >> 1) & 1, status);
             tc_fence_after();
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const int pr = tile * PR_TILE + row;
-            if (!whole && in) {
+            if (!whole && in && odd_steps == 0) {
                 part[pr] = m;
                 part[PR_ROWS + pr] = l;
             }
 #pragma unroll 1
-            for (int k = 0; k < DV; k += 16) {
+            for (int k = odd_steps * (DV / 2); k < (odd_steps + 1) * (DV / 2); k += 16) {
                 uint32_t v[16];
                 __syncwarp();
                 tmem_ld32x32_x16(to + k, v);
@@ -555,9 +630,9 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
             }
             tc_fence_before();
         }
-    } else if (warp < 8 + PR_CONV) {
+    } else if (warp < PR_MMA) {
         // ---- converters: 64-byte quarters of 8 rows per warp and load
-        const int unit = lane & 3, sub = (warp - 8) * 8 + (lane >> 2);
+        const int unit = lane & 3, sub = (warp - PR_SOFT) * 8 + (lane >> 2);
         // Eight lanes read and write 128 bytes without a bank conflict where two rows of a quarter are 64 or 192 bytes apart;
         // rows of 128 bytes take the one half from the even and the other from the odd row.
         const int odd = DK == 128 ? sub & 1 : 0;
