@@ -257,9 +257,11 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
                         const uint4 w4 = *reinterpret_cast<const uint4*>(kr + j * 64);
                         const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            mma_f16(sc[ih], qf[j * 4 + e][0], qf[j * 4 + e][1], qf[j * 4 + e][2], qf[j * 4 + e][3],
-                                    e4m3_halves(w[e]), e4m3_halves(w[e] >> 16));
+                        for (int e = 0; e < 4; ++e) {
+                            uint32_t k0, k1;
+                            e4m3_halves(w[e], k0, k1);
+                            mma_f16(sc[ih], qf[j * 4 + e][0], qf[j * 4 + e][1], qf[j * 4 + e][2], qf[j * 4 + e][3], k0, k1);
+                        }
                     }
                 }
                 const float ks = kv_scale(cur.ks), vlog = static_cast<float>(static_cast<int>(max(cur.vs, 1u)) - 127);
@@ -325,7 +327,9 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         if (tail) w[e] &= keep[e];
-                        mma_f16(o[j], pf[e][0], pf[e][1], pf[e][2], pf[e][3], e4m3_halves(w[e]), e4m3_halves(w[e] >> 16));
+                        uint32_t v0, v1;
+                        e4m3_halves(w[e], v0, v1);
+                        mma_f16(o[j], pf[e][0], pf[e][1], pf[e][2], pf[e][3], v0, v1);
                     }
                 }
                 __syncwarp();   // every lane has read the stage

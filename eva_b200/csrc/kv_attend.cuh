@@ -46,12 +46,12 @@ template <typename T> __device__ __forceinline__ T one_of(float v);
 template <> __device__ __forceinline__ __nv_bfloat16 one_of(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half one_of(float v) { return __float2half_rn(v); }
 
-// two e4m3 codes (the low 16 bits) as two halves, exact
-__device__ __forceinline__ uint32_t e4m3_halves(uint32_t two)
+// four e4m3 codes as four halves, exact
+__device__ __forceinline__ void e4m3_halves(uint32_t four, uint32_t& lo, uint32_t& hi)
 {
-    uint32_t r;
-    asm("{\n .reg .b16 lo;\n cvt.u16.u32 lo, %1;\n cvt.rn.f16x2.e4m3x2 %0, lo;\n}\n" : "=r"(r) : "r"(two));
-    return r;
+    asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}\n"
+        : "=r"(lo), "=r"(hi)
+        : "r"(four));
 }
 
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi)

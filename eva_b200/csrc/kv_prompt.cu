@@ -31,6 +31,7 @@ constexpr int PR_STEP = KV_PAGE;                          // tokens of a step
 // MMAs, one each for the segments and the copies.
 constexpr int PR_SOFT = 16, PR_CONV = 4, PR_MMA = PR_SOFT + PR_CONV, PR_WARPS = PR_MMA + 4;
 constexpr float PR_BIAS = 3.0f, PR_SLACK = 12.0f;         // exponents of a weight at M, and by which it may pass M
+constexpr int PR_BLOCK_COST = 6;                          // steps that a row block's beginning and end take
 constexpr int PR_SCALES = 8, PR_SEGS = 4;                 // steps whose scales are kept, segments in flight
 
 template <int DK, int DV> struct PrCfg {
@@ -98,11 +99,12 @@ __device__ __forceinline__ PrItem pr_item(const KvSeq& s, int group, int window,
 
 __device__ __forceinline__ int pr_blocks(const KvSeq& s, int group) { return (s.n * group + PR_ROWS - 1) / PR_ROWS; }
 
-// Steps of one head of a sequence (whole warp).
+// Cost of one head of a sequence in steps (whole warp): a row block counts its steps and, before them, PR_BLOCK_COST for the time
+// its query, first scores and output take (15k clocks, against 2.5k of a step).
 __device__ __forceinline__ int64_t pr_units(const KvSeq& s, int group, int window)
 {
     int64_t sum = 0;
-    for (int qb = threadIdx.x & 31; qb < pr_blocks(s, group); qb += 32) sum += pr_item(s, group, window, qb).tiles;
+    for (int qb = threadIdx.x & 31; qb < pr_blocks(s, group); qb += 32) sum += pr_item(s, group, window, qb).tiles + PR_BLOCK_COST;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sum;
@@ -120,7 +122,7 @@ struct PrPlace {
 // Consecutive steps of one row block within a piece; t1 == 0 ends the piece.
 struct PrSeg {
     int b, h, qb, t0, t1;          // steps t0 .. t1 - 1
-    int first, after, done;        // holds the row block's first step; steps of it in later pieces; of the piece before
+    int first, after, end;         // holds the row block's first step; steps of it in later pieces; cost from the piece's begin to its end
     KvSeq s;
 };
 
@@ -209,6 +211,13 @@ __device__ __forceinline__ void add2(float& x, float& y, float a, float b)
         : "f"(a), "f"(b));
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // Largest t = score * scale + exponent of a step's scores
 __device__ __forceinline__ float pr_max(uint32_t ts, const float4* sc, float c)
 {
@@ -223,7 +232,7 @@ __device__ __forceinline__ float pr_max(uint32_t ts, const float4* sc, float c)
     for (int x = 0; x < 4; ++x) {
         float b = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) b = fmaxf(b, __uint_as_float(r[16 * x + i]));
+        for (int i = 0; i < 16; i += 2) b = max3(b, __uint_as_float(r[16 * x + i]), __uint_as_float(r[16 * x + i + 1]));
         mx = fmaxf(mx, fmaf(b, sc[x].x * c, sc[x].y));
     }
     return mx;
@@ -325,8 +334,10 @@ template <int DV> __device__ __noinline__ void pr_rescale(uint32_t to, float fal
 // 16 codes (16 bytes) as two 16-byte units of halves
 __device__ __forceinline__ void codes_to_halves(uint4 c, uint4& lo, uint4& hi)
 {
-    lo = make_uint4(e4m3_halves(c.x), e4m3_halves(c.x >> 16), e4m3_halves(c.y), e4m3_halves(c.y >> 16));
-    hi = make_uint4(e4m3_halves(c.z), e4m3_halves(c.z >> 16), e4m3_halves(c.w), e4m3_halves(c.w >> 16));
+    e4m3_halves(c.x, lo.x, lo.y);
+    e4m3_halves(c.y, lo.z, lo.w);
+    e4m3_halves(c.z, hi.x, hi.y);
+    e4m3_halves(c.w, hi.z, hi.w);
 }
 
 __device__ __forceinline__ uint4 ld_shared16(uint32_t addr)
@@ -436,7 +447,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
                 w.h = static_cast<int>(rem / u);
                 rem -= w.h * u;
                 for (int q0 = 0; q0 < pr_blocks(s, p.group); q0 += 32) {
-                    int t = q0 + lane < pr_blocks(s, p.group) ? pr_item(s, p.group, p.window, q0 + lane).tiles : 0;
+                    int t = q0 + lane < pr_blocks(s, p.group) ? pr_item(s, p.group, p.window, q0 + lane).tiles + PR_BLOCK_COST : 0;
                     int64_t sum = t;
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
@@ -493,7 +504,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
             if (threadIdx.x == 0 && g.first && g.after > 0)
                 p.heads_of[blockIdx.x] =
                     make_int4(g.b, g.h, g.qb,
-                              static_cast<int>(((place.begin + g.done + (t1 - t0) + g.after) * place.pieces - 1) / place.total));
+                              static_cast<int>(((place.begin + g.end) * place.pieces - 1) / place.total));
             __syncwarp();
             if (lane == 0) mbar_arrive(&B.segempty[seg % PR_SEGS]);
             // The 32 rows (16 by each parity's warp), each scaled by a power of two to [1, 2) at its largest, as fp16: eight lanes a row, so that copies and
@@ -820,22 +831,28 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
                 wait_on(&B.segempty[i % PR_SEGS], ((i / PR_SEGS) & 1) ^ 1, status);
                 PrSeg& g = segs[i % PR_SEGS];
                 PrItem item{};
-                int have = 0;
-                if (left > 0) {
+                int n = 0, lo = 0, hi = 0, after = 0;
+                while (left > 0 && hi <= lo) {   // the next row block with a step in this piece
                     item = pr_item(s, p.group, p.window, qb);
-                    have = item.tiles - off;
+                    const int have = item.tiles + PR_BLOCK_COST - off;
+                    n = min(have, left);
+                    if (n <= 0) break;   // lengths changed under the call
+                    lo = max(off - PR_BLOCK_COST, 0);
+                    hi = off + n - PR_BLOCK_COST;
+                    after = have - n;
+                    if (hi <= lo) left = 0;   // the piece ends before the row block's first step
                 }
-                const int n = min(have, left);
-                if (n <= 0) {   // the end (or lengths that changed under the call)
+                if (hi <= lo) {
                     g.t0 = g.t1 = 0;
                     mbar_arrive(&B.segfull[i % PR_SEGS]);
                     break;
                 }
-                g.b = b, g.h = h, g.qb = qb, g.s = s, g.done = done;
-                g.t0 = item.t0 + off;
-                g.t1 = g.t0 + n;
-                g.first = off == 0;
-                g.after = have - n;
+                g.b = b, g.h = h, g.qb = qb, g.s = s;
+                g.t0 = item.t0 + lo;
+                g.t1 = item.t0 + hi;
+                g.first = lo == 0;
+                g.after = after;
+                g.end = done + n + after;
                 mbar_arrive(&B.segfull[i % PR_SEGS]);
                 left -= n;
                 done += n;
