@@ -36,9 +36,21 @@ def _device(device) -> torch.device:
     return torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device):
     """The library launches on the current device: make it the tensors'."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):   # the same handle without a Stream object (2 us less a call)
+    def _stream(device):   # noqa: F811
+        return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _rows(t, name, device, dtypes, heads=None, dim=None):
@@ -47,11 +59,6 @@ def _rows(t, name, device, dtypes, heads=None, dim=None):
     if (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim):
         raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {dim}]")
     return t
-
-
-def _strides(t):
-    """Token and head stride in elements; 0 where there is nothing to step to."""
-    return (t.stride(0) if t.shape[0] > 1 else 0), (t.stride(1) if t.shape[1] > 1 else 0)
 
 
 class Rotary:
@@ -81,59 +88,75 @@ class Rotary:
         args = (dim, offset, int(layout == "interleaved"))
         self._c = _lib.EvaRotary(*args, 0, self.mscale, 0, self.turns.data_ptr())
         self._c_inverse = _lib.EvaRotary(*args, 1, self.mscale, 0, self.turns.data_ptr())
+        self._ref, self._ref_inverse = ctypes.byref(self._c), ctypes.byref(self._c_inverse)
+        self._pairs, self._end = layout == "interleaved", offset + dim
 
     def apply(self, x, positions, *, inverse=False, out=None):
         """x [tokens, heads, head_dim] (BF16, Half or Float; last dimension contiguous) rotated by positions (int32 or
         int64 [tokens]); inverse rotates back by the same scale, as the gradient does. out: x itself, or a tensor that does not
         overlap it; default a new one."""
-        _rows(x, "x", self.device, (_BF16, _F16, _F32))
+        device = self.device
+        if not isinstance(x, torch.Tensor) or x.ndim != 3 or x.dtype not in _DTYPE or x.device != device:
+            raise ValueError(f"x must be [tokens, heads, head_dim] of BF16, Half or Float on {device}")
         tokens, heads, head_dim = x.shape
-        if self.offset + self.dim > head_dim:
-            raise ValueError(f"x's heads have {head_dim} dimensions, the rotation ends at {self.offset + self.dim}")
+        if self._end > head_dim:
+            raise ValueError(f"x's heads have {head_dim} dimensions, the rotation ends at {self._end}")
         if heads < 1:
             raise ValueError("x has no heads")
-        if (not isinstance(positions, torch.Tensor) or positions.device != self.device or positions.ndim != 1
-                or positions.shape[0] != tokens or positions.dtype not in (_I32, _I64) or not positions.is_contiguous()):
-            raise ValueError(f"positions must be contiguous int32 or int64 [{tokens}] on {self.device}")
+        if (not isinstance(positions, torch.Tensor) or positions.ndim != 1 or positions.shape[0] != tokens
+                or positions.dtype not in (_I64, _I32) or positions.device != device or not positions.is_contiguous()):
+            raise ValueError(f"positions must be contiguous int32 or int64 [{tokens}] on {device}")
+        src = x if tokens == 0 else self._movable(x, out is x)
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=self.device)
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
         elif out is not x:
-            _rows(out, "out", self.device, (x.dtype,), heads, head_dim)
-            if out.shape[0] != tokens:
-                raise ValueError("out must have x's shape")
-            if any(st == 0 and n > 1 for n, st in zip(out.shape, out.stride())):
-                raise ValueError("out must not overlap itself")
-            if out.data_ptr() == x.data_ptr() and out.stride() == x.stride() and tokens:
-                pass   # the same memory: in place
-            elif _overlap(x, out):
-                raise ValueError("out must be x itself or not overlap it")
+            src = self._check_out(x, src, out)
         if tokens == 0:
             return out
-        src = self._movable(x, out is x)
-        dst = out if self._movable(out, True) is out else None
-        if src is None or dst is None:
-            raise ValueError("a tensor written to needs a contiguous last dimension and, with interleaved pairs, aligned ones")
-        if src is not x and out.data_ptr() == x.data_ptr():
-            raise ValueError("in place, x needs a contiguous last dimension and, with interleaved pairs, aligned ones")
-        (xt, xh), (ot, oh) = _strides(src), _strides(dst)
-        with _on(self.device):
-            rc = self.lib.eva_rotary(ctypes.byref(self._c_inverse if inverse else self._c), src.data_ptr(), _DTYPE[x.dtype],
-                                     tokens, heads, head_dim, xt, xh, positions.data_ptr(), int(positions.dtype == _I64),
-                                     dst.data_ptr(), ot, oh, torch.cuda.current_stream(self.device).cuda_stream)
-        _lib.check(rc, "eva_rotary")
+        if src is None:
+            raise ValueError("the kernel cannot move this x or out: it needs whole interleaved pairs and, of what it writes to, "
+                             "a contiguous last dimension")
+        xt, xh, _ = src.stride()
+        ot, oh, _ = out.stride()
+        if tokens == 1:
+            xt = ot = 0
+        if heads == 1:
+            xh = oh = 0
+        with _on(device):
+            rc = self.lib.eva_rotary(self._ref_inverse if inverse else self._ref, src.data_ptr(), _DTYPE[x.dtype], tokens, heads,
+                                     head_dim, xt, xh, positions.data_ptr(), positions.dtype == _I64, out.data_ptr(), ot, oh,
+                                     _stream(device))
+        if rc:
+            _lib.check(rc, "eva_rotary")
         return out
+
+    def _check_out(self, x, src, out):
+        """What to rotate from (x, or a copy of it) into a given out that is not x; None where the kernel cannot write to out."""
+        _rows(out, "out", self.device, (x.dtype,), x.shape[1], x.shape[2])
+        if out.shape[0] != x.shape[0]:
+            raise ValueError("out must have x's shape")
+        if any(st == 0 and n > 1 for n, st in zip(out.shape, out.stride())):
+            raise ValueError("out must not overlap itself")
+        same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()   # the same memory: in place
+        if not same and _overlap(x, out):
+            raise ValueError("out must be x itself or not overlap it")
+        if x.shape[0] == 0:
+            return x
+        if self._movable(out, True) is None or (same and src is not x):
+            return None
+        return src
 
     def _movable(self, t, must):
         """t, or a contiguous copy of it (None where it must be t itself), as the kernel moves it: whole elements side by side,
         interleaved pairs at addresses that are multiples of a pair."""
-        pair = self.layout == "interleaved"
-        st, sh = _strides(t)
-        ok = t.stride(2) == 1 or t.shape[2] == 1
-        if ok and pair:
-            ok = t.data_ptr() % (2 * t.element_size()) == 0 and st % 2 == 0 and sh % 2 == 0 and t.shape[2] % 2 == 0
-        if ok:
-            return t
-        if must or (pair and t.shape[2] % 2):
+        st, sh, sd = t.stride()
+        n, h, d = t.shape
+        if sd == 1 or d == 1:
+            if not self._pairs:
+                return t
+            if (t.data_ptr() % (2 * t.element_size()) == 0 and d % 2 == 0 and (st % 2 == 0 or n == 1) and (sh % 2 == 0 or h == 1)):
+                return t
+        if must or (self._pairs and d % 2):
             return None
         return t.clone(memory_format=torch.contiguous_format)
 
@@ -225,12 +248,20 @@ class PagedBatch:
             raise ValueError("table rows must not overlap")
         self._c = _lib.EvaKvBatch(self.seqs, 0, max_q, table.shape[1], stride, q_start.data_ptr(), seq_lens.data_ptr(),
                                   table.data_ptr())
+        self._refs = {}
 
     def _for(self, tokens):
-        if tokens > _INT32_MAX:
-            raise ValueError("too many token rows")
-        c = self._c
-        return _lib.EvaKvBatch(c.seqs, tokens, c.max_q, c.max_pages, c.table_stride, c.q_start, c.seq_lens, c.table)
+        """The C struct of a step of so many token rows."""
+        ref = self._refs.get(tokens)
+        if ref is None:
+            if tokens > _INT32_MAX:
+                raise ValueError("too many token rows")
+            if len(self._refs) > 64:
+                self._refs.clear()
+            c = self._c
+            ref = ctypes.byref(_lib.EvaKvBatch(c.seqs, tokens, c.max_q, c.max_pages, c.table_stride, c.q_start, c.seq_lens, c.table))
+            self._refs[tokens] = ref
+        return ref
 
 
 class PagedKVCache:
@@ -257,6 +288,7 @@ class PagedKVCache:
         self._c = _lib.EvaKvCache(pages, kv_heads, key_dim, value_dim, self.k.data_ptr(), self.v.data_ptr(),
                                   self.k_scale.data_ptr(), self.v_scale.data_ptr(), self._status.data_ptr())
         self._ref = ctypes.byref(self._c)
+        self._scale, self._sizes = key_dim ** -0.5, {}   # default scale; workspace bytes by (heads, max_q)
 
     def _buffer(self, t, shape, dtype, name):
         if t is None:
@@ -276,59 +308,77 @@ class PagedKVCache:
         v [tokens, kv_heads, value_dim] (BF16 or Half, any token and head strides), quantised. A block's scale is the smallest
         power of two that fits its tokens; one that a later token raises has its older codes rescaled. A token with a
         non-finite element gets a NaN key: the rows that see it become NaN, and no others."""
-        _rows(k, "k", self.device, (_BF16, _F16), self.kv_heads, self.key_dim)
-        _rows(v, "v", self.device, (k.dtype,), self.kv_heads, self.value_dim)
-        if v.shape[0] != k.shape[0]:
-            raise ValueError("k and v must have the same token rows")
+        device = self.device
+        if (not isinstance(k, torch.Tensor) or k.ndim != 3 or k.dtype not in (_BF16, _F16) or k.device != device
+                or k.shape[1] != self.kv_heads or k.shape[2] != self.key_dim):
+            raise ValueError(f"k must be BF16 or Half [tokens, {self.kv_heads}, {self.key_dim}] on {device}")
+        tokens = k.shape[0]
+        if (not isinstance(v, torch.Tensor) or v.ndim != 3 or v.dtype != k.dtype or v.device != device
+                or v.shape != (tokens, self.kv_heads, self.value_dim)):
+            raise ValueError(f"v must be {k.dtype} [{tokens}, {self.kv_heads}, {self.value_dim}] on {device}")
         if rotary is not None:
-            if not isinstance(rotary, Rotary) or rotary.device != self.device:
-                raise ValueError(f"rotary must be a Rotary on {self.device}")
-            if rotary.offset + rotary.dim > self.key_dim:
-                raise ValueError(f"the rotation ends at {rotary.offset + rotary.dim}, keys have {self.key_dim} dimensions")
-        b = self._batch(batch, k.shape[0])
-        k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (k, v))
-        (kt, kh), (vt, vh) = _strides(k), _strides(v)
-        with _on(self.device):
-            rc = self.lib.eva_kv_append(self._ref, ctypes.byref(b), None if rotary is None else ctypes.byref(rotary._c),
-                                        k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _DTYPE[k.dtype],
-                                        torch.cuda.current_stream(self.device).cuda_stream)
-        _lib.check(rc, "eva_kv_append")
+            if not isinstance(rotary, Rotary) or rotary.device != device:
+                raise ValueError(f"rotary must be a Rotary on {device}")
+            if rotary._end > self.key_dim:
+                raise ValueError(f"the rotation ends at {rotary._end}, keys have {self.key_dim} dimensions")
+        b = self._batch(batch, tokens)
+        if k.stride(2) != 1:
+            k = k.contiguous()
+        if v.stride(2) != 1:
+            v = v.contiguous()
+        (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
+        with _on(device):
+            rc = self.lib.eva_kv_append(self._ref, b, None if rotary is None else rotary._ref, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+                                        _DTYPE[k.dtype], _stream(device))
+        if rc:
+            _lib.check(rc, "eva_kv_append")
 
     def attend(self, q, batch, *, scale=None, window=0, out=None):
         """softmax(scale q k^T) v of q [tokens, heads, key_dim] (BF16 or Half, already rotated) over the batch's sequences,
         new tokens included: a row sees the tokens up to its own position, with window > 0 the last `window` of them.
         heads is a multiple of kv_heads. Returns [tokens, heads, value_dim] of q's type; rows that see nothing are zero, rows behind
         the last sequence are left as they were (in out; a new tensor has no values there)."""
-        _rows(q, "q", self.device, (_BF16, _F16), None, self.key_dim)
-        tokens, heads = q.shape[0], q.shape[1]
+        device = self.device
+        if (not isinstance(q, torch.Tensor) or q.ndim != 3 or q.dtype not in (_BF16, _F16) or q.device != device
+                or q.shape[2] != self.key_dim):
+            raise ValueError(f"q must be BF16 or Half [tokens, heads, {self.key_dim}] on {device}")
+        tokens, heads, _ = q.shape
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"heads must be a multiple of {self.kv_heads}")
         if type(window) is not int or not 0 <= window <= _INT32_MAX:
             raise ValueError("window must be a nonnegative int")
-        scale = self.key_dim ** -0.5 if scale is None else scale
-        if not isinstance(scale, (int, float)) or not 0 <= scale <= 3e38:
+        if scale is None:
+            scale = self._scale
+        elif not isinstance(scale, (int, float)) or not 0 <= scale <= 3e38:
             raise ValueError("scale must be a finite nonnegative number")
         b = self._batch(batch, tokens)
-        st, sh = _strides(q)
-        if q.stride(2) != 1 or st % 8 or sh % 8 or q.data_ptr() % 16:
+        st, sh, sd = q.stride()
+        if tokens == 1:
+            st = 0
+        if heads == 1:
+            sh = 0
+        if sd != 1 or st % 8 or sh % 8 or q.data_ptr() % 16:
             q = q.clone(memory_format=torch.contiguous_format)
-            st, sh = _strides(q)
+            st, sh, _ = q.stride()
         if out is None:
-            out = torch.empty(tokens, heads, self.value_dim, dtype=q.dtype, device=self.device)
-        elif (not isinstance(out, torch.Tensor) or out.device != self.device or out.dtype != q.dtype or not out.is_contiguous()
-              or tuple(out.shape) != (tokens, heads, self.value_dim) or out.data_ptr() % 16):
-            raise ValueError(f"out must be a contiguous {q.dtype} [{tokens}, {heads}, {self.value_dim}] on {self.device}, 16-byte aligned")
+            out = q.new_empty((tokens, heads, self.value_dim))
+        elif (not isinstance(out, torch.Tensor) or out.device != device or out.dtype != q.dtype or not out.is_contiguous()
+              or out.shape != (tokens, heads, self.value_dim) or out.data_ptr() % 16):
+            raise ValueError(f"out must be a contiguous {q.dtype} [{tokens}, {heads}, {self.value_dim}] on {device}, 16-byte aligned")
         elif _overlap(q, out):
             raise ValueError("out must not overlap q")
-        with _on(self.device):
-            n = self.lib.eva_kv_attend_workspace(self._ref, ctypes.byref(b), heads)
-            if n == 0:
-                raise ValueError("unsupported batch")
-            ws = torch.empty(n, dtype=_U8, device=self.device)
-            rc = self.lib.eva_kv_attend(self._ref, ctypes.byref(b), q.data_ptr(), _DTYPE[q.dtype], heads, st, sh, float(scale),
-                                        window, ws.data_ptr(), n, out.data_ptr(),
-                                        torch.cuda.current_stream(self.device).cuda_stream)
-        _lib.check(rc, "eva_kv_attend")
+        n = self._sizes.get((heads, batch.max_q))
+        with _on(device):
+            if n is None:
+                n = self.lib.eva_kv_attend_workspace(self._ref, b, heads)
+                if n == 0:
+                    raise ValueError("unsupported batch")
+                self._sizes[heads, batch.max_q] = n
+            ws = q.new_empty((n,), dtype=_U8)
+            rc = self.lib.eva_kv_attend(self._ref, b, q.data_ptr(), _DTYPE[q.dtype], heads, st, sh, scale, window, ws.data_ptr(), n,
+                                        out.data_ptr(), _stream(device))
+        if rc:
+            _lib.check(rc, "eva_kv_attend")
         return out
 
     def values(self, pages):

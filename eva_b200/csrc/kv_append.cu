@@ -1,19 +1,23 @@
 // Append to the paged 8-bit cache: rotation of the new keys, one power-of-two scale per 16 tokens and head, e4m3
 // codes, in one pass.
 //
-// A warp owns one block (16 tokens of one sequence) and head: its rows stay in registers between the maximum and
-// the rounding, so k and v are read once and the codes written once. The scale 2^e, e = ceil(log2(amax / 448)),
-// comes from the exponent and mantissa bits of amax, and dividing by it is exact, so the only roundings are the
-// rotation's (32 bits) and the one to e4m3. A block that already holds tokens keeps max(old e, new e); when
-// that raises it, the older codes are multiplied by 2^(old - new), exact until they reach e4m3's subnormals.
-// Cosines and sines come from the fast functions at a reduced angle (5e-7, against e4m3's half step of 2^-5).
+// A CTA owns one block (16 tokens of one sequence) and a warp one head at a time, whose rows stay in registers as they came
+// between the maximum and the rounding, so k and v are read once and the codes written once. The cosines and sines of the
+// block's tokens are computed once for all heads and kept in shared memory; a key is rotated twice, for the maximum and for the codes,
+// which costs less than the registers that would hold it. The scale 2^e, e = ceil(log2(amax / 448)), comes from the exponent and
+// mantissa bits of amax, and dividing by it is exact, so the only roundings are the rotation's (32 bits) and the one to e4m3.
+// A block that already holds tokens keeps max(old e, new e); when that raises it, the older codes are multiplied by
+// 2^(old - new), exact until they reach e4m3's subnormals.
 #include "kv.cuh"
 
 #include <cuda_fp8.h>
 
 namespace eva {
 
-constexpr int APPEND_WARPS = 4;   // the blocks of one page, so that its value rows' sectors meet in L2
+constexpr int APPEND_WARPS = 8;
+
+// How a lane's four key dimensions (two pairs) lie: side by side, as two neighbours in either half, or anywhere.
+constexpr int KEYS_QUADS = 0, KEYS_HALVES = 1, KEYS_SINGLE = 2;
 
 struct AppendArgs {
     EvaKvCache c;
@@ -23,7 +27,6 @@ struct AppendArgs {
     const void* v;
     int64_t kt, kh, vt, vh;
     int blocks;   // blocks one sequence's max_q rows can touch
-    int64_t warps;
 };
 
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi)
@@ -51,186 +54,288 @@ __device__ __forceinline__ float inv_scale(int byte) { return __uint_as_float(st
 
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-template <typename T> __device__ __forceinline__ float up(T v);
-template <> __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float up(__half v) { return __half2float(v); }
+// two 16-bit elements as floats; exponent bits of an element that is not finite; exponent bits above which a rotation might not be
+template <typename T> __device__ __forceinline__ float2 up2(uint32_t v);
+template <> __device__ __forceinline__ float2 up2<__nv_bfloat16>(uint32_t v)
+{
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 up2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+template <typename T> constexpr uint32_t INF_BITS = 0;
+template <> constexpr uint32_t INF_BITS<__nv_bfloat16> = 0x7f80u;
+template <> constexpr uint32_t INF_BITS<__half> = 0x7c00u;
+template <typename T> constexpr uint32_t LOUD_BITS = INF_BITS<T>;
+template <> constexpr uint32_t LOUD_BITS<__nv_bfloat16> = 0x7e00u;
 
-template <typename T, int DK, int DV>
+// Dimensions of pair i of a key: the rotated ones as the layout pairs them, the others as neighbours.
+__device__ __forceinline__ int2 key_pair(const EvaRotary& r, int i)
+{
+    if (r.interleaved || r.dim == 0) return make_int2(2 * i, 2 * i + 1);
+    if (i < r.dim / 2) return make_int2(r.offset + i, r.offset + i + r.dim / 2);
+    const int d = 2 * (i - r.dim / 2), e = d < r.offset ? d : d + r.dim;
+    return make_int2(e, e + 1);
+}
+
+template <typename T, int DK, int DV, int KEYS>
 __global__ void __launch_bounds__(APPEND_WARPS * 32) kv_append_kernel(const AppendArgs p)
 {
-    constexpr int KS = DK / 64, VS = DV / 32;   // key pairs and value dimensions of a lane
-    const int lane = threadIdx.x & 31;
-    const int64_t w = static_cast<int64_t>(blockIdx.x) * APPEND_WARPS + (threadIdx.x >> 5);
-    if (w >= p.warps) return;
-    const int64_t bh = w / p.blocks;
-    const int h = static_cast<int>(bh % p.c.kv_heads), b = static_cast<int>(bh / p.c.kv_heads);
+    constexpr int UNITS = DK / 4, KU = (UNITS + 31) / 32;   // four dimensions each; of a lane
+    __shared__ float4 turn[KV_BLOCK][UNITS];                // of a token and unit: cosines of both pairs, sines of both
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+    const int b = blockIdx.x / p.blocks;
     const KvSeq s = kv_seq(p.b, b, p.c.status);
     const int first = max(s.ctx, 0);
-    const int base = (first / KV_BLOCK + static_cast<int>(w - bh * p.blocks)) * KV_BLOCK;
+    const int base = (first / KV_BLOCK + static_cast<int>(blockIdx.x - b * p.blocks)) * KV_BLOCK;
     if (base >= s.len) return;
     const int page = kv_page(p.c, p.b, b, base / KV_PAGE, p.c.status);
     if (page < 0) return;
     const int lo = max(first - base, 0), hi = min(s.len - base, KV_BLOCK), at = base % KV_PAGE;
-    const int64_t ph = static_cast<int64_t>(page) * p.c.kv_heads + h;
     const int64_t tok0 = static_cast<int64_t>(s.row0) + base - s.ctx;   // token row of the block's slot 0
-    const T* kp = static_cast<const T*>(p.k) + h * p.kh + tok0 * p.kt;
-    const T* vp = static_cast<const T*>(p.v) + h * p.vh + tok0 * p.vt;
-
-    // values: dimension lane + 32 m, the block's tokens in registers
-    float v[VS][KV_BLOCK];
-    uint32_t bad = 0, vmax = 0;
+    const bool rotates = p.r.dim > 0;
+    if (rotates) {
+        for (int i = threadIdx.x; i < (hi - lo) * UNITS; i += blockDim.x) {
+            const int r = lo + i / UNITS, u = i % UNITS;
+            float c[2], sn[2];
 #pragma unroll
-    for (int r = 0; r < KV_BLOCK; ++r)
+            for (int k = 0; k < 2; ++k) {
+                const int pair = 2 * u + k, f = p.r.interleaved ? pair - p.r.offset / 2 : pair;   // its frequency
+                c[k] = 1.0f;
+                sn[k] = 0.0f;
+                if (f >= 0 && f < p.r.dim / 2) {
+                    sincospif(kv_half_turns(base + r, p.r.turns[f]), &sn[k], &c[k]);
+                    c[k] *= p.r.mscale;
+                    sn[k] *= p.r.mscale;
+                }
+            }
+            turn[r][u] = make_float4(c[0], c[1], sn[0], sn[1]);
+        }
+        __syncthreads();
+    }
+    int da[KU][2], db[KU][2];   // KEYS_SINGLE: the unit's dimensions; else da[.][0], db[.][0] begin its two neighbours
+    bool has[KU];
 #pragma unroll
-        for (int m = 0; m < VS; ++m) v[m][r] = r >= lo && r < hi ? up(vp[r * p.vt + lane + 32 * m]) : 0.0f;
-    // keys: pair lane + 32 m of the rotated pairs, then of the others (neighbours)
-    float ka[KS][KV_BLOCK], kb[KS][KV_BLOCK];
-    int da[KS], db[KS];
-    const int half = p.r.dim / 2;
+    for (int m = 0; m < KU; ++m) {
+        const int u = lane + 32 * m;
+        has[m] = u < UNITS;
 #pragma unroll
-    for (int m = 0; m < KS; ++m) {
-        const int i = lane + 32 * m;
-        if (i < half) {
-            da[m] = p.r.offset + (p.r.interleaved ? 2 * i : i);
-            db[m] = da[m] + (p.r.interleaved ? 1 : half);
-        } else {
-            const int d = 2 * (i - half);
-            da[m] = d < p.r.offset ? d : d + p.r.dim;
-            db[m] = da[m] + 1;
+        for (int k = 0; k < 2; ++k) {
+            const int2 d = key_pair(p.r, min(2 * u + k, DK / 2 - 1));
+            da[m][k] = d.x;
+            db[m][k] = d.y;
         }
     }
-#pragma unroll
-    for (int m = 0; m < KS; ++m)
+    for (int h = warp; h < p.c.kv_heads; h += nwarps) {
+        const int64_t ph = static_cast<int64_t>(page) * p.c.kv_heads + h;
+        const T* kp = static_cast<const T*>(p.k) + h * p.kh + tok0 * p.kt;
+        const T* vp = static_cast<const T*>(p.v) + h * p.vh + tok0 * p.vt + 4 * lane;
+        // the raw rows: values of dimensions 4 lane .. 4 lane + 3; key units as (a0, a1), (b0, b1)
+        uint32_t v[KV_BLOCK][2], ka[KU][KV_BLOCK], kb[KU][KV_BLOCK];
 #pragma unroll
         for (int r = 0; r < KV_BLOCK; ++r) {
             const bool in = r >= lo && r < hi;
-            ka[m][r] = in ? up(kp[r * p.kt + da[m]]) : 0.0f;
-            kb[m][r] = in ? up(kp[r * p.kt + db[m]]) : 0.0f;
-        }
+            v[r][0] = v[r][1] = 0;
+            if (in && 4 * lane < DV) {
+                if constexpr (KEYS != KEYS_SINGLE) {
+                    const uint2 w = *reinterpret_cast<const uint2*>(vp + r * p.vt);
+                    v[r][0] = w.x;
+                    v[r][1] = w.y;
+                } else {
+                    const uint16_t* q = reinterpret_cast<const uint16_t*>(vp + r * p.vt);
+                    v[r][0] = q[0] | static_cast<uint32_t>(q[1]) << 16;
+                    v[r][1] = q[2] | static_cast<uint32_t>(q[3]) << 16;
+                }
+            }
 #pragma unroll
-    for (int m = 0; m < VS; ++m)
+            for (int m = 0; m < KU; ++m) {
+                ka[m][r] = kb[m][r] = 0;
+                if (in && has[m]) {
+                    const uint16_t* q = reinterpret_cast<const uint16_t*>(kp + r * p.kt);
+                    if constexpr (KEYS == KEYS_QUADS) {   // a0 b0 a1 b1
+                        const uint2 w = *reinterpret_cast<const uint2*>(q + da[m][0]);
+                        ka[m][r] = __byte_perm(w.x, w.y, 0x5410);
+                        kb[m][r] = __byte_perm(w.x, w.y, 0x7632);
+                    } else if constexpr (KEYS == KEYS_HALVES) {
+                        // rotated: neighbours (a0, a1) and (b0, b1); else (a0, b0) and (a1, b1)
+                        const bool turned = 2 * (lane + 32 * m) < p.r.dim / 2;
+                        const uint32_t x = *reinterpret_cast<const uint32_t*>(q + da[m][0]);
+                        const uint32_t y = *reinterpret_cast<const uint32_t*>(q + (turned ? db[m][0] : da[m][1]));
+                        ka[m][r] = turned ? x : __byte_perm(x, y, 0x5410);
+                        kb[m][r] = turned ? y : __byte_perm(x, y, 0x7632);
+                    } else {
+                        ka[m][r] = q[da[m][0]] | static_cast<uint32_t>(q[da[m][1]]) << 16;
+                        kb[m][r] = q[db[m][0]] | static_cast<uint32_t>(q[db[m][1]]) << 16;
+                    }
+                }
+            }
+        }
+        // largest magnitudes of the raw elements, as integers of 16 bits (NaN above infinity above all)
+        uint32_t vmax = 0, kraw = 0;
 #pragma unroll
         for (int r = 0; r < KV_BLOCK; ++r) {
-            if (!finite(v[m][r])) {
-                bad |= 1u << r;
-                v[m][r] = 0.0f;
-            }
-            vmax = max(vmax, __float_as_uint(fabsf(v[m][r])));
-        }
-    uint32_t kmax = 0;
+            vmax = __vimax3_u16x2(vmax, v[r][0] & 0x7fff7fffu, v[r][1] & 0x7fff7fffu);
 #pragma unroll
-    for (int m = 0; m < KS; ++m) {
-        const int i = lane + 32 * m;
-        if (i < half) {
-            const uint64_t turns = p.r.turns[i];
+            for (int m = 0; m < KU; ++m) kraw = __vimax3_u16x2(kraw, ka[m][r] & 0x7fff7fffu, kb[m][r] & 0x7fff7fffu);
+        }
+        vmax = max(vmax & 0xffffu, vmax >> 16);
+        kraw = max(kraw & 0xffffu, kraw >> 16);
+        auto rotated = [&](int m, int r, float2& ya, float2& yb) {
+            const float2 a = up2<T>(ka[m][r]), c = up2<T>(kb[m][r]);
+            ya = a;
+            yb = c;
+            if (rotates) {
+                const float4 t = turn[r][has[m] ? lane + 32 * m : 0];
+                const float2 cs = make_float2(t.x, t.y), sn = make_float2(t.z, t.w);
+                ya = fma2(c, make_float2(-sn.x, -sn.y), mul2(a, cs));
+                yb = fma2(a, sn, mul2(c, cs));
+            }
+        };
+        // A token with an element that is not finite has no key of its own, and does not count for the scale.
+        uint32_t bad = 0;
+        if (__any_sync(0xffffffffu, vmax >= INF_BITS<T> || kraw >= LOUD_BITS<T>)) {
+            vmax = 0;
+#pragma unroll 1
+            for (int r = lo; r < hi; ++r) {
+                bool odd = false;
 #pragma unroll
-            for (int r = 0; r < KV_BLOCK; ++r) {
-                float sn, cs;
-                __sincosf(kv_half_turns(base + r, turns) * 3.14159265358979f, &sn, &cs);
-                sn *= p.r.mscale;
-                cs *= p.r.mscale;
-                const float x = ka[m][r], y = kb[m][r];
-                ka[m][r] = x * cs - y * sn;
-                kb[m][r] = y * cs + x * sn;
+                for (int x = 0; x < KV_BLOCK; ++x) {   // (registers have no index)
+                    if (x != r) continue;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        uint32_t w = v[x][k];
+                        if ((w & 0x7fffu) >= INF_BITS<T>) w &= 0xffff0000u, odd = true;
+                        if ((w >> 16 & 0x7fffu) >= INF_BITS<T>) w &= 0xffffu, odd = true;
+                        v[x][k] = w;
+                        vmax = max(vmax, max(w & 0x7fffu, w >> 16 & 0x7fffu));
+                    }
+#pragma unroll
+                    for (int m = 0; m < KU; ++m) {
+                        float2 ya, yb;
+                        rotated(m, x, ya, yb);
+                        odd |= !finite(ya.x) || !finite(ya.y) || !finite(yb.x) || !finite(yb.y);
+                    }
+                }
+                if (__any_sync(0xffffffffu, odd)) bad |= 1u << r;
             }
         }
+        float kmax = 0.0f;
 #pragma unroll
         for (int r = 0; r < KV_BLOCK; ++r) {
-            if (!finite(ka[m][r]) || !finite(kb[m][r])) bad |= 1u << r;
-            if (finite(ka[m][r])) kmax = max(kmax, __float_as_uint(fabsf(ka[m][r])));
-            if (finite(kb[m][r])) kmax = max(kmax, __float_as_uint(fabsf(kb[m][r])));
-        }
-    }
-    bad = __reduce_or_sync(0xffffffffu, bad);
-    // a token with a non-finite element has no key of its own: it does not count for the scale either
-    if (bad) {
-        kmax = 0;
+            if (bad >> r & 1 || r < lo || r >= hi) continue;
 #pragma unroll
-        for (int m = 0; m < KS; ++m)
-#pragma unroll
-            for (int r = 0; r < KV_BLOCK; ++r) {
-                if (bad >> r & 1) ka[m][r] = kb[m][r] = __uint_as_float(0x7fc00000u);
-                else kmax = max(kmax, max(__float_as_uint(fabsf(ka[m][r])), __float_as_uint(fabsf(kb[m][r]))));
-            }
-    }
-    kmax = __reduce_max_sync(0xffffffffu, kmax);
-    vmax = __reduce_max_sync(0xffffffffu, vmax);
-
-    uint8_t* ks = static_cast<uint8_t*>(p.c.k_scale) + ph * KV_PAGE_BLOCKS + at / KV_BLOCK;
-    uint8_t* vs = static_cast<uint8_t*>(p.c.v_scale) + ph * KV_PAGE_BLOCKS + at / KV_BLOCK;
-    uint8_t* kc = static_cast<uint8_t*>(p.c.k) + (ph * KV_PAGE + at) * DK;
-    uint8_t* vc = static_cast<uint8_t*>(p.c.v) + ph * KV_PAGE * DV + at;
-    int ke = scale_byte(kmax), ve = scale_byte(vmax);
-    if (lo > 0) {
-        const int ko = max(static_cast<int>(*ks), 1), vo = max(static_cast<int>(*vs), 1);
-        ke = max(ke, ko);
-        ve = max(ve, vo);
-        if (ke > ko) {   // the older keys: lo rows of DK bytes, contiguous
-            const float m = inv_scale(ke) * kv_scale(ko);
-            for (int i = lane; i < lo * DK / 2; i += 32) {
-                uint16_t* q = reinterpret_cast<uint16_t*>(kc) + i;
-                *q = static_cast<uint16_t>(e4m3_scaled(*q, m));
+            for (int m = 0; m < KU; ++m) {
+                float2 ya, yb;
+                rotated(m, r, ya, yb);
+                kmax = fmaxf(fmaxf(kmax, fmaxf(fabsf(ya.x), fabsf(ya.y))), fmaxf(fabsf(yb.x), fabsf(yb.y)));
             }
         }
-        const float m = inv_scale(ve) * kv_scale(vo);
-#pragma unroll
-        for (int j = 0; j < VS; ++j) {
-            uint8_t* q = vc + static_cast<int64_t>(lane + 32 * j) * KV_PAGE;
-            const uint4 o = *reinterpret_cast<const uint4*>(q);
-            uint32_t in[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {   // tokens 2 t, 2 t + 1
-                const uint32_t was = in[t / 2] >> (t % 2 * 16) & 0xffffu;
-                const uint32_t moved = ve > vo ? e4m3_scaled(was, m) : was;
-                const uint32_t fresh = e4m3x2(v[j][2 * t] * inv_scale(ve), v[j][2 * t + 1] * inv_scale(ve));
-                const uint32_t a = 2 * t < lo ? moved : 2 * t < hi ? fresh : was;
-                const uint32_t c = 2 * t + 1 < lo ? moved : 2 * t + 1 < hi ? fresh : was;
-                const uint32_t two = (a & 0xffu) | (c & 0xff00u);
-                in[t / 2] = t % 2 ? (in[t / 2] & 0xffffu) | two << 16 : (in[t / 2] & 0xffff0000u) | two;
+        vmax = __reduce_max_sync(0xffffffffu, vmax);
+        uint8_t* ks = static_cast<uint8_t*>(p.c.k_scale) + ph * KV_PAGE_BLOCKS + at / KV_BLOCK;
+        uint8_t* vs = static_cast<uint8_t*>(p.c.v_scale) + ph * KV_PAGE_BLOCKS + at / KV_BLOCK;
+        uint8_t* kc = static_cast<uint8_t*>(p.c.k) + (ph * KV_PAGE + at) * DK;
+        uint8_t* vc = static_cast<uint8_t*>(p.c.v) + ph * KV_PAGE * DV + at;
+        int ke = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(kmax)));
+        int ve = scale_byte(__float_as_uint(up2<T>(vmax).x));
+        float vmoved = 1.0f;
+        bool vgrown = false;
+        if (lo > 0) {
+            const int ko = min(max(static_cast<int>(*ks), 1), 253), vo = min(max(static_cast<int>(*vs), 1), 253);
+            ke = max(ke, ko);
+            ve = max(ve, vo);
+            vgrown = ve > vo;
+            vmoved = inv_scale(ve) * kv_scale(vo);
+            if (ke > ko) {   // the older keys: lo rows of DK bytes, contiguous
+                const float m = inv_scale(ke) * kv_scale(ko);
+                for (int i = lane; i < lo * DK / 2; i += 32) {
+                    uint16_t* q = reinterpret_cast<uint16_t*>(kc) + i;
+                    *q = static_cast<uint16_t>(e4m3_scaled(*q, m));
+                }
             }
-            *reinterpret_cast<uint4*>(q) = make_uint4(in[0], in[1], in[2], in[3]);
         }
-    } else {
+        const float vinv = inv_scale(ve), kinv = inv_scale(ke);
+        if (4 * lane < DV) {
+            const bool merge = lo > 0 || hi < KV_BLOCK;   // the block holds, or may hold, other tokens' bytes
 #pragma unroll
-        for (int j = 0; j < VS; ++j) {
-            uint8_t* q = vc + static_cast<int64_t>(lane + 32 * j) * KV_PAGE;
-            uint32_t in[4] = {0, 0, 0, 0};
+            for (int j = 0; j < 4; ++j) {
+                uint8_t* q = vc + static_cast<int64_t>(4 * lane + j) * KV_PAGE;
+                uint4 was = make_uint4(0, 0, 0, 0);
+                if (merge) was = *reinterpret_cast<const uint4*>(q);
+                uint32_t in[4] = {was.x, was.y, was.z, was.w};
 #pragma unroll
-            for (int t = 0; t < 8; ++t)
-                in[t / 2] |= e4m3x2(v[j][2 * t] * inv_scale(ve), v[j][2 * t + 1] * inv_scale(ve)) << (t % 2 * 16);
-            if (hi == KV_BLOCK) {
+                for (int t = 0; t < 8; ++t) {   // tokens 2 t, 2 t + 1
+                    const float2 x = up2<T>(v[2 * t][j / 2]), y = up2<T>(v[2 * t + 1][j / 2]);
+                    uint32_t two = e4m3x2((j % 2 ? x.y : x.x) * vinv, (j % 2 ? y.y : y.x) * vinv);
+                    if (merge) {
+                        const uint32_t old = in[t / 2] >> (t % 2 * 16) & 0xffffu;
+                        const uint32_t moved = vgrown ? e4m3_scaled(old, vmoved) : old;
+                        const uint32_t a = 2 * t < lo ? moved : 2 * t < hi ? two : old;
+                        const uint32_t c = 2 * t + 1 < lo ? moved : 2 * t + 1 < hi ? two : old;
+                        two = (a & 0xffu) | (c & 0xff00u);
+                    }
+                    in[t / 2] = t % 2 ? (in[t / 2] & 0xffffu) | two << 16 : (in[t / 2] & 0xffff0000u) | two;
+                }
                 *reinterpret_cast<uint4*>(q) = make_uint4(in[0], in[1], in[2], in[3]);
-            } else {
-                for (int t = 0; t < KV_BLOCK; ++t)
-                    if (t < hi) q[t] = static_cast<uint8_t>(in[t / 4] >> (t % 4 * 8));
             }
         }
-    }
-    const float inv = inv_scale(ke);
 #pragma unroll
-    for (int m = 0; m < KS; ++m)
+        for (int r = 0; r < KV_BLOCK; ++r) {
+            if (r < lo || r >= hi) continue;
 #pragma unroll
-        for (int r = 0; r < KV_BLOCK; ++r)
-            if (r >= lo && r < hi) {
-                const uint32_t two = e4m3x2(ka[m][r] * inv, kb[m][r] * inv);
-                kc[r * DK + da[m]] = static_cast<uint8_t>(two);
-                kc[r * DK + db[m]] = static_cast<uint8_t>(two >> 8);
+            for (int m = 0; m < KU; ++m) {
+                float2 ya, yb;
+                rotated(m, r, ya, yb);
+                uint32_t x = e4m3x2(ya.x * kinv, ya.y * kinv), y = e4m3x2(yb.x * kinv, yb.y * kinv);   // (a0, a1), (b0, b1)
+                if (bad >> r & 1) x = y = 0x7f7fu;
+                if (!has[m]) continue;
+                uint8_t* q = kc + r * DK;
+                const bool neighbours = KEYS == KEYS_QUADS || (KEYS == KEYS_HALVES && 2 * (lane + 32 * m) >= p.r.dim / 2);
+                if constexpr (KEYS == KEYS_SINGLE) {
+                    q[da[m][0]] = static_cast<uint8_t>(x);
+                    q[da[m][1]] = static_cast<uint8_t>(x >> 8);
+                    q[db[m][0]] = static_cast<uint8_t>(y);
+                    q[db[m][1]] = static_cast<uint8_t>(y >> 8);
+                } else if (neighbours) {
+                    const uint32_t w = __byte_perm(x, y, 0x5140);   // a0 b0 a1 b1
+                    if constexpr (KEYS == KEYS_QUADS) {
+                        *reinterpret_cast<uint32_t*>(q + da[m][0]) = w;
+                    } else {
+                        *reinterpret_cast<uint16_t*>(q + da[m][0]) = static_cast<uint16_t>(w);
+                        *reinterpret_cast<uint16_t*>(q + da[m][1]) = static_cast<uint16_t>(w >> 16);
+                    }
+                } else {
+                    *reinterpret_cast<uint16_t*>(q + da[m][0]) = static_cast<uint16_t>(x);
+                    *reinterpret_cast<uint16_t*>(q + db[m][0]) = static_cast<uint16_t>(y);
+                }
             }
-    __syncwarp();   // every lane has read the old scales
-    if (lane == 0) {
-        *ks = static_cast<uint8_t>(ke);
-        *vs = static_cast<uint8_t>(ve);
+        }
+        __syncwarp();   // every lane has read the old scales
+        if (lane == 0) {
+            *ks = static_cast<uint8_t>(ke);
+            *vs = static_cast<uint8_t>(ve);
+        }
     }
+}
+
+template <typename T, int DK, int DV> static void append_launch(const AppendArgs& p, int keys, unsigned grid, cudaStream_t st)
+{
+    const int threads = 32 * (p.c.kv_heads < APPEND_WARPS ? p.c.kv_heads : APPEND_WARPS);
+    if (keys == KEYS_QUADS) kv_append_kernel<T, DK, DV, KEYS_QUADS><<<grid, threads, 0, st>>>(p);
+    else if (keys == KEYS_HALVES) kv_append_kernel<T, DK, DV, KEYS_HALVES><<<grid, threads, 0, st>>>(p);
+    else kv_append_kernel<T, DK, DV, KEYS_SINGLE><<<grid, threads, 0, st>>>(p);
 }
 
 template <typename T> static cudaError_t append_typed(const AppendArgs& p, cudaStream_t st)
 {
-    const int64_t grid = (p.warps + APPEND_WARPS - 1) / APPEND_WARPS;
+    const int64_t grid = static_cast<int64_t>(p.b.seqs) * p.blocks;
     if (grid > 0x7fffffff) return cudaErrorInvalidValue;
+    // Four dimensions at a time where rows, heads and the rotation's halves lie on their boundaries; else one by one.
+    const uint64_t off = reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) |
+                         static_cast<uint64_t>(p.kt | p.kh | p.vt | p.vh) * 2;
+    const bool quads = p.r.interleaved || p.r.dim == 0;
+    const int keys = off % 8 != 0 ? KEYS_SINGLE : quads ? KEYS_QUADS : p.r.dim % 4 == 0 ? KEYS_HALVES : KEYS_SINGLE;
     const unsigned g = static_cast<unsigned>(grid);
-    if (p.c.key_dim == 64) kv_append_kernel<T, 64, 64><<<g, APPEND_WARPS * 32, 0, st>>>(p);
-    else if (p.c.key_dim == 128) kv_append_kernel<T, 128, 128><<<g, APPEND_WARPS * 32, 0, st>>>(p);
-    else kv_append_kernel<T, 192, 128><<<g, APPEND_WARPS * 32, 0, st>>>(p);
+    if (p.c.key_dim == 64) append_launch<T, 64, 64>(p, keys, g, st);
+    else if (p.c.key_dim == 128) append_launch<T, 128, 128>(p, keys, g, st);
+    else append_launch<T, 192, 128>(p, keys, g, st);
     return cudaGetLastError();
 }
 
@@ -281,7 +386,6 @@ extern "C" int eva_kv_append(const EvaKvCache* cache, const EvaKvBatch* batch, c
     p.vt = v_token_stride;
     p.vh = v_head_stride;
     p.blocks = (batch->max_q + KV_BLOCK - 2) / KV_BLOCK + 1;
-    p.warps = static_cast<int64_t>(batch->seqs) * cache->kv_heads * p.blocks;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const cudaError_t e = dtype == EVA_DTYPE_BF16 ? append_typed<__nv_bfloat16>(p, st) : append_typed<__half>(p, st);
     return e == cudaSuccess ? EVA_OK : EVA_ERR_CUDA;

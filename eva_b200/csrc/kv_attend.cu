@@ -436,7 +436,8 @@ __global__ void __launch_bounds__(COMBINE_THREADS) kv_combine_kernel(const Atten
 template <int DK, int DV, typename T> static cudaError_t decode_launch(const AttendArgs& p, int pieces, cudaStream_t st)
 {
     using C = DecCfg<DK, DV>;
-    cudaError_t e = cudaFuncSetAttribute(kv_decode_kernel<DK, DV, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_smem(reinterpret_cast<const void*>(&kv_decode_kernel<DK, DV, T>), C::SMEM, done);
     if (e != cudaSuccess) return e;
     kv_decode_kernel<DK, DV, T><<<pieces / C::W, C::W * 32, C::SMEM, st>>>(p);
     e = cudaGetLastError();

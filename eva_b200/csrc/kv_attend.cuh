@@ -1,6 +1,8 @@
 // Shared by the attention kernels over the paged cache.
 #pragma once
 
+#include <atomic>
+
 #include "kv.cuh"
 
 namespace eva {
@@ -65,6 +67,18 @@ __device__ __forceinline__ float ex2(float x)
     float y;
     asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Shared memory of a kernel above the default, set once per device (`done`: a bit each).
+inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done)
+{
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = dev >= 0 && dev < 64 ? uint64_t{1} << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 // Many rows (kv_prompt.cu): workspace bytes for a value dimension, and the launch.

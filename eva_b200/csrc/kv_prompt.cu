@@ -932,7 +932,8 @@ __global__ void __launch_bounds__(COMBINE_THREADS) kv_prompt_combine(const Atten
 template <int DK, int DV, typename T> static cudaError_t prompt_launch(const AttendArgs& p, cudaStream_t st)
 {
     using C = PrCfg<DK, DV>;
-    cudaError_t e = cudaFuncSetAttribute(kv_prompt_kernel<DK, DV, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_smem(reinterpret_cast<const void*>(&kv_prompt_kernel<DK, DV, T>), C::SMEM, done);
     if (e != cudaSuccess) return e;
     const int pieces = num_sms();
     kv_prompt_kernel<DK, DV, T><<<pieces, PR_WARPS * 32, C::SMEM, st>>>(p);
