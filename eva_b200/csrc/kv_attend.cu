@@ -3,13 +3,16 @@
 // At most 16 rows (new tokens x query heads of a group) share each key and value, so the cache's bytes are the cost: every
 // one is read once. The tokens of all sequences and heads, in tiles of a page (64), form one line of work that is cut
 // into equal pieces, one per warp of the GPU, whatever the lengths are; a warp's tiles come through its own
-// two-stage ring of bulk copies (a page of a head is contiguous). Scores and outputs are m16n8k16 products with fp32 sums
-// on the codes themselves (e4m3 is exact in fp16). Their scales stay outside: a token's key scale multiplies its
-// score, its value scale 2^e joins the exponent, t = score + e, and the softmax's running maximum is that of t:
+// two-stage ring of bulk copies (a page of a head is contiguous). Scores and outputs are m16n8k16 products with fp32 sums,
+// transposed: keys and values are the 16-row operand and the query rows the 8-column one, so that up to eight rows cost what one
+// does and no product is padding. The codes themselves are multiplied (e4m3 is exact in fp16); their scales stay outside: a
+// token's key scale multiplies its score, its value scale 2^e joins the exponent, t = score + e, and the softmax's running
+// maximum is that of t:
 //   out = sum 2^(t - M) code / sum 2^(t - M) 2^-e.
 // Weights are rounded to fp16 with 2^14 as the largest, so that tokens down to 2^-28 of the largest keep 11 bits.
-// The order of a tile's tokens within a product is free, and chosen so that both operands are 16-byte shared-memory loads:
-// lane quad q holds tokens 16 q .. 16 q + 15 (one scale block) and, of the keys, dimensions 16 q .. 16 q + 15 of each 64.
+// The order of a tile's tokens within a product is free, and chosen so that both operands are 16-byte shared-memory loads and
+// the weights need no exchange but movmatrix: product e of a tile has, in its rows r and r + 8, tokens
+// 16 (r / 2) + 4 e + (0, 2) + r % 2, and lane quad q holds of the values tokens 16 q .. 16 q + 15.
 // An item (sequence and head) whose tiles fall to several warps leaves fp32 partial sums, which
 // kv_combine_kernel joins in their order, so results do not depend on timing.
 #include <algorithm>
@@ -47,6 +50,14 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Transposes an 8 x 8 matrix of halves whose row lane / 4 has its columns 2 (lane % 4), + 1 in x.
+__device__ __forceinline__ uint32_t transposed(uint32_t x)
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
 // Tiles of one head of a sequence: the pages from the first token that its first row sees to its last one. A sequence with
 // rows but no token has one (empty) tile, so that its rows are written.
 __device__ __forceinline__ int dec_tiles(const KvSeq& s, int window, int* first)
@@ -60,17 +71,18 @@ struct DecTile {   // what the consumer of a tile needs
     int b, h, n, row0, len, tok;     // tok: first token; -1: nothing to read
     bool first, last;                // of its item
     int left;                        // tiles of the item after this one
-    uint32_t ks, vs;                 // scale bytes of the lane quad's block
+    uint32_t ks, vs;                 // scale bytes of the block of the lane's scores (lane / 8)
 };
 
-template <int DK, int DV, typename T>
+// NT: groups of eight rows
+template <int DK, int DV, typename T, int NT>
 __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(const AttendArgs p)
 {
     using C = DecCfg<DK, DV>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ alignas(8) uint64_t bars[C::W][C::STAGES];
     __shared__ int sums[C::W];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane & 3, n8 = lane >> 2;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane & 3, r8 = lane >> 2;
     uint8_t* ring = smem_raw + ((128 - (smem_u32(smem_raw) & 127)) & 127) + warp * C::STAGES * C::STAGE;
     if (lane == 0) {
         for (int i = 0; i < C::STAGES; ++i) mbar_init(&bars[warp][i], 1);
@@ -146,8 +158,8 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
                 if (page >= 0) {
                     t.tok = pi * KV_PAGE;
                     const int64_t ph = static_cast<int64_t>(page) * p.c.kv_heads + h;
-                    t.ks = static_cast<const uint8_t*>(p.c.k_scale)[ph * KV_PAGE_BLOCKS + quad];
-                    t.vs = static_cast<const uint8_t*>(p.c.v_scale)[ph * KV_PAGE_BLOCKS + quad];
+                    t.ks = static_cast<const uint8_t*>(p.c.k_scale)[ph * KV_PAGE_BLOCKS + (lane >> 3)];
+                    t.vs = static_cast<const uint8_t*>(p.c.v_scale)[ph * KV_PAGE_BLOCKS + (lane >> 3)];
                     if (lane == 0) {
                         uint8_t* dst = ring + slot * C::STAGE;
                         mbar_arrive_expect_tx(&bars[warp][slot], C::STAGE);
@@ -177,22 +189,22 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
         DecTile cur{}, nxt{};
         if (next < end) cur = issue(0);
         if (next < end) nxt = issue(1);
-        uint32_t qf[DK / 16][4];
-        float o[DV / 8][4], m0 = 0, m1 = 0, l0 = 0, l1 = 0, c0 = 0, c1 = 0;
-        int hi0 = 0, hi1 = 0, lo0 = 0, lo1 = 0;
+        // of each group of rows: the query as B operand, the output (rows 2 quad, + 1 of dimensions r8, r8 + 8 of each 16), and of
+        // rows 2 quad, + 1 maximum, sum, factor and range of tokens
+        uint32_t qf[NT][DK / 16][2];
+        float o[NT][DV / 16][4], m[NT][2], l[NT][2], c[NT][2];
+        int hi[NT][2], lo[NT][2];
         bool whole = false;
         for (int64_t at = begin; at < end; ++at) {
             const int slot = static_cast<int>(at - begin) & 1;
             if (cur.first || at == begin) {
                 whole = cur.first;
-                m0 = m1 = -INFINITY;
-                l0 = l1 = 0.0f;
 #pragma unroll
-                for (int j = 0; j < DV / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-                // query rows n8 and n8 + 8, scaled by a power of two to [1, 2) at their largest
+                for (int g8 = 0; g8 < NT; ++g8) {
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int r = n8 + 8 * half, tok = r / p.group;
+                    for (int j = 0; j < DV / 16; ++j) o[g8][j][0] = o[g8][j][1] = o[g8][j][2] = o[g8][j][3] = 0.0f;
+                    // query row r8 of the group, scaled by a power of two to [1, 2) at its largest
+                    const int r = 8 * g8 + r8, tok = r / p.group;
                     const bool in = tok < cur.n;
                     const T* q = static_cast<const T*>(p.q) + (static_cast<int64_t>(cur.row0) + tok) * p.qt +
                                  (static_cast<int64_t>(cur.h) * p.group + (r - tok * p.group)) * p.qh + quad * 16;
@@ -218,12 +230,10 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
                         }
                     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
                     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-                    const uint32_t some_odd = __ballot_sync(0xffffffffu, odd);
-                    odd = (some_odd >> (n8 * 4) & 15u) != 0 || big == INFINITY;
+                    odd = (__ballot_sync(0xffffffffu, odd) >> (r8 * 4) & 15u) != 0 || big == INFINITY;
                     const int e2 = min(max(static_cast<int>(__float_as_uint(big) >> 23), 1), 252);
                     const float down = __uint_as_float(static_cast<uint32_t>(254 - e2) << 23);
-                    const float c = odd ? __uint_as_float(0x7fc00000u)
-                                        : p.scale * __uint_as_float(static_cast<uint32_t>(e2) << 23);
+                    const float own = odd ? __uint_as_float(0x7fc00000u) : p.scale * __uint_as_float(static_cast<uint32_t>(e2) << 23);
 #pragma unroll
                     for (int j = 0; j < DK / 64; ++j)
 #pragma unroll
@@ -232,14 +242,19 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const float2 f = two_floats<T>(w[e]);
-                                // elements 8 k + 2 e, + 1 of the lane's 16: step 2 k + e / 2, k index pair e % 2
-                                qf[j * 4 + 2 * k + e / 2][half + 2 * (e % 2)] = half2_bits(f.x * down, f.y * down);
+                                // elements 8 k + 2 e, + 1 of the lane's 16: product 2 k + e / 2, k index pair e % 2
+                                qf[g8][j * 4 + 2 * k + e / 2][e % 2] = half2_bits(f.x * down, f.y * down);
                             }
                         }
-                    const int hi = in ? cur.len - cur.n + tok + 1 : 0;
-                    const int lo = p.window > 0 ? max(0, hi - p.window) : 0;
-                    if (half == 0) c0 = c, hi0 = hi, lo0 = lo;
-                    else c1 = c, hi1 = hi, lo1 = lo;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int t = (8 * g8 + 2 * quad + x) / p.group;
+                        c[g8][x] = __shfl_sync(0xffffffffu, own, 8 * quad + 4 * x);
+                        hi[g8][x] = t < cur.n ? cur.len - cur.n + t + 1 : 0;
+                        lo[g8][x] = p.window > 0 ? max(0, hi[g8][x] - p.window) : 0;
+                        m[g8][x] = -INFINITY;
+                        l[g8][x] = 0.0f;
+                    }
                 }
             }
             if (cur.tok >= 0) {
@@ -247,72 +262,84 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
                 const uint8_t* V = K + C::KB;
                 mbar_wait(&bars[warp][slot], phase >> slot & 1, p.c.status);
                 phase ^= 1u << slot;
-                float sc[8][4];   // 4-token step i, half h: [2 i + h]; columns: tokens 16 quad + 4 i + 2 h + {0, 1}
+                float sc[NT][4][4];   // product e: tokens t0 + 4 e + (0, 0, 2, 2), rows 2 quad + (0, 1, 0, 1)
 #pragma unroll
-                for (int ih = 0; ih < 8; ++ih) {
-                    sc[ih][0] = sc[ih][1] = sc[ih][2] = sc[ih][3] = 0.0f;
-                    const uint8_t* kr = K + (16 * (n8 >> 1) + 2 * ih + (n8 & 1)) * DK + quad * 16;
+                for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                    for (int g8 = 0; g8 < NT; ++g8) sc[g8][e][0] = sc[g8][e][1] = sc[g8][e][2] = sc[g8][e][3] = 0.0f;
+                    const uint8_t* kr = K + (16 * (r8 >> 1) + 4 * e + (r8 & 1)) * DK + quad * 16;
 #pragma unroll
                     for (int j = 0; j < DK / 64; ++j) {
-                        const uint4 w4 = *reinterpret_cast<const uint4*>(kr + j * 64);
-                        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+                        const uint4 x4 = *reinterpret_cast<const uint4*>(kr + j * 64);
+                        const uint4 y4 = *reinterpret_cast<const uint4*>(kr + 2 * DK + j * 64);
+                        const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            uint32_t k0, k1;
-                            e4m3_halves(w[e], k0, k1);
-                            mma_f16(sc[ih], qf[j * 4 + e][0], qf[j * 4 + e][1], qf[j * 4 + e][2], qf[j * 4 + e][3], k0, k1);
+                        for (int k = 0; k < 4; ++k) {
+                            uint32_t a0, a1, a2, a3;
+                            e4m3_halves(x[k], a0, a2);
+                            e4m3_halves(y[k], a1, a3);
+#pragma unroll
+                            for (int g8 = 0; g8 < NT; ++g8) mma_f16(sc[g8][e], a0, a1, a2, a3, qf[g8][j * 4 + k][0], qf[g8][j * 4 + k][1]);
                         }
                     }
                 }
                 const float ks = kv_scale(cur.ks), vlog = static_cast<float>(static_cast<int>(max(cur.vs, 1u)) - 127);
-                const float f0 = ks * c0, f1 = ks * c1;
-                const int t0 = cur.tok + 16 * quad;
-                const bool part = cur.tok + KV_PAGE > cur.len - cur.n + 1 || p.window > 0;   // some row does not see all
-                float x0 = -INFINITY, x1 = -INFINITY;
-#pragma unroll
-                for (int ih = 0; ih < 8; ++ih)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float a = sc[ih][e] * f0 + vlog, c = sc[ih][2 + e] * f1 + vlog;
-                        if (part) {
-                            const int t = t0 + 2 * ih + e;
-                            a = t >= lo0 && t < hi0 ? a : -INFINITY;
-                            c = t >= lo1 && t < hi1 ? c : -INFINITY;
-                        }
-                        sc[ih][e] = a;
-                        sc[ih][2 + e] = c;
-                        x0 = fmaxf(x0, a);
-                        x1 = fmaxf(x1, c);
-                    }
-                x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-                x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
-                x0 = fmaxf(m0, fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2)));
-                x1 = fmaxf(m1, fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2)));
-                if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
-                    const float d0 = m0 == -INFINITY ? 0.0f : ex2(m0 - x0), d1 = m1 == -INFINITY ? 0.0f : ex2(m1 - x1);
-                    l0 *= d0;
-                    l1 *= d1;
-#pragma unroll
-                    for (int j = 0; j < DV / 8; ++j) o[j][0] *= d0, o[j][1] *= d0, o[j][2] *= d1, o[j][3] *= d1;
-                    m0 = x0;
-                    m1 = x1;
-                }
-                const float r0 = P_BIAS - (m0 == -INFINITY ? 0.0f : m0), r1 = P_BIAS - (m1 == -INFINITY ? 0.0f : m1);
-                float w0 = 0.0f, w1 = 0.0f;
-                uint32_t pf[4][4];
-#pragma unroll
-                for (int ih = 0; ih < 8; ++ih) {
-                    const float a0 = ex2(sc[ih][0] + r0), a1 = ex2(sc[ih][1] + r0);
-                    const float b0 = ex2(sc[ih][2] + r1), b1 = ex2(sc[ih][3] + r1);
-                    w0 += a0 + a1;
-                    w1 += b0 + b1;
-                    pf[ih >> 1][2 * (ih & 1)] = half2_bits(a0, a1);
-                    pf[ih >> 1][2 * (ih & 1) + 1] = half2_bits(b0, b1);
-                }
                 const float iv = __uint_as_float((254u - min(max(cur.vs, 1u), 253u)) << 23);   // 2^-vlog
-                l0 = fmaf(w0, iv, l0);
-                l1 = fmaf(w1, iv, l1);
-                const int live = cur.len - t0;   // tokens of the quad's block; what lies behind may be anything, NaN codes too
+                const int t0 = cur.tok + 16 * (r8 >> 1) + (r8 & 1);
+                const bool part = cur.tok + KV_PAGE > cur.len - cur.n + 1 || p.window > 0;   // some row does not see all
+                uint32_t pf[NT][4][2];
+#pragma unroll
+                for (int g8 = 0; g8 < NT; ++g8) {
+                    float x[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            float a = sc[g8][e][k] * (ks * c[g8][k & 1]) + vlog;
+                            if (part) {
+                                const int t = t0 + 4 * e + (k & 2);
+                                a = t >= lo[g8][k & 1] && t < hi[g8][k & 1] ? a : -INFINITY;
+                            }
+                            sc[g8][e][k] = a;
+                            x[k & 1] = fmaxf(x[k & 1], a);
+                        }
+#pragma unroll
+                    for (int s2 = 4; s2 < 32; s2 <<= 1) {
+                        x[0] = fmaxf(x[0], __shfl_xor_sync(0xffffffffu, x[0], s2));
+                        x[1] = fmaxf(x[1], __shfl_xor_sync(0xffffffffu, x[1], s2));
+                    }
+                    if (__any_sync(0xffffffffu, x[0] > m[g8][0] || x[1] > m[g8][1])) {
+                        float fall[2];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const float now = fmaxf(m[g8][k], x[k]);
+                            fall[k] = m[g8][k] == -INFINITY ? 1.0f : ex2(m[g8][k] - now);   // (nothing there yet, or NaN)
+                            l[g8][k] *= fall[k];
+                            m[g8][k] = now;
+                        }
+#pragma unroll
+                        for (int j = 0; j < DV / 16; ++j)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) o[g8][j][k] *= fall[k & 1];
+                    }
+                    const float ref[2] = {P_BIAS - (m[g8][0] == -INFINITY ? 0.0f : m[g8][0]), P_BIAS - (m[g8][1] == -INFINITY ? 0.0f : m[g8][1])};
+                    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float w[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            w[k] = ex2(sc[g8][e][k] + ref[k & 1]);
+                            sum[k & 1] += w[k];
+                        }
+                        pf[g8][e][0] = transposed(half2_bits(w[0], w[1]));
+                        pf[g8][e][1] = transposed(half2_bits(w[2], w[3]));
+                    }
+                    l[g8][0] = fmaf(sum[0], iv, l[g8][0]);
+                    l[g8][1] = fmaf(sum[1], iv, l[g8][1]);
+                }
+                // tokens of the quad's block; what lies behind the sequence's end may be anything, NaN codes too
+                const int live = cur.len - cur.tok - 16 * quad;
                 const bool tail = cur.tok + KV_PAGE > cur.len;
                 uint32_t keep[4];
 #pragma unroll
@@ -321,15 +348,18 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
                     keep[e] = k >= 4 ? 0xffffffffu : k <= 0 ? 0u : (1u << (8 * k)) - 1u;
                 }
 #pragma unroll
-                for (int j = 0; j < DV / 8; ++j) {
-                    const uint4 w4 = *reinterpret_cast<const uint4*>(V + (8 * j + n8) * KV_PAGE + quad * 16);
-                    uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+                for (int j = 0; j < DV / 16; ++j) {
+                    const uint4 x4 = *reinterpret_cast<const uint4*>(V + (16 * j + r8) * KV_PAGE + quad * 16);
+                    const uint4 y4 = *reinterpret_cast<const uint4*>(V + (16 * j + r8 + 8) * KV_PAGE + quad * 16);
+                    uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        if (tail) w[e] &= keep[e];
-                        uint32_t v0, v1;
-                        e4m3_halves(w[e], v0, v1);
-                        mma_f16(o[j], pf[e][0], pf[e][1], pf[e][2], pf[e][3], v0, v1);
+                        if (tail) x[e] &= keep[e], y[e] &= keep[e];
+                        uint32_t a0, a1, a2, a3;
+                        e4m3_halves(x[e], a0, a2);
+                        e4m3_halves(y[e], a1, a3);
+#pragma unroll
+                        for (int g8 = 0; g8 < NT; ++g8) mma_f16(o[g8][j], a0, a1, a2, a3, pf[g8][e][0], pf[g8][e][1]);
                     }
                 }
                 __syncwarp();   // every lane has read the stage
@@ -338,44 +368,42 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
             cur = nxt;
             if (next < end) nxt = issue(slot);
             if (done.last || at == end - 1) {
-                l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-                l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-                l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-                l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
                 const int rows = done.n * p.group;
-                if (whole && done.last) {
+                const bool out = whole && done.last;
+                // partial: slot 1 where the item begins here, slot 0 where it began in an earlier warp
+                const int R = p.part_rows;
+                float* dst = p.part + (static_cast<int64_t>(g) * 2 + (whole ? 1 : 0)) * part_floats(R, DV);
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const int r = n8 + 8 * half, tok = r / p.group;
-                        if (r < rows) {
-                            const float l = half ? l1 : l0, inv = l == 0.0f ? 0.0f : 1.0f / l;
-                            T* out = static_cast<T*>(p.out) +
-                                     ((static_cast<int64_t>(done.row0) + tok) * p.heads + done.h * p.group + (r - tok * p.group)) * DV +
-                                     2 * quad;
+                for (int g8 = 0; g8 < NT; ++g8)
 #pragma unroll
-                            for (int j = 0; j < DV / 8; ++j)
-                                *reinterpret_cast<uint32_t*>(out + 8 * j) =
-                                    two_bits<T>(o[j][2 * half] * inv, o[j][2 * half + 1] * inv);
-                        }
-                    }
-                } else {
-                    // partial: slot 1 where the item begins here, slot 0 where it began in an earlier warp
-                    const int R = p.part_rows;
-                    float* dst = p.part + (static_cast<int64_t>(g) * 2 + (whole ? 1 : 0)) * part_floats(R, DV);
+                    for (int x = 0; x < 2; ++x) {
+                        float sum = l[g8][x];
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const int r = n8 + 8 * half;
-                        if (r < rows) {
-                            if (quad == 0) {
-                                dst[r] = half ? m1 : m0;
-                                dst[R + r] = half ? l1 : l0;
+                        for (int s2 = 4; s2 < 32; s2 <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s2);
+                        const int r = 8 * g8 + 2 * quad + x, tok = r / p.group;
+                        if (r >= rows) continue;
+                        if (out) {
+                            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                            T* row = static_cast<T*>(p.out) +
+                                     ((static_cast<int64_t>(done.row0) + tok) * p.heads + done.h * p.group + (r - tok * p.group)) * DV + r8;
+#pragma unroll
+                            for (int j = 0; j < DV / 16; ++j) {
+                                row[16 * j] = one_of<T>(o[g8][j][x] * inv);
+                                row[16 * j + 8] = one_of<T>(o[g8][j][2 + x] * inv);
+                            }
+                        } else {
+                            if (r8 == 0) {
+                                dst[r] = m[g8][x];
+                                dst[R + r] = sum;
                             }
 #pragma unroll
-                            for (int j = 0; j < DV / 8; ++j)
-                                *reinterpret_cast<float2*>(dst + 2 * R + r * DV + 8 * j + 2 * quad) =
-                                    make_float2(o[j][2 * half], o[j][2 * half + 1]);
+                            for (int j = 0; j < DV / 16; ++j) {
+                                dst[2 * R + r * DV + r8 + 16 * j] = o[g8][j][x];
+                                dst[2 * R + r * DV + r8 + 16 * j + 8] = o[g8][j][2 + x];
+                            }
                         }
                     }
+                if (!out) {
                     if (whole) {
                         // last warp with a tile of the item: the one whose piece holds tile at + left
                         const int64_t last = at + done.left;
@@ -388,63 +416,41 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
     if (lane == 0) p.heads_of[g] = head;
 }
 
-// Joins the partial sums of the item that begins in piece blockIdx.x and ends in a later one; row blockIdx.y.
+// Joins the partial sums of the items that begin in one piece and end in a later one: a warp takes a row (of part_rows) of such
+// an item at a time, its lanes four dimensions each.
 template <int DV, typename T>
-__global__ void __launch_bounds__(COMBINE_THREADS) kv_combine_kernel(const AttendArgs p)
+__global__ void __launch_bounds__(COMBINE_THREADS) kv_combine_kernel(const AttendArgs p, int pieces)
 {
-    constexpr int GROUPS = COMBINE_THREADS / DV;
-    __shared__ float acc[GROUPS][DV], ls[GROUPS];
+    const int lane = threadIdx.x & 31, R = p.part_rows, step = part_floats(R, DV), warps = gridDim.x * (COMBINE_THREADS / 32);
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int g = blockIdx.x, r = blockIdx.y;
-    const int4 head = p.heads_of[g];
-    if (head.x < 0) return;
-    const KvSeq s = kv_seq(p.b, head.x, p.c.status);
-    if (r >= s.n * p.group) return;
-    const int R = p.part_rows, step = part_floats(R, DV);
-    const int d = threadIdx.x % DV, grp = threadIdx.x / DV;
-    // part k of the item: piece g, slot 1, then pieces g + 1 .. head.z, slot 0
-    const float* base = p.part + static_cast<int64_t>(g) * 2 * step;
-    const int parts = head.z - g + 1;
-    auto part = [&](int k) { return base + (k == 0 ? step : static_cast<int64_t>(k) * 2 * step); };
-    float m = -INFINITY;
-    for (int k = 0; k < parts; ++k) m = fmaxf(m, part(k)[r]);
-    const float ref = m == -INFINITY ? 0.0f : m;
-    float o = 0.0f, l = 0.0f;
-#pragma unroll 4
-    for (int k = grp; k < parts; k += GROUPS) {
-        const float* q = part(k);
-        const float w = ex2(q[r] - ref);
-        l = fmaf(q[R + r], w, l);
-        o = fmaf(q[2 * R + r * DV + d], w, o);
-    }
-    acc[grp][d] = o;
-    if (d == 0) ls[grp] = l;
-    __syncthreads();
-    if (grp == 0) {
-        l = o = 0.0f;
-#pragma unroll
-        for (int k = 0; k < GROUPS; ++k) {
-            l += ls[k];
-            o += acc[k][d];
-        }
+    for (int i = blockIdx.x * (COMBINE_THREADS / 32) + (threadIdx.x >> 5); i < pieces * R; i += warps) {
+        const int g = i / R, r = i - g * R;
+        const int4 head = p.heads_of[g];
+        if (head.x < 0) continue;
+        const KvSeq s = kv_seq(p.b, head.x, p.c.status);
+        if (r >= s.n * p.group) continue;
+        // part k of the item: piece g, slot 1, then pieces g + 1 .. head.z, slot 0
+        const float* base = p.part + static_cast<int64_t>(g) * 2 * step;
+        const int parts = head.z - g + 1;
+        auto part = [&](int k) { return base + (k == 0 ? step : static_cast<int64_t>(k) * 2 * step); };
         const int tok = r / p.group;
-        static_cast<T*>(p.out)[((static_cast<int64_t>(s.row0) + tok) * p.heads + head.y * p.group + (r - tok * p.group)) * DV + d] =
-            one_of<T>(l == 0.0f ? 0.0f : o / l);
+        join_parts<DV, T>(part, parts, r, R + r, 2 * R + r * DV,
+                          static_cast<T*>(p.out) + ((static_cast<int64_t>(s.row0) + tok) * p.heads + head.y * p.group + (r - tok * p.group)) * DV, lane);
     }
 }
 
-template <int DK, int DV, typename T> static cudaError_t decode_launch(const AttendArgs& p, int pieces, cudaStream_t st)
+template <int DK, int DV, typename T, int NT> static cudaError_t decode_launch(const AttendArgs& p, int pieces, cudaStream_t st)
 {
     using C = DecCfg<DK, DV>;
     static std::atomic<uint64_t> done{0};
-    cudaError_t e = allow_smem(reinterpret_cast<const void*>(&kv_decode_kernel<DK, DV, T>), C::SMEM, done);
+    cudaError_t e = allow_smem(reinterpret_cast<const void*>(&kv_decode_kernel<DK, DV, T, NT>), C::SMEM, done);
     if (e != cudaSuccess) return e;
-    kv_decode_kernel<DK, DV, T><<<pieces / C::W, C::W * 32, C::SMEM, st>>>(p);
+    kv_decode_kernel<DK, DV, T, NT><<<pieces / C::W, C::W * 32, C::SMEM, st>>>(p);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     // launched while the decode kernel runs; its blocks wait for that kernel's end before they read
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(pieces, p.part_rows);
+    cfg.gridDim = dim3(std::min(2 * num_sms(), (pieces * p.part_rows + COMBINE_THREADS / 32 - 1) / (COMBINE_THREADS / 32)));
     cfg.blockDim = dim3(COMBINE_THREADS);
     cfg.stream = st;
     cudaLaunchAttribute attr{};
@@ -452,14 +458,15 @@ template <int DK, int DV, typename T> static cudaError_t decode_launch(const Att
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv_combine_kernel<DV, T>, p);
+    return cudaLaunchKernelEx(&cfg, kv_combine_kernel<DV, T>, p, pieces);
 }
 
 template <typename T> static cudaError_t decode_typed(const AttendArgs& p, int pieces, cudaStream_t st)
 {
-    if (p.c.key_dim == 64) return decode_launch<64, 64, T>(p, pieces, st);
-    if (p.c.key_dim == 128) return decode_launch<128, 128, T>(p, pieces, st);
-    return decode_launch<192, 128, T>(p, pieces, st);
+    const bool one = p.part_rows <= 8;
+    if (p.c.key_dim == 64) return one ? decode_launch<64, 64, T, 1>(p, pieces, st) : decode_launch<64, 64, T, 2>(p, pieces, st);
+    if (p.c.key_dim == 128) return one ? decode_launch<128, 128, T, 1>(p, pieces, st) : decode_launch<128, 128, T, 2>(p, pieces, st);
+    return one ? decode_launch<192, 128, T, 1>(p, pieces, st) : decode_launch<192, 128, T, 2>(p, pieces, st);
 }
 
 }  // namespace eva

@@ -69,6 +69,41 @@ __device__ __forceinline__ float ex2(float x)
     return y;
 }
 
+// One row's output from its partial sums, by a warp: maximum at part(k)[im], sum at part(k)[is], output from part(k) + io.
+template <int DV, typename T, typename P>
+__device__ __forceinline__ void join_parts(const P& part, int parts, int im, int is, int64_t io, T* out, int lane)
+{
+    float m = -INFINITY;
+    for (int k = lane; k < parts; k += 32) m = fmaxf(m, part(k)[im]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    const int d = (lane * 4) % DV;
+    float o[4] = {}, l = 0.0f;
+    for (int k0 = 0; k0 < parts; k0 += 32) {
+        float w = 0.0f;
+        if (k0 + lane < parts) {
+            w = ex2(part(k0 + lane)[im] - ref);
+            l = fmaf(part(k0 + lane)[is], w, l);
+        }
+        const int n = min(32, parts - k0);
+#pragma unroll 8
+        for (int k = 0; k < n; ++k) {
+            const float wk = __shfl_sync(0xffffffffu, w, k);
+            const float2 v = *reinterpret_cast<const float2*>(part(k0 + k) + io + d), u = *reinterpret_cast<const float2*>(part(k0 + k) + io + d + 2);
+            o[0] = fmaf(v.x, wk, o[0]);
+            o[1] = fmaf(v.y, wk, o[1]);
+            o[2] = fmaf(u.x, wk, o[2]);
+            o[3] = fmaf(u.y, wk, o[3]);
+        }
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (lane * 4 < DV)
+        *reinterpret_cast<uint2*>(out + d) = make_uint2(two_bits<T>(o[0] * inv, o[1] * inv), two_bits<T>(o[2] * inv, o[3] * inv));
+}
+
 // Shared memory of a kernel above the default, set once per device (`done`: a bit each).
 inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done)
 {

@@ -897,36 +897,8 @@ __global__ void __launch_bounds__(COMBINE_THREADS) kv_prompt_combine(const Atten
     const int step = PR_ROWS * (DV + 2), parts = head.w - g + 1;
     const float* base = p.part + static_cast<int64_t>(g) * 2 * step;
     auto part = [&](int k) { return base + (k == 0 ? step : static_cast<int64_t>(k) * 2 * step); };
-    float m = -INFINITY;
-    for (int k = lane; k < parts; k += 32) m = fmaxf(m, part(k)[pr]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float ref = m == -INFINITY ? 0.0f : m;
-    const int d = (lane * 4) % DV;
-    float o[4] = {}, l = 0.0f;
-    for (int k0 = 0; k0 < parts; k0 += 32) {
-        float w = 0.0f;
-        if (k0 + lane < parts) {
-            w = ex2(part(k0 + lane)[pr] - ref);
-            l = fmaf(part(k0 + lane)[PR_ROWS + pr], w, l);
-        }
-        const int n = min(32, parts - k0);
-#pragma unroll 8
-        for (int k = 0; k < n; ++k) {
-            const float wk = __shfl_sync(0xffffffffu, w, k);
-            const float4 v = *reinterpret_cast<const float4*>(part(k0 + k) + 2 * PR_ROWS + static_cast<int64_t>(pr) * DV + d);
-            o[0] = fmaf(v.x, wk, o[0]);
-            o[1] = fmaf(v.y, wk, o[1]);
-            o[2] = fmaf(v.z, wk, o[2]);
-            o[3] = fmaf(v.w, wk, o[3]);
-        }
-    }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T* out = static_cast<T*>(p.out) + ((static_cast<int64_t>(s.row0) + tok) * p.heads + head.y * p.group + (r - tok * p.group)) * DV;
-    if (lane * 4 < DV)
-        *reinterpret_cast<uint2*>(out + d) = make_uint2(two_bits<T>(o[0] * inv, o[1] * inv), two_bits<T>(o[2] * inv, o[3] * inv));
+    join_parts<DV, T>(part, parts, pr, PR_ROWS + pr, 2 * PR_ROWS + static_cast<int64_t>(pr) * DV,
+                      static_cast<T*>(p.out) + ((static_cast<int64_t>(s.row0) + tok) * p.heads + head.y * p.group + (r - tok * p.group)) * DV, lane);
 }
 
 template <int DK, int DV, typename T> static cudaError_t prompt_launch(const AttendArgs& p, cudaStream_t st)
