@@ -70,9 +70,15 @@ __device__ __forceinline__ int dec_tiles(const KvSeq& s, int window, int* first)
 struct DecTile {   // what the consumer of a tile needs
     int b, h, n, row0, len, tok;     // tok: first token; -1: nothing to read
     bool first, last;                // of its item
-    int left;                        // tiles of the item after this one
+    int index, left;                 // tiles of the item before and after this one
     uint32_t ks, vs;                 // scale bytes of the block of the lane's scores (lane / 8)
 };
+
+struct alignas(16) DecRest {   // partial sums that a piece leaves of an item: its first (-1: none left) and last piece, rows, head
+    int first, last, row0, n, h;
+};
+
+constexpr size_t DEC_RECORD = 2 * sizeof(DecRest) + DEC_ROWS * sizeof(int);   // of a piece: its two rests and counters
 
 // NT: groups of eight rows
 template <int DK, int DV, typename T, int NT>
@@ -102,7 +108,8 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
     const int nw = static_cast<int>(min(static_cast<int64_t>(C::W * gridDim.x), total));   // pieces, none of them empty
     const int64_t begin = g < nw ? total * g / nw : 0;
     int64_t end = g < nw ? total * (g + 1) / nw : 0;
-    int4 head = make_int4(-1, 0, 0, 0);
+    DecRest lead{}, tail{};   // of an item that began before the piece, and of one that goes on behind it
+    lead.first = tail.first = -1;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (begin < end) {
         // the sequence, head and tile at `begin`
@@ -144,7 +151,7 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
 
         auto issue = [&](int slot) -> DecTile {
             DecTile t{};
-            t.b = b, t.h = h, t.n = s.n, t.row0 = s.row0, t.len = s.len, t.first = i == 0, t.left = tiles - 1 - i;
+            t.b = b, t.h = h, t.n = s.n, t.row0 = s.row0, t.len = s.len, t.first = i == 0, t.index = i, t.left = tiles - 1 - i;
             t.last = t.left == 0;
             t.tok = -1;
             if (s.len > 0) {
@@ -404,38 +411,66 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
                         }
                     }
                 if (!out) {
-                    if (whole) {
-                        // last warp with a tile of the item: the one whose piece holds tile at + left
-                        const int64_t last = at + done.left;
-                        head = make_int4(done.b, done.h, static_cast<int>(((last + 1) * nw - 1) / total), 0);
-                    }
+                    // the item's pieces: those that hold its first and its last tile
+                    DecRest& rest = whole ? tail : lead;
+                    rest.first = static_cast<int>(((at - done.index + 1) * nw - 1) / total);
+                    rest.last = static_cast<int>(((at + done.left + 1) * nw - 1) / total);
+                    rest.row0 = done.row0, rest.n = done.n, rest.h = done.h;
                 }
             }
         }
     }
-    if (lane == 0) p.heads_of[g] = head;
+    if (lane == 0) {
+        DecRest* to = reinterpret_cast<DecRest*>(p.heads_of) + 2 * g;
+        to[0] = lead;
+        to[1] = tail;
+    }
+    // counters of the joining kernel's groups
+    int* count = reinterpret_cast<int*>(reinterpret_cast<DecRest*>(p.heads_of) + 2 * C::W * gridDim.x) + g * DEC_ROWS;
+    if (lane < DEC_ROWS) count[lane] = 0;
 }
 
-// Joins the partial sums of the items that begin in one piece and end in a later one: a warp takes a row (of part_rows) of such
-// an item at a time, its lanes four dimensions each.
+// Joins the partial sums of the items that lie in several pieces. The parts of an item are joined in groups of eight by the warp of
+// the group's first piece (and row); where there are more groups, the one that is done last joins the groups, in their
+// order whichever that is, so that an item of a thousand pieces takes as long as three loads, not a hundred.
 template <int DV, typename T>
 __global__ void __launch_bounds__(COMBINE_THREADS) kv_combine_kernel(const AttendArgs p, int pieces)
 {
-    const int lane = threadIdx.x & 31, R = p.part_rows, step = part_floats(R, DV), warps = gridDim.x * (COMBINE_THREADS / 32);
+    const int lane = threadIdx.x & 31, R = p.part_rows, step = part_floats(R, DV);
+    const int64_t task = static_cast<int64_t>(blockIdx.x) * (COMBINE_THREADS / 32) + (threadIdx.x >> 5);
+    const int g = static_cast<int>(task / R), r = static_cast<int>(task - static_cast<int64_t>(g) * R);
+    if (g >= pieces) return;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int i = blockIdx.x * (COMBINE_THREADS / 32) + (threadIdx.x >> 5); i < pieces * R; i += warps) {
-        const int g = i / R, r = i - g * R;
-        const int4 head = p.heads_of[g];
-        if (head.x < 0) continue;
-        const KvSeq s = kv_seq(p.b, head.x, p.c.status);
-        if (r >= s.n * p.group) continue;
-        // part k of the item: piece g, slot 1, then pieces g + 1 .. head.z, slot 0
-        const float* base = p.part + static_cast<int64_t>(g) * 2 * step;
-        const int parts = head.z - g + 1;
+    const DecRest* rests = reinterpret_cast<const DecRest*>(p.heads_of);
+    int* counts = reinterpret_cast<int*>(reinterpret_cast<DecRest*>(p.heads_of) + 2 * pieces);
+    for (int slot = 0; slot < 2; ++slot) {
+        const DecRest rest = rests[2 * g + slot];
+        const int i = g - rest.first;   // this piece's part of the item
+        if (rest.first < 0 || i % 8 != 0 || r >= rest.n * p.group) continue;
+        // part k of the item: its first piece, slot 1, then the next pieces, slot 0
+        float* base = p.part + static_cast<int64_t>(rest.first) * 2 * step;
         auto part = [&](int k) { return base + (k == 0 ? step : static_cast<int64_t>(k) * 2 * step); };
-        const int tok = r / p.group;
-        join_parts<DV, T>(part, parts, r, R + r, 2 * R + r * DV,
-                          static_cast<T*>(p.out) + ((static_cast<int64_t>(s.row0) + tok) * p.heads + head.y * p.group + (r - tok * p.group)) * DV, lane);
+        const int parts = rest.last - rest.first + 1, groups = (parts + 7) / 8, tok = r / p.group;
+        T* out = static_cast<T*>(p.out) + ((static_cast<int64_t>(rest.row0) + tok) * p.heads + rest.h * p.group + (r - tok * p.group)) * DV;
+        float m, l, o[4];
+        join_parts<DV>([&](int k) { return part(i + k); }, min(8, parts - i), r, R + r, 2 * R + r * DV, lane, m, l, o);
+        if (groups > 1) {
+            float* own = part(i);   // no other warp reads this row of it
+            __syncwarp();
+            if (lane == 0) own[r] = m, own[R + r] = l;
+            if (lane * 4 < DV) {
+                *reinterpret_cast<float2*>(own + 2 * R + r * DV + lane * 4) = make_float2(o[0], o[1]);
+                *reinterpret_cast<float2*>(own + 2 * R + r * DV + lane * 4 + 2) = make_float2(o[2], o[3]);
+            }
+            __threadfence();
+            __syncwarp();
+            int before = 0;
+            if (lane == 0) before = atomicAdd(counts + rest.first * DEC_ROWS + r, 1);
+            if (__shfl_sync(0xffffffffu, before, 0) != groups - 1) continue;
+            __threadfence();
+            join_parts<DV>([&](int k) { return part(8 * k); }, groups, r, R + r, 2 * R + r * DV, lane, m, l, o);
+        }
+        put_row<DV, T>(out, l, o, lane);
     }
 }
 
@@ -448,17 +483,8 @@ template <int DK, int DV, typename T, int NT> static cudaError_t decode_launch(c
     kv_decode_kernel<DK, DV, T, NT><<<pieces / C::W, C::W * 32, C::SMEM, st>>>(p);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    // launched while the decode kernel runs; its blocks wait for that kernel's end before they read
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(std::min(2 * num_sms(), (pieces * p.part_rows + COMBINE_THREADS / 32 - 1) / (COMBINE_THREADS / 32)));
-    cfg.blockDim = dim3(COMBINE_THREADS);
-    cfg.stream = st;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv_combine_kernel<DV, T>, p, pieces);
+    const int64_t tasks = static_cast<int64_t>(pieces) * p.part_rows, each = COMBINE_THREADS / 32;
+    return launch_after(kv_combine_kernel<DV, T>, dim3(static_cast<unsigned>((tasks + each - 1) / each)), dim3(COMBINE_THREADS), st, p, pieces);
 }
 
 template <typename T> static cudaError_t decode_typed(const AttendArgs& p, int pieces, cudaStream_t st)
@@ -490,7 +516,7 @@ extern "C" size_t eva_kv_attend_workspace(const EvaKvCache* cache, const EvaKvBa
     const int64_t rows = shared_rows(*cache, *batch, heads);
     if (rows > DEC_ROWS) return prompt_workspace(cache->value_dim);
     const size_t pieces = static_cast<size_t>(num_sms()) * dec_warps(cache->key_dim, cache->value_dim);
-    return pieces * (sizeof(int4) + 2 * sizeof(float) * part_floats(static_cast<int>(rows), cache->value_dim));
+    return pieces * (DEC_RECORD + 2 * sizeof(float) * part_floats(static_cast<int>(rows), cache->value_dim));
 }
 
 extern "C" int eva_kv_attend(const EvaKvCache* cache, const EvaKvBatch* batch, const void* q, int32_t dtype, int32_t heads,
@@ -524,7 +550,7 @@ extern "C" int eva_kv_attend(const EvaKvCache* cache, const EvaKvBatch* batch, c
         const int pieces = num_sms() * dec_warps(cache->key_dim, cache->value_dim);
         p.part_rows = static_cast<int>(rows);
         p.heads_of = static_cast<int4*>(workspace);
-        p.part = reinterpret_cast<float*>(p.heads_of + pieces);
+        p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pieces * DEC_RECORD);
         e = dtype == EVA_DTYPE_BF16 ? decode_typed<__nv_bfloat16>(p, pieces, st) : decode_typed<__half>(p, pieces, st);
     } else {
         e = launch_prompt(p, workspace, dtype == EVA_DTYPE_BF16, st);

@@ -18,7 +18,7 @@ struct AttendArgs {
     int heads, group, window;
     float scale;           // times log2(e): the softmax's exponentials are powers of two
     int part_rows;         // rows of a partial sum
-    int4* heads_of;        // [pieces]: item that begins in a piece and goes on {sequence, head, last piece}, -1: none
+    int4* heads_of;        // [pieces]: what a piece leaves unfinished (each kernel's own record)
     float* part;           // [pieces][2] partial sums
 };
 
@@ -69,39 +69,53 @@ __device__ __forceinline__ float ex2(float x)
     return y;
 }
 
-// One row's output from its partial sums, by a warp: maximum at part(k)[im], sum at part(k)[is], output from part(k) + io.
-template <int DV, typename T, typename P>
-__device__ __forceinline__ void join_parts(const P& part, int parts, int im, int is, int64_t io, T* out, int lane)
+// Joins a row's partial sums, by a warp, eight at a time (their loads do not wait for one another): maximum at part(k)[im], sum at
+// part(k)[is], output from part(k) + io; every lane gets the joint maximum and sum, and of the output dimensions
+// 4 lane .. 4 lane + 3 (modulo DV).
+template <int DV, typename P>
+__device__ __forceinline__ void join_parts(const P& part, int parts, int im, int is, int64_t io, int lane, float& m, float& l, float (&o)[4])
 {
-    float m = -INFINITY;
-    for (int k = lane; k < parts; k += 32) m = fmaxf(m, part(k)[im]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float ref = m == -INFINITY ? 0.0f : m;
     const int d = (lane * 4) % DV;
-    float o[4] = {}, l = 0.0f;
-    for (int k0 = 0; k0 < parts; k0 += 32) {
-        float w = 0.0f;
-        if (k0 + lane < parts) {
-            w = ex2(part(k0 + lane)[im] - ref);
-            l = fmaf(part(k0 + lane)[is], w, l);
-        }
-        const int n = min(32, parts - k0);
-#pragma unroll 8
-        for (int k = 0; k < n; ++k) {
-            const float wk = __shfl_sync(0xffffffffu, w, k);
-            const float2 v = *reinterpret_cast<const float2*>(part(k0 + k) + io + d), u = *reinterpret_cast<const float2*>(part(k0 + k) + io + d + 2);
-            o[0] = fmaf(v.x, wk, o[0]);
-            o[1] = fmaf(v.y, wk, o[1]);
-            o[2] = fmaf(u.x, wk, o[2]);
-            o[3] = fmaf(u.y, wk, o[3]);
-        }
-    }
+    m = -INFINITY;
+    o[0] = o[1] = o[2] = o[3] = l = 0.0f;
+    for (int k0 = 0; k0 < parts; k0 += 8) {
+        float mk[8], lk[8];
+        float2 x[8], y[8];
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+        for (int k = 0; k < 8; ++k) {
+            const bool in = k0 + k < parts;
+            const float* q = part(in ? k0 + k : k0);
+            mk[k] = in ? q[im] : -INFINITY;
+            lk[k] = in ? q[is] : 0.0f;
+            x[k] = in ? *reinterpret_cast<const float2*>(q + io + d) : make_float2(0.0f, 0.0f);
+            y[k] = in ? *reinterpret_cast<const float2*>(q + io + d + 2) : make_float2(0.0f, 0.0f);
+        }
+        float now = m;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) now = fmaxf(now, mk[k]);
+        const float ref = now == -INFINITY ? 0.0f : now, fall = m == -INFINITY ? 1.0f : ex2(m - ref);   // (0, or NaN, so far)
+        l *= fall;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] *= fall;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float w = mk[k] == -INFINITY ? 1.0f : ex2(mk[k] - ref);   // (nothing, or NaN)
+            l = fmaf(lk[k], w, l);
+            o[0] = fmaf(x[k].x, w, o[0]);
+            o[1] = fmaf(x[k].y, w, o[1]);
+            o[2] = fmaf(y[k].x, w, o[2]);
+            o[3] = fmaf(y[k].y, w, o[3]);
+        }
+        m = now;
+    }
+}
+
+// The row's output from what join_parts gives.
+template <int DV, typename T> __device__ __forceinline__ void put_row(T* out, float l, const float (&o)[4], int lane)
+{
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (lane * 4 < DV)
-        *reinterpret_cast<uint2*>(out + d) = make_uint2(two_bits<T>(o[0] * inv, o[1] * inv), two_bits<T>(o[2] * inv, o[3] * inv));
+        *reinterpret_cast<uint2*>(out + lane * 4) = make_uint2(two_bits<T>(o[0] * inv, o[1] * inv), two_bits<T>(o[2] * inv, o[3] * inv));
 }
 
 // Shared memory of a kernel above the default, set once per device (`done`: a bit each).
@@ -114,6 +128,22 @@ inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
     return e;
+}
+
+// Launch while the kernel before it in the stream still runs; its blocks wait (griddepcontrol.wait) for that kernel's end.
+template <typename... A>
+inline cudaError_t launch_after(void (*kernel)(A...), dim3 grid, dim3 block, cudaStream_t st, A... args)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 // Many rows (kv_prompt.cu): workspace bytes for a value dimension, and the launch.

@@ -470,6 +470,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
         }
         if (lane == 0) place = w;
     }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -889,6 +890,7 @@ template <int DV, typename T>
 __global__ void __launch_bounds__(COMBINE_THREADS) kv_prompt_combine(const AttendArgs p)
 {
     const int g = blockIdx.x, lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int4 head = p.heads_of[g];
     if (head.x < 0) return;
     const KvSeq s = kv_seq(p.b, head.x, p.c.status);
@@ -897,8 +899,9 @@ __global__ void __launch_bounds__(COMBINE_THREADS) kv_prompt_combine(const Atten
     const int step = PR_ROWS * (DV + 2), parts = head.w - g + 1;
     const float* base = p.part + static_cast<int64_t>(g) * 2 * step;
     auto part = [&](int k) { return base + (k == 0 ? step : static_cast<int64_t>(k) * 2 * step); };
-    join_parts<DV, T>(part, parts, pr, PR_ROWS + pr, 2 * PR_ROWS + static_cast<int64_t>(pr) * DV,
-                      static_cast<T*>(p.out) + ((static_cast<int64_t>(s.row0) + tok) * p.heads + head.y * p.group + (r - tok * p.group)) * DV, lane);
+    float m, l, o[4];
+    join_parts<DV>(part, parts, pr, PR_ROWS + pr, 2 * PR_ROWS + static_cast<int64_t>(pr) * DV, lane, m, l, o);
+    put_row<DV, T>(static_cast<T*>(p.out) + ((static_cast<int64_t>(s.row0) + tok) * p.heads + head.y * p.group + (r - tok * p.group)) * DV, l, o, lane);
 }
 
 template <int DK, int DV, typename T> static cudaError_t prompt_launch(const AttendArgs& p, cudaStream_t st)
@@ -911,8 +914,7 @@ template <int DK, int DV, typename T> static cudaError_t prompt_launch(const Att
     kv_prompt_kernel<DK, DV, T><<<pieces, PR_WARPS * 32, C::SMEM, st>>>(p);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    kv_prompt_combine<DV, T><<<dim3(pieces, PR_ROWS / PR_COMBINE_ROWS), COMBINE_THREADS, 0, st>>>(p);
-    return cudaGetLastError();
+    return launch_after(kv_prompt_combine<DV, T>, dim3(pieces, PR_ROWS / PR_COMBINE_ROWS), dim3(COMBINE_THREADS), st, p);
 }
 
 size_t prompt_workspace(int dv)
