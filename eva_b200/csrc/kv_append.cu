@@ -1,10 +1,10 @@
 // Append to the paged 8-bit cache: rotation of the new keys, one power-of-two scale per 16 tokens and head, e4m3
 // codes, in one pass.
 //
-// A CTA owns one block (16 tokens of one sequence) and a warp one head at a time, whose rows stay in registers as they came
-// between the maximum and the rounding, so k and v are read once and the codes written once. The cosines and sines of the
-// block's tokens are computed once for all heads and kept in shared memory; a key is rotated twice, for the maximum and for the codes,
-// which costs less than the registers that would hold it. The scale 2^e, e = ceil(log2(amax / 448)), comes from the exponent and
+// A CTA owns one block (16 tokens of one sequence) and a warp one head at a time. It goes over the head's rows twice, for the
+// maximum and for the codes; the second time they come from L1 (6 KB of keys a warp), which keeps the registers free for more warps
+// (holding the rows, 128 to 255 registers, was 10 % to 20 % slower). The cosines and sines of the block's tokens are
+// computed once for all heads and kept in shared memory. The scale 2^e, e = ceil(log2(amax / 448)), comes from the exponent and
 // mantissa bits of amax, and dividing by it is exact, so the only roundings are the rotation's (32 bits) and the one to e4m3.
 // A block that already holds tokens keeps max(old e, new e); when that raises it, the older codes are multiplied by
 // 2^(old - new), exact until they reach e4m3's subnormals.
@@ -77,7 +77,7 @@ __device__ __forceinline__ int2 key_pair(const EvaRotary& r, int i)
 }
 
 template <typename T, int DK, int DV, int KEYS>
-__global__ void __launch_bounds__(APPEND_WARPS * 32) kv_append_kernel(const AppendArgs p)
+__global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv_append_kernel(const AppendArgs p)
 {
     constexpr int UNITS = DK / 4, KU = (UNITS + 31) / 32;   // four dimensions each; of a lane
     __shared__ float4 turn[KV_BLOCK][UNITS];                // of a token and unit: cosines of both pairs, sines of both
@@ -126,60 +126,52 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) kv_append_kernel(const Appe
     }
     for (int h = warp; h < p.c.kv_heads; h += nwarps) {
         const int64_t ph = static_cast<int64_t>(page) * p.c.kv_heads + h;
+        uint8_t* ks = static_cast<uint8_t*>(p.c.k_scale) + ph * KV_PAGE_BLOCKS + at / KV_BLOCK;
+        uint8_t* vs = static_cast<uint8_t*>(p.c.v_scale) + ph * KV_PAGE_BLOCKS + at / KV_BLOCK;
+        uint8_t* kc = static_cast<uint8_t*>(p.c.k) + (ph * KV_PAGE + at) * DK;
+        uint8_t* vc = static_cast<uint8_t*>(p.c.v) + ph * KV_PAGE * DV + at;
+        int kbyte = 0, vbyte = 0;   // the scales of the tokens that the block holds already
+        if (lo > 0) {
+            kbyte = min(max(static_cast<int>(*ks), 1), 253);
+            vbyte = min(max(static_cast<int>(*vs), 1), 253);
+        }
         const T* kp = static_cast<const T*>(p.k) + h * p.kh + tok0 * p.kt;
         const T* vp = static_cast<const T*>(p.v) + h * p.vh + tok0 * p.vt + 4 * lane;
-        // the raw rows: values of dimensions 4 lane .. 4 lane + 3; key units as (a0, a1), (b0, b1)
-        uint32_t v[KV_BLOCK][2], ka[KU][KV_BLOCK], kb[KU][KV_BLOCK];
-#pragma unroll
-        for (int r = 0; r < KV_BLOCK; ++r) {
-            const bool in = r >= lo && r < hi;
-            v[r][0] = v[r][1] = 0;
-            if (in && 4 * lane < DV) {
+        const bool vlane = 4 * lane < DV;
+        // raw elements of token r: values of dimensions 4 lane .. 4 lane + 3; a key unit as (a0, a1), (b0, b1)
+        auto values = [&](int r) {
+            uint2 w = make_uint2(0, 0);
+            if (vlane) {
                 if constexpr (KEYS != KEYS_SINGLE) {
-                    const uint2 w = *reinterpret_cast<const uint2*>(vp + r * p.vt);
-                    v[r][0] = w.x;
-                    v[r][1] = w.y;
+                    w = *reinterpret_cast<const uint2*>(vp + r * p.vt);
                 } else {
                     const uint16_t* q = reinterpret_cast<const uint16_t*>(vp + r * p.vt);
-                    v[r][0] = q[0] | static_cast<uint32_t>(q[1]) << 16;
-                    v[r][1] = q[2] | static_cast<uint32_t>(q[3]) << 16;
+                    w = make_uint2(q[0] | static_cast<uint32_t>(q[1]) << 16, q[2] | static_cast<uint32_t>(q[3]) << 16);
                 }
             }
-#pragma unroll
-            for (int m = 0; m < KU; ++m) {
-                ka[m][r] = kb[m][r] = 0;
-                if (in && has[m]) {
-                    const uint16_t* q = reinterpret_cast<const uint16_t*>(kp + r * p.kt);
-                    if constexpr (KEYS == KEYS_QUADS) {   // a0 b0 a1 b1
-                        const uint2 w = *reinterpret_cast<const uint2*>(q + da[m][0]);
-                        ka[m][r] = __byte_perm(w.x, w.y, 0x5410);
-                        kb[m][r] = __byte_perm(w.x, w.y, 0x7632);
-                    } else if constexpr (KEYS == KEYS_HALVES) {
-                        // rotated: neighbours (a0, a1) and (b0, b1); else (a0, b0) and (a1, b1)
-                        const bool turned = 2 * (lane + 32 * m) < p.r.dim / 2;
-                        const uint32_t x = *reinterpret_cast<const uint32_t*>(q + da[m][0]);
-                        const uint32_t y = *reinterpret_cast<const uint32_t*>(q + (turned ? db[m][0] : da[m][1]));
-                        ka[m][r] = turned ? x : __byte_perm(x, y, 0x5410);
-                        kb[m][r] = turned ? y : __byte_perm(x, y, 0x7632);
-                    } else {
-                        ka[m][r] = q[da[m][0]] | static_cast<uint32_t>(q[da[m][1]]) << 16;
-                        kb[m][r] = q[db[m][0]] | static_cast<uint32_t>(q[db[m][1]]) << 16;
-                    }
+            return w;
+        };
+        auto keys = [&](int r, int m) {
+            uint2 w = make_uint2(0, 0);
+            if (has[m]) {
+                const uint16_t* q = reinterpret_cast<const uint16_t*>(kp + r * p.kt);
+                if constexpr (KEYS == KEYS_QUADS) {   // a0 b0 a1 b1
+                    const uint2 x = *reinterpret_cast<const uint2*>(q + da[m][0]);
+                    w = make_uint2(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632));
+                } else if constexpr (KEYS == KEYS_HALVES) {
+                    // rotated: neighbours (a0, a1) and (b0, b1); else (a0, b0) and (a1, b1)
+                    const bool turned = 2 * (lane + 32 * m) < p.r.dim / 2;
+                    const uint32_t x = *reinterpret_cast<const uint32_t*>(q + da[m][0]);
+                    const uint32_t y = *reinterpret_cast<const uint32_t*>(q + (turned ? db[m][0] : da[m][1]));
+                    w = turned ? make_uint2(x, y) : make_uint2(__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632));
+                } else {
+                    w = make_uint2(q[da[m][0]] | static_cast<uint32_t>(q[da[m][1]]) << 16, q[db[m][0]] | static_cast<uint32_t>(q[db[m][1]]) << 16);
                 }
             }
-        }
-        // largest magnitudes of the raw elements, as integers of 16 bits (NaN above infinity above all)
-        uint32_t vmax = 0, kraw = 0;
-#pragma unroll
-        for (int r = 0; r < KV_BLOCK; ++r) {
-            vmax = __vimax3_u16x2(vmax, v[r][0] & 0x7fff7fffu, v[r][1] & 0x7fff7fffu);
-#pragma unroll
-            for (int m = 0; m < KU; ++m) kraw = __vimax3_u16x2(kraw, ka[m][r] & 0x7fff7fffu, kb[m][r] & 0x7fff7fffu);
-        }
-        vmax = max(vmax & 0xffffu, vmax >> 16);
-        kraw = max(kraw & 0xffffu, kraw >> 16);
-        auto rotated = [&](int m, int r, float2& ya, float2& yb) {
-            const float2 a = up2<T>(ka[m][r]), c = up2<T>(kb[m][r]);
+            return w;
+        };
+        auto rotated = [&](uint2 w, int r, int m, float2& ya, float2& yb) {
+            const float2 a = up2<T>(w.x), c = up2<T>(w.y);
             ya = a;
             yb = c;
             if (rotates) {
@@ -189,121 +181,125 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) kv_append_kernel(const Appe
                 yb = fma2(a, sn, mul2(c, cs));
             }
         };
-        // A token with an element that is not finite has no key of its own, and does not count for the scale.
-        uint32_t bad = 0;
-        if (__any_sync(0xffffffffu, vmax >= INF_BITS<T> || kraw >= LOUD_BITS<T>)) {
-            vmax = 0;
-#pragma unroll 1
-            for (int r = lo; r < hi; ++r) {
-                bool odd = false;
-#pragma unroll
-                for (int x = 0; x < KV_BLOCK; ++x) {   // (registers have no index)
-                    if (x != r) continue;
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        uint32_t w = v[x][k];
-                        if ((w & 0x7fffu) >= INF_BITS<T>) w &= 0xffff0000u, odd = true;
-                        if ((w >> 16 & 0x7fffu) >= INF_BITS<T>) w &= 0xffffu, odd = true;
-                        v[x][k] = w;
-                        vmax = max(vmax, max(w & 0x7fffu, w >> 16 & 0x7fffu));
-                    }
-#pragma unroll
-                    for (int m = 0; m < KU; ++m) {
-                        float2 ya, yb;
-                        rotated(m, x, ya, yb);
-                        odd |= !finite(ya.x) || !finite(ya.y) || !finite(yb.x) || !finite(yb.y);
-                    }
-                }
-                if (__any_sync(0xffffffffu, odd)) bad |= 1u << r;
-            }
-        }
+        // largest magnitudes: of the raw elements as integers of 16 bits (NaN above infinity above all), of the rotated keys
+        uint32_t vmax = 0, raw = 0;
         float kmax = 0.0f;
-#pragma unroll
-        for (int r = 0; r < KV_BLOCK; ++r) {
-            if (bad >> r & 1 || r < lo || r >= hi) continue;
+#pragma unroll 4
+        for (int r = lo; r < hi; ++r) {
+            const uint2 v = values(r);
+            vmax = __vimax3_u16x2(vmax, v.x & 0x7fff7fffu, v.y & 0x7fff7fffu);
 #pragma unroll
             for (int m = 0; m < KU; ++m) {
+                const uint2 w = keys(r, m);
                 float2 ya, yb;
-                rotated(m, r, ya, yb);
+                rotated(w, r, m, ya, yb);
+                raw = __vimax3_u16x2(raw, w.x & 0x7fff7fffu, w.y & 0x7fff7fffu);
                 kmax = fmaxf(fmaxf(kmax, fmaxf(fabsf(ya.x), fabsf(ya.y))), fmaxf(fabsf(yb.x), fabsf(yb.y)));
             }
         }
-        vmax = __reduce_max_sync(0xffffffffu, vmax);
-        uint8_t* ks = static_cast<uint8_t*>(p.c.k_scale) + ph * KV_PAGE_BLOCKS + at / KV_BLOCK;
-        uint8_t* vs = static_cast<uint8_t*>(p.c.v_scale) + ph * KV_PAGE_BLOCKS + at / KV_BLOCK;
-        uint8_t* kc = static_cast<uint8_t*>(p.c.k) + (ph * KV_PAGE + at) * DK;
-        uint8_t* vc = static_cast<uint8_t*>(p.c.v) + ph * KV_PAGE * DV + at;
-        int ke = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(kmax)));
-        int ve = scale_byte(__float_as_uint(up2<T>(vmax).x));
-        float vmoved = 1.0f;
-        bool vgrown = false;
-        if (lo > 0) {
-            const int ko = min(max(static_cast<int>(*ks), 1), 253), vo = min(max(static_cast<int>(*vs), 1), 253);
-            ke = max(ke, ko);
-            ve = max(ve, vo);
-            vgrown = ve > vo;
-            vmoved = inv_scale(ve) * kv_scale(vo);
-            if (ke > ko) {   // the older keys: lo rows of DK bytes, contiguous
-                const float m = inv_scale(ke) * kv_scale(ko);
-                for (int i = lane; i < lo * DK / 2; i += 32) {
-                    uint16_t* q = reinterpret_cast<uint16_t*>(kc) + i;
-                    *q = static_cast<uint16_t>(e4m3_scaled(*q, m));
+        vmax = max(vmax & 0xffffu, vmax >> 16);
+        raw = max(raw & 0xffffu, raw >> 16);
+        // A token with an element that is not finite has no key of its own, and does not count for the key's scale; of its values the
+        // finite ones stay.
+        uint32_t bad = 0;
+        auto finite_only = [&](uint32_t w) {
+            if ((w & 0x7fffu) >= INF_BITS<T>) w &= 0xffff0000u;
+            if ((w >> 16 & 0x7fffu) >= INF_BITS<T>) w &= 0xffffu;
+            return w;
+        };
+        const bool odd = __any_sync(0xffffffffu, vmax >= INF_BITS<T> || raw >= LOUD_BITS<T>);
+        if (odd) {
+            vmax = 0;
+            kmax = 0.0f;
+#pragma unroll 1
+            for (int r = lo; r < hi; ++r) {
+                const uint2 v = values(r);
+                const uint32_t x = finite_only(v.x), y = finite_only(v.y);
+                bool strange = x != v.x || y != v.y;
+                float top = 0.0f;
+#pragma unroll
+                for (int m = 0; m < KU; ++m) {
+                    float2 ya, yb;
+                    rotated(keys(r, m), r, m, ya, yb);
+                    strange |= !finite(ya.x) || !finite(ya.y) || !finite(yb.x) || !finite(yb.y);
+                    top = fmaxf(fmaxf(top, fmaxf(fabsf(ya.x), fabsf(ya.y))), fmaxf(fabsf(yb.x), fabsf(yb.y)));
                 }
+                vmax = max(max(vmax, max(x & 0x7fffu, x >> 16 & 0x7fffu)), max(y & 0x7fffu, y >> 16 & 0x7fffu));
+                if (__any_sync(0xffffffffu, strange)) bad |= 1u << r;
+                else kmax = fmaxf(kmax, top);
             }
         }
+        const int ve = max(scale_byte(__float_as_uint(up2<T>(__reduce_max_sync(0xffffffffu, vmax)).x)), vbyte);
+        const int ke = max(scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(kmax))), kbyte);
         const float vinv = inv_scale(ve), kinv = inv_scale(ke);
-        if (4 * lane < DV) {
-            const bool merge = lo > 0 || hi < KV_BLOCK;   // the block holds, or may hold, other tokens' bytes
+        if (lo > 0 && ke > kbyte) {   // the older keys: lo rows of DK bytes, contiguous
+            const float m = kinv * kv_scale(kbyte);
+            for (int i = lane; i < lo * DK / 2; i += 32) {
+                uint16_t* q = reinterpret_cast<uint16_t*>(kc) + i;
+                *q = static_cast<uint16_t>(e4m3_scaled(*q, m));
+            }
+        }
+        // values: 16 tokens of a dimension are 16 bytes
+        if (vlane) {
+            const bool grown = lo > 0 && ve > vbyte, merge = lo > 0 || hi < KV_BLOCK;   // the block holds, or may hold, others' bytes
+            const float moves = vinv * kv_scale(vbyte);
+            uint32_t in[4][4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                uint8_t* q = vc + static_cast<int64_t>(4 * lane + j) * KV_PAGE;
                 uint4 was = make_uint4(0, 0, 0, 0);
-                if (merge) was = *reinterpret_cast<const uint4*>(q);
-                uint32_t in[4] = {was.x, was.y, was.z, was.w};
+                if (merge) was = *reinterpret_cast<const uint4*>(vc + static_cast<int64_t>(4 * lane + j) * KV_PAGE);
+                in[j][0] = was.x, in[j][1] = was.y, in[j][2] = was.z, in[j][3] = was.w;
+            }
 #pragma unroll
-                for (int t = 0; t < 8; ++t) {   // tokens 2 t, 2 t + 1
-                    const float2 x = up2<T>(v[2 * t][j / 2]), y = up2<T>(v[2 * t + 1][j / 2]);
+            for (int t = 0; t < 8; ++t) {   // tokens 2 t, 2 t + 1
+                const bool fresh0 = 2 * t >= lo && 2 * t < hi, fresh1 = 2 * t + 1 >= lo && 2 * t + 1 < hi;
+                if (merge && !fresh0 && !fresh1 && !(grown && 2 * t < lo)) continue;
+                uint2 v0 = fresh0 ? values(2 * t) : make_uint2(0, 0), v1 = fresh1 ? values(2 * t + 1) : make_uint2(0, 0);
+                if (odd) {
+                    v0 = make_uint2(finite_only(v0.x), finite_only(v0.y));
+                    v1 = make_uint2(finite_only(v1.x), finite_only(v1.y));
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 x = up2<T>(j < 2 ? v0.x : v0.y), y = up2<T>(j < 2 ? v1.x : v1.y);
                     uint32_t two = e4m3x2((j % 2 ? x.y : x.x) * vinv, (j % 2 ? y.y : y.x) * vinv);
                     if (merge) {
-                        const uint32_t old = in[t / 2] >> (t % 2 * 16) & 0xffffu;
-                        const uint32_t moved = vgrown ? e4m3_scaled(old, vmoved) : old;
-                        const uint32_t a = 2 * t < lo ? moved : 2 * t < hi ? two : old;
-                        const uint32_t c = 2 * t + 1 < lo ? moved : 2 * t + 1 < hi ? two : old;
+                        const uint32_t old = in[j][t / 2] >> (t % 2 * 16) & 0xffffu;
+                        const uint32_t moved = grown ? e4m3_scaled(old, moves) : old;
+                        const uint32_t a = 2 * t < lo ? moved : fresh0 ? two : old, c = 2 * t + 1 < lo ? moved : fresh1 ? two : old;
                         two = (a & 0xffu) | (c & 0xff00u);
                     }
-                    in[t / 2] = t % 2 ? (in[t / 2] & 0xffffu) | two << 16 : (in[t / 2] & 0xffff0000u) | two;
+                    in[j][t / 2] = t % 2 ? (in[j][t / 2] & 0xffffu) | two << 16 : (in[j][t / 2] & 0xffff0000u) | two;
                 }
-                *reinterpret_cast<uint4*>(q) = make_uint4(in[0], in[1], in[2], in[3]);
             }
-        }
 #pragma unroll
-        for (int r = 0; r < KV_BLOCK; ++r) {
-            if (r < lo || r >= hi) continue;
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<uint4*>(vc + static_cast<int64_t>(4 * lane + j) * KV_PAGE) = make_uint4(in[j][0], in[j][1], in[j][2], in[j][3]);
+        }
+#pragma unroll 4
+        for (int r = lo; r < hi; ++r) {
 #pragma unroll
             for (int m = 0; m < KU; ++m) {
                 float2 ya, yb;
-                rotated(m, r, ya, yb);
+                rotated(keys(r, m), r, m, ya, yb);
                 uint32_t x = e4m3x2(ya.x * kinv, ya.y * kinv), y = e4m3x2(yb.x * kinv, yb.y * kinv);   // (a0, a1), (b0, b1)
                 if (bad >> r & 1) x = y = 0x7f7fu;
                 if (!has[m]) continue;
                 uint8_t* q = kc + r * DK;
-                const bool neighbours = KEYS == KEYS_QUADS || (KEYS == KEYS_HALVES && 2 * (lane + 32 * m) >= p.r.dim / 2);
                 if constexpr (KEYS == KEYS_SINGLE) {
                     q[da[m][0]] = static_cast<uint8_t>(x);
                     q[da[m][1]] = static_cast<uint8_t>(x >> 8);
                     q[db[m][0]] = static_cast<uint8_t>(y);
                     q[db[m][1]] = static_cast<uint8_t>(y >> 8);
-                } else if (neighbours) {
+                } else {
                     const uint32_t w = __byte_perm(x, y, 0x5140);   // a0 b0 a1 b1
                     if constexpr (KEYS == KEYS_QUADS) {
                         *reinterpret_cast<uint32_t*>(q + da[m][0]) = w;
                     } else {
-                        *reinterpret_cast<uint16_t*>(q + da[m][0]) = static_cast<uint16_t>(w);
-                        *reinterpret_cast<uint16_t*>(q + da[m][1]) = static_cast<uint16_t>(w >> 16);
+                        const bool turned = 2 * (lane + 32 * m) < p.r.dim / 2;
+                        *reinterpret_cast<uint16_t*>(q + da[m][0]) = static_cast<uint16_t>(turned ? x : w);
+                        *reinterpret_cast<uint16_t*>(q + (turned ? db[m][0] : da[m][1])) = static_cast<uint16_t>(turned ? y : w >> 16);
                     }
-                } else {
-                    *reinterpret_cast<uint16_t*>(q + da[m][0]) = static_cast<uint16_t>(x);
-                    *reinterpret_cast<uint16_t*>(q + db[m][0]) = static_cast<uint16_t>(y);
                 }
             }
         }

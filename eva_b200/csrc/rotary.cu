@@ -14,13 +14,15 @@ namespace eva {
 
 constexpr int ROT_THREADS = 256;
 
+template <bool INTER> constexpr int ROT_HEADS = INTER ? 8 : 4;   // heads of a thread at most: eight units in flight
+
 struct RotArgs {
     const void* x;
     void* out;
     const void* pos;
     const uint64_t* turns;
     int64_t xt, xh, ot, oh;
-    int pos64, tokens, heads, head_dim, dim, offset, hc, nhc, units, copy;
+    int pos64, tokens, heads, head_dim, dim, offset, hc, nhc, units, copy, narrow;
     float mscale, sgn;
 };
 
@@ -43,60 +45,74 @@ template <typename T, int V, bool INTER>
 __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const RotArgs p)
 {
     using Vec = RotVec<T, V>;
-    constexpr int NP = INTER ? V / 2 : V;
+    constexpr int NP = INTER ? V / 2 : V, B = ROT_HEADS<INTER>;
+    // (token, group of heads, unit) of the thread; 32-bit divisions where they do
     const int64_t i = static_cast<int64_t>(blockIdx.x) * ROT_THREADS + threadIdx.x;
-    const int64_t row = i / p.units;
-    const int u = static_cast<int>(i - row * p.units);
-    const int64_t tok = row / p.nhc;
+    int64_t row, tok;
+    if (p.narrow) {
+        row = static_cast<uint32_t>(i) / static_cast<uint32_t>(p.units);
+        tok = static_cast<uint32_t>(row) / static_cast<uint32_t>(p.nhc);
+    } else {
+        row = i / p.units;
+        tok = row / p.nhc;
+    }
     if (tok >= p.tokens) return;
-    const int h0 = static_cast<int>(row - tok * p.nhc) * p.hc, h1 = min(p.heads, h0 + p.hc);
+    const int u = static_cast<int>(i - row * p.units), h0 = static_cast<int>(row - tok * p.nhc) * p.hc, h1 = min(p.heads, h0 + p.hc);
     const T* x = static_cast<const T*>(p.x) + tok * p.xt;
     T* o = static_cast<T*>(p.out) + tok * p.ot;
     const int pre = p.copy ? p.offset / V : 0, nrot = (INTER ? p.dim : p.dim / 2) / V;
-    if (u < pre || u >= pre + nrot) {
-        const int d = u < pre ? u * V : p.offset + p.dim + (u - pre - nrot) * V;
-#pragma unroll 4
-        for (int h = h0; h < h1; ++h)
-            *reinterpret_cast<Vec*>(o + h * p.oh + d) = *reinterpret_cast<const Vec*>(x + h * p.xh + d);
-        return;
-    }
-    const int64_t pos = p.pos64 ? static_cast<const int64_t*>(p.pos)[tok] : static_cast<const int32_t*>(p.pos)[tok];
-    const int p0 = (u - pre) * NP;
-    float c[NP], s[NP];
+    const bool turns = u >= pre && u < pre + nrot;
+    const int d = u < pre ? u * V : turns ? p.offset + (u - pre) * V : p.offset + p.dim + (u - pre - nrot) * V;
+    const int half = p.dim / 2;
+    // All of the thread's loads first, then its angles: a load is 1 us away, and so is the position. Copied and rotated units of a
+    // warp take one path, so that their loads are under way together, and a thread with all B heads has no branch between them
+    // (8192 x 32 heads of 192 dimensions, 64 rotated: 43 us; with a check of each head 76 us; torch copies as much in 35 us).
+    Vec a[B], b[INTER ? 1 : B];
+    const bool full = h1 - h0 == B;
+    auto load = [&](int k) {
+        a[k] = *reinterpret_cast<const Vec*>(x + (h0 + k) * p.xh + d);
+        if constexpr (!INTER)
+            if (turns) b[k] = *reinterpret_cast<const Vec*>(x + (h0 + k) * p.xh + d + half);
+    };
+    if (full) {
 #pragma unroll
-    for (int j = 0; j < NP; ++j) {
-        sincospif(kv_half_turns(pos, p.turns[p0 + j]), &s[j], &c[j]);
-        c[j] *= p.mscale;
-        s[j] *= p.sgn;
-    }
-    const int d = p.offset + (u - pre) * V;
-    if constexpr (INTER) {
-#pragma unroll 4
-        for (int h = h0; h < h1; ++h) {
-            Vec a = *reinterpret_cast<const Vec*>(x + h * p.xh + d);
-#pragma unroll
-            for (int j = 0; j < NP; ++j) {
-                const float e = rot_up(a.v[2 * j]), f = rot_up(a.v[2 * j + 1]);
-                a.v[2 * j] = rot_down<T>(e * c[j] - f * s[j]);
-                a.v[2 * j + 1] = rot_down<T>(f * c[j] + e * s[j]);
-            }
-            *reinterpret_cast<Vec*>(o + h * p.oh + d) = a;
-        }
+        for (int k = 0; k < B; ++k) load(k);
     } else {
-        const int half = p.dim / 2;
-#pragma unroll 4
-        for (int h = h0; h < h1; ++h) {
-            Vec a = *reinterpret_cast<const Vec*>(x + h * p.xh + d);
-            Vec b = *reinterpret_cast<const Vec*>(x + h * p.xh + d + half);
+#pragma unroll
+        for (int k = 0; k < B; ++k)
+            if (h0 + k < h1) load(k);
+    }
+    float c[NP], s[NP];
+    if (turns) {
+        const int64_t pos = p.pos64 ? static_cast<const int64_t*>(p.pos)[tok] : static_cast<const int32_t*>(p.pos)[tok];
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            sincospif(kv_half_turns(pos, p.turns[(u - pre) * NP + j]), &s[j], &c[j]);
+            c[j] *= p.mscale;
+            s[j] *= p.sgn;
+        }
+    }
+    auto store = [&](int k) {
+        if (turns) {
 #pragma unroll
             for (int j = 0; j < NP; ++j) {
-                const float e = rot_up(a.v[j]), f = rot_up(b.v[j]);
-                a.v[j] = rot_down<T>(e * c[j] - f * s[j]);
-                b.v[j] = rot_down<T>(f * c[j] + e * s[j]);
+                T& lo = INTER ? a[k].v[2 * j] : a[k].v[j];
+                T& hi = INTER ? a[k].v[2 * j + 1] : b[INTER ? 0 : k].v[j];
+                const float e = rot_up(lo), f = rot_up(hi);
+                lo = rot_down<T>(e * c[j] - f * s[j]);
+                hi = rot_down<T>(f * c[j] + e * s[j]);
             }
-            *reinterpret_cast<Vec*>(o + h * p.oh + d) = a;
-            *reinterpret_cast<Vec*>(o + h * p.oh + d + half) = b;
+            if constexpr (!INTER) *reinterpret_cast<Vec*>(o + (h0 + k) * p.oh + d + half) = b[k];
         }
+        *reinterpret_cast<Vec*>(o + (h0 + k) * p.oh + d) = a[k];
+    };
+    if (full) {
+#pragma unroll
+        for (int k = 0; k < B; ++k) store(k);
+    } else {
+#pragma unroll
+        for (int k = 0; k < B; ++k)
+            if (h0 + k < h1) store(k);
     }
 }
 
@@ -105,13 +121,14 @@ template <typename T, int V, bool INTER> static cudaError_t rotary_launch(RotArg
     const int nrot = (INTER ? p.dim : p.dim / 2) / V;
     p.units = nrot + (p.copy ? (p.head_dim - p.dim) / V : 0);
     if (p.units == 0) return cudaSuccess;
-    // Heads of one thread: as many as leave four warps for each SM's schedulers (their cosines are shared), 8 at most.
-    const int64_t all = static_cast<int64_t>(p.tokens) * p.heads * p.units;
-    p.hc = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min(8, p.heads), all / (num_sms() * 512))));
+    // Heads of one thread (they share its cosines): as many as leave 16 warps for each SM.
+    const int64_t all = static_cast<int64_t>(p.tokens) * p.heads * p.units, most = std::min(ROT_HEADS<INTER>, p.heads);
+    p.hc = static_cast<int>(std::max<int64_t>(1, std::min(most, all / (num_sms() * 512))));
     p.nhc = (p.heads + p.hc - 1) / p.hc;
     const int64_t threads = static_cast<int64_t>(p.tokens) * p.nhc * p.units;
     const int64_t grid = (threads + ROT_THREADS - 1) / ROT_THREADS;
     if (grid > 0x7fffffff) return cudaErrorInvalidValue;
+    p.narrow = grid * ROT_THREADS < int64_t{1} << 32;
     rotary_kernel<T, V, INTER><<<static_cast<unsigned>(grid), ROT_THREADS, 0, st>>>(p);
     return cudaGetLastError();
 }
