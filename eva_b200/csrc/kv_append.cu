@@ -111,19 +111,21 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv_append_kernel(const A
         }
         __syncthreads();
     }
-    int da[KU][2], db[KU][2];   // KEYS_SINGLE: the unit's dimensions; else da[.][0], db[.][0] begin its two neighbours
+    // The lane's units; lanes with none repeat the last one, which changes no maximum and spares the loads a branch, and do not store.
+    int unit[KU], da[KU][2], db[KU][2];   // KEYS_SINGLE: the unit's dimensions; else da[.][0], db[.][0] begin its two neighbours
     bool has[KU];
 #pragma unroll
     for (int m = 0; m < KU; ++m) {
-        const int u = lane + 32 * m;
-        has[m] = u < UNITS;
+        has[m] = lane + 32 * m < UNITS;
+        unit[m] = min(lane + 32 * m, UNITS - 1);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const int2 d = key_pair(p.r, min(2 * u + k, DK / 2 - 1));
+            const int2 d = key_pair(p.r, 2 * unit[m] + k);
             da[m][k] = d.x;
             db[m][k] = d.y;
         }
     }
+    const bool vlane = 4 * lane < DV;
     for (int h = warp; h < p.c.kv_heads; h += nwarps) {
         const int64_t ph = static_cast<int64_t>(page) * p.c.kv_heads + h;
         uint8_t* ks = static_cast<uint8_t*>(p.c.k_scale) + ph * KV_PAGE_BLOCKS + at / KV_BLOCK;
@@ -136,46 +138,37 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv_append_kernel(const A
             vbyte = min(max(static_cast<int>(*vs), 1), 253);
         }
         const T* kp = static_cast<const T*>(p.k) + h * p.kh + tok0 * p.kt;
-        const T* vp = static_cast<const T*>(p.v) + h * p.vh + tok0 * p.vt + 4 * lane;
-        const bool vlane = 4 * lane < DV;
+        const T* vp = static_cast<const T*>(p.v) + h * p.vh + tok0 * p.vt + (vlane ? 4 * lane : 0);
         // raw elements of token r: values of dimensions 4 lane .. 4 lane + 3; a key unit as (a0, a1), (b0, b1)
         auto values = [&](int r) {
-            uint2 w = make_uint2(0, 0);
-            if (vlane) {
-                if constexpr (KEYS != KEYS_SINGLE) {
-                    w = *reinterpret_cast<const uint2*>(vp + r * p.vt);
-                } else {
-                    const uint16_t* q = reinterpret_cast<const uint16_t*>(vp + r * p.vt);
-                    w = make_uint2(q[0] | static_cast<uint32_t>(q[1]) << 16, q[2] | static_cast<uint32_t>(q[3]) << 16);
-                }
+            if constexpr (KEYS != KEYS_SINGLE) {
+                return *reinterpret_cast<const uint2*>(vp + r * p.vt);
+            } else {
+                const uint16_t* q = reinterpret_cast<const uint16_t*>(vp + r * p.vt);
+                return make_uint2(q[0] | static_cast<uint32_t>(q[1]) << 16, q[2] | static_cast<uint32_t>(q[3]) << 16);
             }
-            return w;
         };
         auto keys = [&](int r, int m) {
-            uint2 w = make_uint2(0, 0);
-            if (has[m]) {
-                const uint16_t* q = reinterpret_cast<const uint16_t*>(kp + r * p.kt);
-                if constexpr (KEYS == KEYS_QUADS) {   // a0 b0 a1 b1
-                    const uint2 x = *reinterpret_cast<const uint2*>(q + da[m][0]);
-                    w = make_uint2(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632));
-                } else if constexpr (KEYS == KEYS_HALVES) {
-                    // rotated: neighbours (a0, a1) and (b0, b1); else (a0, b0) and (a1, b1)
-                    const bool turned = 2 * (lane + 32 * m) < p.r.dim / 2;
-                    const uint32_t x = *reinterpret_cast<const uint32_t*>(q + da[m][0]);
-                    const uint32_t y = *reinterpret_cast<const uint32_t*>(q + (turned ? db[m][0] : da[m][1]));
-                    w = turned ? make_uint2(x, y) : make_uint2(__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632));
-                } else {
-                    w = make_uint2(q[da[m][0]] | static_cast<uint32_t>(q[da[m][1]]) << 16, q[db[m][0]] | static_cast<uint32_t>(q[db[m][1]]) << 16);
-                }
+            const uint16_t* q = reinterpret_cast<const uint16_t*>(kp + r * p.kt);
+            if constexpr (KEYS == KEYS_QUADS) {   // a0 b0 a1 b1
+                const uint2 x = *reinterpret_cast<const uint2*>(q + da[m][0]);
+                return make_uint2(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632));
+            } else if constexpr (KEYS == KEYS_HALVES) {
+                // rotated: neighbours (a0, a1) and (b0, b1); else (a0, b0) and (a1, b1)
+                const bool turned = 2 * unit[m] < p.r.dim / 2;
+                const uint32_t x = *reinterpret_cast<const uint32_t*>(q + da[m][0]);
+                const uint32_t y = *reinterpret_cast<const uint32_t*>(q + (turned ? db[m][0] : da[m][1]));
+                return turned ? make_uint2(x, y) : make_uint2(__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632));
+            } else {
+                return make_uint2(q[da[m][0]] | static_cast<uint32_t>(q[da[m][1]]) << 16, q[db[m][0]] | static_cast<uint32_t>(q[db[m][1]]) << 16);
             }
-            return w;
         };
         auto rotated = [&](uint2 w, int r, int m, float2& ya, float2& yb) {
             const float2 a = up2<T>(w.x), c = up2<T>(w.y);
             ya = a;
             yb = c;
             if (rotates) {
-                const float4 t = turn[r][has[m] ? lane + 32 * m : 0];
+                const float4 t = turn[r][unit[m]];
                 const float2 cs = make_float2(t.x, t.y), sn = make_float2(t.z, t.w);
                 ya = fma2(c, make_float2(-sn.x, -sn.y), mul2(a, cs));
                 yb = fma2(a, sn, mul2(c, cs));
@@ -296,7 +289,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv_append_kernel(const A
                     if constexpr (KEYS == KEYS_QUADS) {
                         *reinterpret_cast<uint32_t*>(q + da[m][0]) = w;
                     } else {
-                        const bool turned = 2 * (lane + 32 * m) < p.r.dim / 2;
+                        const bool turned = 2 * unit[m] < p.r.dim / 2;
                         *reinterpret_cast<uint16_t*>(q + da[m][0]) = static_cast<uint16_t>(turned ? x : w);
                         *reinterpret_cast<uint16_t*>(q + (turned ? db[m][0] : da[m][1])) = static_cast<uint16_t>(turned ? y : w >> 16);
                     }
