@@ -393,3 +393,59 @@ class PagedKVCache:
 
     def clear_status(self) -> None:
         self._status.zero_()
+
+
+class PagedAttention:
+    """The attention half of a layer: query, key and value projections, rotation, append, attention, output projection.
+
+    wqkv: BF16 [heads * key_dim + kv_heads * (key_dim + value_dim), hidden] (queries, keys, values, one below the other),
+    wo: BF16 [hidden, heads * value_dim]; the cache and the rotation are the layer's own (or shared, for the rotation). The
+    projections are plain matrix products; keys and values go to the cache as they lie in the projection's rows."""
+
+    def __init__(self, cache, wqkv, wo, heads, rotary=None, *, scale=None, window=0):
+        if not isinstance(cache, PagedKVCache):
+            raise ValueError("cache must be a PagedKVCache")
+        if type(heads) is not int or heads < 1 or heads % cache.kv_heads:
+            raise ValueError(f"heads must be a multiple of {cache.kv_heads}")
+        rows = heads * cache.key_dim + cache.kv_heads * (cache.key_dim + cache.value_dim)
+        for name, w, shape in (("wqkv", wqkv, (rows, None)), ("wo", wo, (None, heads * cache.value_dim))):
+            if (not isinstance(w, torch.Tensor) or w.dtype != _BF16 or w.ndim != 2 or w.device != cache.device
+                    or any(n is not None and n != m for n, m in zip(shape, w.shape))):
+                raise ValueError(f"{name} must be BF16 {['hidden' if n is None else n for n in shape]} on {cache.device}")
+        if wqkv.shape[1] != wo.shape[0]:
+            raise ValueError("wqkv and wo must have the same hidden size")
+        if rotary is not None and not isinstance(rotary, Rotary):
+            raise ValueError("rotary must be a Rotary")
+        self.cache, self.wqkv, self.wo, self.heads, self.rotary = cache, wqkv, wo, heads, rotary
+        self.scale, self.window, self.hidden = scale, window, wqkv.shape[1]
+
+    def forward(self, h, batch, positions, *, out_f32=None):
+        """h: BF16 [tokens, hidden], the batch's new tokens; positions: int32 or int64 [tokens], each token's place in its
+        sequence. Returns BF16 [tokens, hidden], in FP32 into out_f32 where that is given."""
+        c = self.cache
+        if h.ndim != 2 or h.shape[1] != self.hidden or h.dtype != _BF16 or h.device != c.device:
+            raise ValueError(f"h must be BF16 [tokens, {self.hidden}] on {c.device}")
+        rows = h @ self.wqkv.T
+        nq, nk = self.heads * c.key_dim, c.kv_heads * c.key_dim
+        q = rows[:, :nq].unflatten(1, (self.heads, c.key_dim))
+        k = rows[:, nq:nq + nk].unflatten(1, (c.kv_heads, c.key_dim))
+        v = rows[:, nq + nk:].unflatten(1, (c.kv_heads, c.value_dim))
+        if self.rotary is not None:
+            q = self.rotary.apply(q, positions, out=q)
+        c.append(k, v, batch, rotary=self.rotary)
+        y = c.attend(q, batch, scale=self.scale, window=self.window).flatten(1) @ self.wo.T
+        return y if out_f32 is None else out_f32.copy_(y)
+
+    __call__ = forward
+
+
+def make_attention(n_layers, hidden, heads, kv_heads, key_dim, value_dim, pages, *, rotary=None, device="cuda", seed=0, window=0):
+    """Synthetic attention halves (seeded weights, empty caches of `pages` pages)."""
+    g = torch.Generator().manual_seed(seed)
+
+    def weight(n, m):
+        return (torch.randn(n, m, generator=g) * m ** -0.5).to(_BF16).to(device)
+
+    rows = heads * key_dim + kv_heads * (key_dim + value_dim)
+    return [PagedAttention(PagedKVCache(pages, kv_heads, key_dim, value_dim, device=device), weight(rows, hidden),
+                           weight(hidden, heads * value_dim), heads, rotary, window=window) for _ in range(n_layers)]

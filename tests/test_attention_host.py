@@ -120,6 +120,35 @@ def test_entry_points_check_their_arguments_before_any_device_work():
     assert L.eva_kv_attend_workspace(r(_cache()), r(_batch()), 3) == 0
 
 
+@pytest.mark.parametrize("dk", [64, 128, 192])
+def test_append_moves_each_dimension_once_at_aligned_places(dk):
+    """The key kernel's units of two pairs (restated): every dimension in one unit, and where it moves two or four neighbours at
+    a time (pairs side by side, or halves of an even number of pairs) their first one is a multiple of as many."""
+    def pair(inter, dim, off, i):
+        if inter or dim == 0:
+            return 2 * i, 2 * i + 1
+        if i < dim // 2:
+            return off + i, off + i + dim // 2
+        d = 2 * (i - dim // 2)
+        e = d if d < off else d + dim
+        return e, e + 1
+
+    for inter in (False, True):
+        for dim in range(0, dk + 1, 2):
+            for off in range(0, dk - dim + 1, 2):
+                seen = []
+                for u in range(dk // 4):
+                    (a0, b0), (a1, b1) = pair(inter, dim, off, 2 * u), pair(inter, dim, off, 2 * u + 1)
+                    seen += [a0, b0, a1, b1]
+                    if inter or dim == 0:
+                        assert a0 % 4 == 0 and (b0, a1, b1) == (a0 + 1, a0 + 2, a0 + 3)
+                    elif dim % 4 == 0 and 2 * u < dim // 2:
+                        assert a0 % 2 == 0 and b0 % 2 == 0 and (a1, b1) == (a0 + 1, b0 + 1)
+                    elif dim % 4 == 0:
+                        assert a0 % 2 == 0 and a1 % 2 == 0 and (b0, b1) == (a0 + 1, a1 + 1)
+                assert sorted(seen) == list(range(dk))
+
+
 def test_oracle_scale_exponent():
     for amax, e in ((448.0, 0), (448.0001, 1), (1.75, -8), (1.0, -8), (0.0, -126), (3.0e38, 120), (1e-40, -126)):
         assert A.scale_exponent(amax) == e, amax

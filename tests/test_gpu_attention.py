@@ -483,6 +483,63 @@ def test_a_batch_that_does_not_fit_is_flagged_and_left_out(new, lens):
         s.cache.clear_status()
 
 
+def test_layer_stack_with_attention(oracle):
+    """MoEStack with attention halves, a prompt and then single tokens of two sequences, against the 64-bit forms layer by layer.
+    The oracle attends over the codes that the caches hold: a key or value that differs by a rounding may fall to the next
+    code, a whole step of e4m3, and the first token of a sequence carries that to its output with weight 1, so that no
+    bound of single elements holds without it (the append has its own tests). Each layer rounds to BF16 nine times (two norms, rows of the
+    projection, query, attention, its projection, the MoE's input, inner and output); a rounding moves a vector by at most 2^-9 of
+    its 2-norm, and two roundings of neighbours by 2^-8: 18 x 2^-8 over two layers."""
+    import numpy as np
+    from eva_b200 import config as C
+    from eva_b200.attention import make_attention
+    from eva_b200.experts import make_layer
+    from eva_b200.runner import EvaMoE
+    from eva_b200.stack import MoEStack, make_norms
+    cfg = C.MoEConfig("small", hidden=512, inter=256, n_experts=16, topk=4, router="sigmoid", n_group=4, topk_group=2,
+                      route_scale=2.5, norm_topk=True, shared_inter=384, bits=3, shared_bits=4)
+    L, H, heads, kvh, dk, dv = 2, cfg.hidden, 4, 2, 128, 128
+    hosts = [make_layer(cfg, "cpu", seed=50 + i) for i in range(L)]
+    r = Rotary(64, layout="interleaved", offset=64)
+    att = make_attention(L, H, heads, kvh, dk, dv, 6, rotary=r, seed=3)
+    norms, anorms = make_norms(L, H, DEV, seed=4), make_norms(L, H, DEV, seed=5)[:L]
+    stack = MoEStack([EvaMoE(h.to(DEV), max_rows=48) for h in hosts], norms, attention=att, attention_norms=anorms)
+    table = [[4, 1], [0, 3]]
+    g = torch.Generator().manual_seed(1)
+    f32 = lambda t: oracle.bf16_to_f32(t.contiguous().view(torch.int16).cpu().numpy().view(np.uint16))   # noqa: E731
+    b16 = lambda a: torch.from_numpy(np.asarray(a, np.float32)).to(BF16).double().numpy()   # noqa: E731
+    lens = [0, 0]
+    for new in ([30, 12], [1, 1], [1, 1]):
+        lens = [a + b for a, b in zip(lens, new)]
+        start = [0, new[0], sum(new)]
+        pos = torch.cat([torch.arange(n - m, n) for m, n in zip(new, lens)])
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)   # noqa: E731
+        x = torch.randn(start[-1], H, generator=g).to(BF16)
+        out = stack.forward(x.to(DEV), batch=PagedBatch(i32(start), i32(lens), i32(table), max(new)), positions=pos.to(DEV))
+        resid = f32(x).astype(np.float64)
+        for i in range(L):
+            h = b16(oracle.rmsnorm(resid.astype(np.float32), f32(anorms[i]), 1e-6))
+            rows = torch.from_numpy(b16(h @ f32(att[i].wqkv).astype(np.float64).T))
+            q = rows[:, :heads * dk]
+            q = A.rotate(q.unflatten(1, (heads, dk)), pos, r.inv_freq, 1.0, "interleaved", 64).to(BF16).double()
+            c = att[i].cache
+            host = {"k": c.k.cpu(), "v": c.v.cpu(), "ks": c.k_scale.cpu().view(torch.uint8).int() - 127,
+                    "vs": c.v_scale.cpu().view(torch.uint8).int() - 127}
+            o, _, _, _ = A.attend(host, q, start, lens, table, dk ** -0.5)
+            resid = resid + b16(b16(o.flatten(1).numpy()) @ f32(att[i].wo).astype(np.float64).T)
+            h = oracle.f32_to_bf16(oracle.rmsnorm(resid.astype(np.float32), f32(norms[i]), 1e-6))
+            resid = resid + oracle.layer_forward(h, hosts[i])[0]
+        ref = oracle.rmsnorm(resid.astype(np.float32), f32(norms[-1]), 1e-6)
+        got = f32(out)
+        err = float(np.linalg.norm(got - ref) / np.linalg.norm(ref))
+        assert err <= 18 * 2.0**-8, (new, err)
+    assert all(a.cache.status() == 0 for a in att)
+    with pytest.raises(ValueError):
+        stack.forward(x.to(DEV))
+    with pytest.raises(ValueError):
+        MoEStack(stack.layers, norms, attention=att)
+
+
 def test_refusals():
     s = Setup((64, 64), 2, [1, 1], [10, 20]).fill()
     q, k = s.rows(4, 64, BF16).to(DEV), s.rows(2, 64, BF16).to(DEV)
