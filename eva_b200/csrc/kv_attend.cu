@@ -24,7 +24,7 @@
 
 namespace eva {
 
-constexpr int DEC_ROWS = 16;
+constexpr int DEC_ROWS = 16, DEC_PIECE = 6;
 constexpr float P_BIAS = 14.0f;   // weights are at most 2^14
 
 template <int DK, int DV> struct DecCfg {
@@ -105,7 +105,9 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
     for (int i = 0; i < C::W; ++i) total += sums[i];
     total *= p.c.kv_heads;
     const int g = warp * gridDim.x + blockIdx.x;
-    const int nw = static_cast<int>(min(static_cast<int64_t>(C::W * gridDim.x), total));   // pieces, none of them empty
+    // Pieces, none of them empty; of DEC_PIECE tiles at least where that leaves one for each SM, since every piece that cuts an item
+    // leaves partial sums.
+    const int nw = static_cast<int>(min(min(static_cast<int64_t>(C::W * gridDim.x), total), max(static_cast<int64_t>(gridDim.x), total / DEC_PIECE)));
     const int64_t begin = g < nw ? total * g / nw : 0;
     int64_t end = g < nw ? total * (g + 1) / nw : 0;
     DecRest lead{}, tail{};   // of an item that began before the piece, and of one that goes on behind it
@@ -193,6 +195,14 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
         };
 
         uint32_t phase = 0;
+        // the first item's queries, 1 us away, while its first tiles are looked up
+        if (r8 < s.n * p.group) {
+            const int tok = r8 / p.group;
+            const T* q = static_cast<const T*>(p.q) + (static_cast<int64_t>(s.row0) + tok) * p.qt +
+                         (static_cast<int64_t>(h) * p.group + (r8 - tok * p.group)) * p.qh + quad * 16;
+#pragma unroll
+            for (int j = 0; j < DK / 64; ++j) asm volatile("prefetch.global.L1 [%0];" ::"l"(q + j * 64));
+        }
         DecTile cur{}, nxt{};
         if (next < end) cur = issue(0);
         if (next < end) nxt = issue(1);
