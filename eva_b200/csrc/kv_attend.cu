@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
                 const float ks = kv_scale(cur.ks), vlog = static_cast<float>(static_cast<int>(max(cur.vs, 1u)) - 127);
                 const float iv = __uint_as_float((254u - min(max(cur.vs, 1u), 253u)) << 23);   // 2^-vlog
                 const int t0 = cur.tok + 16 * (r8 >> 1) + (r8 & 1);
-                const bool part = cur.tok + KV_PAGE > cur.len - cur.n + 1 || p.window > 0;   // some row does not see all
+                const bool part = cur.tok + KV_PAGE > cur.len - cur.n + 1 || (p.window > 0 && cur.tok < cur.len - p.window);   // not for all rows
                 uint32_t pf[NT][4][2];
 #pragma unroll
                 for (int g8 = 0; g8 < NT; ++g8) {
