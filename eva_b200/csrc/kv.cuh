@@ -9,6 +9,31 @@ namespace eva {
 constexpr int KV_PAGE = EVA_KV_PAGE, KV_BLOCK = EVA_KV_BLOCK, KV_PAGE_BLOCKS = KV_PAGE / KV_BLOCK;
 constexpr int ST_BAD_BATCH = EVA_STATUS_BAD_BATCH;
 
+// The end of the kernel before this one in the stream (launch_after), and leave for the one behind to be launched.
+__device__ __forceinline__ void after_previous()
+{
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Launch while the kernel before it in the stream still runs: a kernel launched so begins with after_previous(), which waits for that
+// kernel's end and its writes. The four kernels of a decoding layer are a few us each, and their launches overlap this way.
+template <typename... A>
+inline cudaError_t launch_after(void (*kernel)(A...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Sequence b of a batch: its token rows row0 .. row0 + n - 1 are the positions ctx .. len - 1 (ctx may be
 // negative: rows without a token). A sequence whose numbers do not fit the batch has no rows and no tokens.
 struct KvSeq {

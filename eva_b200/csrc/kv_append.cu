@@ -77,11 +77,12 @@ __device__ __forceinline__ int2 key_pair(const EvaRotary& r, int i)
 }
 
 template <typename T, int DK, int DV, int KEYS>
-__global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv_append_kernel(const AppendArgs p)
+__global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv_append_kernel(AppendArgs p)
 {
     constexpr int UNITS = DK / 4, KU = (UNITS + 31) / 32;   // four dimensions each; of a lane
     __shared__ float4 turn[KV_BLOCK][UNITS];                // of a token and unit: cosines of both pairs, sines of both
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+    after_previous();
     const int b = blockIdx.x / p.blocks;
     const KvSeq s = kv_seq(p.b, b, p.c.status);
     const int first = max(s.ctx, 0);
@@ -304,12 +305,12 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv_append_kernel(const A
     }
 }
 
-template <typename T, int DK, int DV> static void append_launch(const AppendArgs& p, int keys, unsigned grid, cudaStream_t st)
+template <typename T, int DK, int DV> static cudaError_t append_launch(const AppendArgs& p, int keys, unsigned grid, cudaStream_t st)
 {
-    const int threads = 32 * (p.c.kv_heads < APPEND_WARPS ? p.c.kv_heads : APPEND_WARPS);
-    if (keys == KEYS_QUADS) kv_append_kernel<T, DK, DV, KEYS_QUADS><<<grid, threads, 0, st>>>(p);
-    else if (keys == KEYS_HALVES) kv_append_kernel<T, DK, DV, KEYS_HALVES><<<grid, threads, 0, st>>>(p);
-    else kv_append_kernel<T, DK, DV, KEYS_SINGLE><<<grid, threads, 0, st>>>(p);
+    const dim3 threads(32 * (p.c.kv_heads < APPEND_WARPS ? p.c.kv_heads : APPEND_WARPS));
+    if (keys == KEYS_QUADS) return launch_after(kv_append_kernel<T, DK, DV, KEYS_QUADS>, dim3(grid), threads, 0, st, p);
+    if (keys == KEYS_HALVES) return launch_after(kv_append_kernel<T, DK, DV, KEYS_HALVES>, dim3(grid), threads, 0, st, p);
+    return launch_after(kv_append_kernel<T, DK, DV, KEYS_SINGLE>, dim3(grid), threads, 0, st, p);
 }
 
 template <typename T> static cudaError_t append_typed(const AppendArgs& p, cudaStream_t st)
@@ -322,10 +323,9 @@ template <typename T> static cudaError_t append_typed(const AppendArgs& p, cudaS
     const bool quads = p.r.interleaved || p.r.dim == 0;
     const int keys = off % 8 != 0 ? KEYS_SINGLE : quads ? KEYS_QUADS : p.r.dim % 4 == 0 ? KEYS_HALVES : KEYS_SINGLE;
     const unsigned g = static_cast<unsigned>(grid);
-    if (p.c.key_dim == 64) append_launch<T, 64, 64>(p, keys, g, st);
-    else if (p.c.key_dim == 128) append_launch<T, 128, 128>(p, keys, g, st);
-    else append_launch<T, 192, 128>(p, keys, g, st);
-    return cudaGetLastError();
+    if (p.c.key_dim == 64) return append_launch<T, 64, 64>(p, keys, g, st);
+    if (p.c.key_dim == 128) return append_launch<T, 128, 128>(p, keys, g, st);
+    return append_launch<T, 192, 128>(p, keys, g, st);
 }
 
 bool kv_cache_ok(const EvaKvCache* c)

@@ -82,7 +82,7 @@ constexpr size_t DEC_RECORD = 2 * sizeof(DecRest) + DEC_ROWS * sizeof(int);   //
 
 // NT: groups of eight rows
 template <int DK, int DV, typename T, int NT>
-__global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(const AttendArgs p)
+__global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(AttendArgs p)
 {
     using C = DecCfg<DK, DV>;
     extern __shared__ uint8_t smem_raw[];
@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
         for (int i = 0; i < C::STAGES; ++i) mbar_init(&bars[warp][i], 1);
         fence_barrier_init();
     }
+    after_previous();
     // length of the line of work
     int mine = 0, at0;
     for (int b = threadIdx.x; b < p.b.seqs; b += C::W * 32) mine += dec_tiles(kv_seq(p.b, b, p.c.status), p.window, &at0);
@@ -112,7 +113,6 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
     int64_t end = g < nw ? total * (g + 1) / nw : 0;
     DecRest lead{}, tail{};   // of an item that began before the piece, and of one that goes on behind it
     lead.first = tail.first = -1;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (begin < end) {
         // the sequence, head and tile at `begin`
         int b = 0, h = 0, i = 0, tiles = 0, first = 0;
@@ -444,13 +444,13 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(co
 // the group's first piece (and row); where there are more groups, the one that is done last joins the groups, in their
 // order whichever that is, so that an item of a thousand pieces takes as long as three loads, not a hundred.
 template <int DV, typename T>
-__global__ void __launch_bounds__(COMBINE_THREADS) kv_combine_kernel(const AttendArgs p, int pieces)
+__global__ void __launch_bounds__(COMBINE_THREADS) kv_combine_kernel(AttendArgs p, int pieces)
 {
     const int lane = threadIdx.x & 31, R = p.part_rows, step = part_floats(R, DV);
     const int64_t task = static_cast<int64_t>(blockIdx.x) * (COMBINE_THREADS / 32) + (threadIdx.x >> 5);
     const int g = static_cast<int>(task / R), r = static_cast<int>(task - static_cast<int64_t>(g) * R);
     if (g >= pieces) return;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    after_previous();
     const DecRest* rests = reinterpret_cast<const DecRest*>(p.heads_of);
     int* counts = reinterpret_cast<int*>(reinterpret_cast<DecRest*>(p.heads_of) + 2 * pieces);
     for (int slot = 0; slot < 2; ++slot) {
@@ -484,17 +484,16 @@ __global__ void __launch_bounds__(COMBINE_THREADS) kv_combine_kernel(const Atten
     }
 }
 
-template <int DK, int DV, typename T, int NT> static cudaError_t decode_launch(const AttendArgs& p, int pieces, cudaStream_t st)
+template <int DK, int DV, typename T, int NT> static cudaError_t decode_launch(AttendArgs p, int pieces, cudaStream_t st)
 {
     using C = DecCfg<DK, DV>;
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_smem(reinterpret_cast<const void*>(&kv_decode_kernel<DK, DV, T, NT>), C::SMEM, done);
     if (e != cudaSuccess) return e;
-    kv_decode_kernel<DK, DV, T, NT><<<pieces / C::W, C::W * 32, C::SMEM, st>>>(p);
-    e = cudaGetLastError();
+    e = launch_after(kv_decode_kernel<DK, DV, T, NT>, dim3(pieces / C::W), dim3(C::W * 32), C::SMEM, st, p);
     if (e != cudaSuccess) return e;
     const int64_t tasks = static_cast<int64_t>(pieces) * p.part_rows, each = COMBINE_THREADS / 32;
-    return launch_after(kv_combine_kernel<DV, T>, dim3(static_cast<unsigned>((tasks + each - 1) / each)), dim3(COMBINE_THREADS), st, p, pieces);
+    return launch_after(kv_combine_kernel<DV, T>, dim3(static_cast<unsigned>((tasks + each - 1) / each)), dim3(COMBINE_THREADS), 0, st, p, pieces);
 }
 
 template <typename T> static cudaError_t decode_typed(const AttendArgs& p, int pieces, cudaStream_t st)

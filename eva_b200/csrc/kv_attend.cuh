@@ -130,22 +130,6 @@ inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_
     return e;
 }
 
-// Launch while the kernel before it in the stream still runs; its blocks wait (griddepcontrol.wait) for that kernel's end.
-template <typename... A>
-inline cudaError_t launch_after(void (*kernel)(A...), dim3 grid, dim3 block, cudaStream_t st, A... args)
-{
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.stream = st;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 // Many rows (kv_prompt.cu): workspace bytes for a value dimension, and the launch.
 size_t prompt_workspace(int dv);
 cudaError_t launch_prompt(AttendArgs p, void* workspace, bool bf16, cudaStream_t st);

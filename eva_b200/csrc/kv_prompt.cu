@@ -362,7 +362,7 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, uint4 v)
 __device__ __forceinline__ uint32_t sw128(int r, int u) { return static_cast<uint32_t>(r * 128 + ((u ^ (r & 7)) << 4)); }
 
 template <int DK, int DV, typename T>
-__global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const AttendArgs p)
+__global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs p)
 {
     using C = PrCfg<DK, DV>;
     extern __shared__ uint8_t smem_raw[];
@@ -411,6 +411,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
     if (warp == PR_MMA) tmem_alloc(&B.tmem, 512);
     for (int i = threadIdx.x; i < PR_SPANS; i += PR_WARPS * 32) spans[i] = 0;
     __syncthreads();
+    after_previous();
     // this CTA's piece of the line
     const int span = (p.b.seqs + PR_SPANS - 1) / PR_SPANS;
     for (int b = warp; b < p.b.seqs; b += PR_WARPS) {
@@ -470,7 +471,6 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(const Atten
         }
         if (lane == 0) place = w;
     }
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -887,10 +887,10 @@ constexpr int PR_COMBINE_ROWS = COMBINE_THREADS / 32;   // rows of a combining b
 
 // Joins the partial sums of the row block that begins in piece blockIdx.x and ends in a later one.
 template <int DV, typename T>
-__global__ void __launch_bounds__(COMBINE_THREADS) kv_prompt_combine(const AttendArgs p)
+__global__ void __launch_bounds__(COMBINE_THREADS) kv_prompt_combine(AttendArgs p)
 {
     const int g = blockIdx.x, lane = threadIdx.x & 31;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    after_previous();
     const int4 head = p.heads_of[g];
     if (head.x < 0) return;
     const KvSeq s = kv_seq(p.b, head.x, p.c.status);
@@ -904,17 +904,16 @@ __global__ void __launch_bounds__(COMBINE_THREADS) kv_prompt_combine(const Atten
     put_row<DV, T>(static_cast<T*>(p.out) + ((static_cast<int64_t>(s.row0) + tok) * p.heads + head.y * p.group + (r - tok * p.group)) * DV, l, o, lane);
 }
 
-template <int DK, int DV, typename T> static cudaError_t prompt_launch(const AttendArgs& p, cudaStream_t st)
+template <int DK, int DV, typename T> static cudaError_t prompt_launch(AttendArgs p, cudaStream_t st)
 {
     using C = PrCfg<DK, DV>;
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_smem(reinterpret_cast<const void*>(&kv_prompt_kernel<DK, DV, T>), C::SMEM, done);
     if (e != cudaSuccess) return e;
     const int pieces = num_sms();
-    kv_prompt_kernel<DK, DV, T><<<pieces, PR_WARPS * 32, C::SMEM, st>>>(p);
-    e = cudaGetLastError();
+    e = launch_after(kv_prompt_kernel<DK, DV, T>, dim3(pieces), dim3(PR_WARPS * 32), C::SMEM, st, p);
     if (e != cudaSuccess) return e;
-    return launch_after(kv_prompt_combine<DV, T>, dim3(pieces, PR_ROWS / PR_COMBINE_ROWS), dim3(COMBINE_THREADS), st, p);
+    return launch_after(kv_prompt_combine<DV, T>, dim3(pieces, PR_ROWS / PR_COMBINE_ROWS), dim3(COMBINE_THREADS), 0, st, p);
 }
 
 size_t prompt_workspace(int dv)

@@ -42,10 +42,11 @@ template <typename T, int V> struct alignas(sizeof(T) * V) RotVec {
 // Units of a head, V elements each (half layout: a rotated unit is V elements of each half):
 // [0, offset / V) copied, then the rotated ones, then the copied rest. V divides every part.
 template <typename T, int V, bool INTER>
-__global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const RotArgs p)
+__global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(RotArgs p)
 {
     using Vec = RotVec<T, V>;
     constexpr int NP = INTER ? V / 2 : V, B = ROT_HEADS<INTER>;
+    after_previous();
     // (token, group of heads, unit) of the thread; 32-bit divisions where they do
     const int64_t i = static_cast<int64_t>(blockIdx.x) * ROT_THREADS + threadIdx.x;
     int64_t row, tok;
@@ -129,8 +130,7 @@ template <typename T, int V, bool INTER> static cudaError_t rotary_launch(RotArg
     const int64_t grid = (threads + ROT_THREADS - 1) / ROT_THREADS;
     if (grid > 0x7fffffff) return cudaErrorInvalidValue;
     p.narrow = grid * ROT_THREADS < int64_t{1} << 32;
-    rotary_kernel<T, V, INTER><<<static_cast<unsigned>(grid), ROT_THREADS, 0, st>>>(p);
-    return cudaGetLastError();
+    return launch_after(rotary_kernel<T, V, INTER>, dim3(static_cast<unsigned>(grid)), dim3(ROT_THREADS), 0, st, p);
 }
 
 template <typename T> static cudaError_t rotary_typed(const RotArgs& p, bool inter, cudaStream_t st)
