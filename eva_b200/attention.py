@@ -111,6 +111,8 @@ class Rotary:
             out = torch.empty_like(x, memory_format=torch.contiguous_format)
         elif out is not x:
             src = self._check_out(x, src, out)
+        elif any(st == 0 and n > 1 for n, st in zip(x.shape, x.stride())):
+            raise ValueError("in place, x must not overlap itself")
         if tokens == 0:
             return out
         if src is None:
@@ -224,7 +226,8 @@ class PagedBatch:
     The tensors stay the caller's: a captured step is replayed with new contents in them (max_q and the table's width
     bound what they may hold). A padding sequence has length 0 (its rows come out zero, nothing is appended). What does
     not fit (page ids outside the cache, lengths beyond the table, rows out of order) sets STATUS_BAD_BATCH in the cache's
-    status and is left out. A page that two sequences of a batch append to is the caller's error: its contents are then undefined."""
+    status and is left out. A page that stands twice among those that one call appends to (of two sequences, or of one) is the
+    caller's error: its contents are then undefined."""
 
     def __init__(self, q_start, seq_lens, table, max_q):
         for name, t, nd in (("q_start", q_start, 1), ("seq_lens", seq_lens, 1), ("table", table, 2)):
@@ -256,6 +259,8 @@ class PagedBatch:
         if ref is None:
             if tokens > _INT32_MAX:
                 raise ValueError("too many token rows")
+            if tokens and self.seqs and not self.max_q:
+                raise ValueError("a batch with max_q 0 has no token rows")
             if len(self._refs) > 64:
                 self._refs.clear()
             c = self._c

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(At
     using C = DecCfg<DK, DV>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ alignas(8) uint64_t bars[C::W][C::STAGES];
-    __shared__ int sums[C::W];
+    __shared__ int64_t spans[C::W * 32];   // tiles of a head, by runs of sequences
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane & 3, r8 = lane >> 2;
     uint8_t* ring = smem_raw + ((128 - (smem_u32(smem_raw) & 127)) & 127) + warp * C::STAGES * C::STAGE;
     if (lane == 0) {
@@ -95,15 +95,18 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(At
         fence_barrier_init();
     }
     after_previous();
-    // length of the line of work
-    int mine = 0, at0;
-    for (int b = threadIdx.x; b < p.b.seqs; b += C::W * 32) mine += dec_tiles(kv_seq(p.b, b, p.c.status), p.window, &at0);
-    mine = __reduce_add_sync(0xffffffffu, mine);
-    if (lane == 0) sums[warp] = mine;
+    // length of the line of work: a thread sums a span of sequences
+    const int span = (p.b.seqs + C::W * 32 - 1) / (C::W * 32);
+    int at0;
+    int64_t mine = 0;
+    for (int b = threadIdx.x * span; b < min(p.b.seqs, static_cast<int>(threadIdx.x + 1) * span); ++b)
+        mine += dec_tiles(kv_seq(p.b, b, p.c.status), p.window, &at0);
+    spans[threadIdx.x] = mine;
     __syncthreads();
     int64_t total = 0;
+    for (int i = lane; i < C::W * 32; i += 32) total += spans[i];
 #pragma unroll
-    for (int i = 0; i < C::W; ++i) total += sums[i];
+    for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
     total *= p.c.kv_heads;
     const int g = warp * gridDim.x + blockIdx.x;
     // Pieces, none of them empty; of DEC_PIECE tiles at least where that leaves one for each SM, since every piece that cuts an item
@@ -118,28 +121,38 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(At
         int b = 0, h = 0, i = 0, tiles = 0, first = 0;
         KvSeq s{};
         {
-            int64_t before = 0;
+            int64_t rem = begin;
             bool found = false;
-            for (int b0 = 0; b0 < p.b.seqs; b0 += 32) {
-                int t = b0 + lane < p.b.seqs ? dec_tiles(kv_seq(p.b, b0 + lane, p.c.status), p.window, &at0) : 0, sum = t;
+            // the lane, of 32 that hold t (and so many heads of it), whose part of the line holds tile `rem`; -1 and the next tile
+            auto holder = [&](int64_t t, int64_t& own) {
+                int64_t sum = t;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int x = __shfl_up_sync(0xffffffffu, sum, o);
-                    if (lane >= o) sum += x;
+                for (int x = 1; x < 32; x <<= 1) {
+                    const int64_t y = __shfl_up_sync(0xffffffffu, sum, x);
+                    if (lane >= x) sum += y;
                 }
-                const uint32_t hit = __ballot_sync(0xffffffffu, before + static_cast<int64_t>(sum) * p.c.kv_heads > begin);
-                if (hit) {
-                    const int l = __ffs(hit) - 1;
+                const uint32_t hit = __ballot_sync(0xffffffffu, sum * p.c.kv_heads > rem);
+                const int l = hit ? __ffs(hit) - 1 : 31;
+                rem -= __shfl_sync(0xffffffffu, hit ? sum - t : sum, l) * p.c.kv_heads;
+                own = __shfl_sync(0xffffffffu, t, l);
+                return hit ? l : -1;
+            };
+            for (int i0 = 0; i0 < C::W * 32 && !found; i0 += 32) {
+                int64_t own;
+                int l = holder(spans[i0 + lane], own);
+                if (l < 0) continue;
+                const int b1 = min(p.b.seqs, (i0 + l + 1) * span);
+                for (int b0 = (i0 + l) * span; b0 < b1 && !found; b0 += 32) {
+                    const int t = b0 + lane < b1 ? dec_tiles(kv_seq(p.b, b0 + lane, p.c.status), p.window, &at0) : 0;
+                    l = holder(t, own);
+                    if (l < 0) continue;
+                    tiles = static_cast<int>(own);
                     b = b0 + l;
-                    const int64_t rem =
-                        begin - before - static_cast<int64_t>(__shfl_sync(0xffffffffu, sum - t, l)) * p.c.kv_heads;
-                    tiles = __shfl_sync(0xffffffffu, t, l);
                     h = static_cast<int>(rem / tiles);
                     i = static_cast<int>(rem - static_cast<int64_t>(h) * tiles);
                     found = true;
-                    break;
                 }
-                before += static_cast<int64_t>(__shfl_sync(0xffffffffu, sum, 31)) * p.c.kv_heads;
+                break;
             }
             if (found) {
                 s = kv_seq(p.b, b, p.c.status);

@@ -414,9 +414,18 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
     after_previous();
     // this CTA's piece of the line
     const int span = (p.b.seqs + PR_SPANS - 1) / PR_SPANS;
-    for (int b = warp; b < p.b.seqs; b += PR_WARPS) {
-        const int64_t u = pr_units(kv_seq(p.b, b, status), p.group, p.window);
-        if (lane == 0 && u > 0) atomicAdd(&spans[b / span], static_cast<unsigned long long>(u));
+    if (p.b.seqs < 64) {   // a warp for each sequence's row blocks, or a thread
+        for (int b = warp; b < p.b.seqs; b += PR_WARPS) {
+            const int64_t u = pr_units(kv_seq(p.b, b, status), p.group, p.window);
+            if (lane == 0 && u > 0) atomicAdd(&spans[b / span], static_cast<unsigned long long>(u));
+        }
+    } else {
+        for (int b = threadIdx.x; b < p.b.seqs; b += PR_WARPS * 32) {
+            const KvSeq s = kv_seq(p.b, b, status);
+            int64_t u = 0;
+            for (int qb = 0; qb < pr_blocks(s, p.group); ++qb) u += pr_item(s, p.group, p.window, qb).tiles + PR_BLOCK_COST;
+            if (u > 0) atomicAdd(&spans[b / span], static_cast<unsigned long long>(u));
+        }
     }
     __syncthreads();
     if (warp == 0) {

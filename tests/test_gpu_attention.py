@@ -367,6 +367,30 @@ def test_repeated_calls_give_the_same_bits():
             assert torch.equal(first, s.cache.attend(q, s.batch))
 
 
+@pytest.mark.parametrize("heads,seqs", [(2, 2500), (40, 300)])
+def test_attention_of_many_sequences(heads, seqs):
+    """More sequences than threads look through at once, some empty; two query heads (few rows) and forty (many)."""
+    g = torch.Generator().manual_seed(seqs)
+    lens = torch.randint(0, 40, (seqs,), generator=g).tolist()
+    lens[seqs // 2] = 700
+    new = [min(1, n) for n in lens]
+    s = Setup((64, 64), 1, new, lens, seed=1).fill()
+    q = s.rows(heads, 64, BF16, 2.0).to(DEV)
+    _check_attention(s, q, s.cache.attend(q, s.batch), 0.125)
+    assert s.cache.status() == 0
+
+
+def test_attention_of_one_long_sequence_and_head():
+    """One item in all the pieces of the GPU: their partial sums are joined in groups, and the groups."""
+    for heads, new in ((1, 1), (24, 1), (2, 60)):
+        n = 30000
+        s = Setup((64, 64), 1, [new], [n], seed=heads).fill()
+        q = s.rows(heads, 64, F16, 2.0).to(DEV)
+        out = s.cache.attend(q, s.batch)
+        _check_attention(s, q, out, 0.125)
+        assert torch.equal(out, s.cache.attend(q, s.batch))
+
+
 # ---- the three together, streams, graphs, refusals ------------------------------------------------------------
 
 @pytest.mark.parametrize("dims,layout", [((128, 128), "half"), ((192, 128), "interleaved")])
@@ -565,6 +589,8 @@ def test_refusals():
         lambda: r.apply(q, torch.zeros(2, dtype=torch.int64, device=DEV), out=q[:, :, :].transpose(0, 1)),
         lambda: r.apply(q.double(), torch.zeros(2, dtype=torch.int64, device=DEV)),
         lambda: r.apply(q, torch.zeros(2, dtype=torch.int64, device=DEV), out=q[:1].expand(2, 4, 64)),
+        lambda: (lambda e: r.apply(e, torch.zeros(2, dtype=torch.int64, device=DEV), out=e))(q[:1].expand(2, 4, 64)),
+        lambda: s.cache.attend(q, PagedBatch(s.batch.q_start, s.batch.seq_lens, s.batch.table, 0)),
     ]
     for i, f in enumerate(bad):
         with pytest.raises(ValueError):
