@@ -9,7 +9,8 @@
 The reference's attention (runtime/ds41/model.py:566-937 `Attention`) reads a 4-bit compressed cache through an index;
 this is plain causal attention, for layers of DeepSeek shape without that index. Everything runs on the caller's current
 CUDA stream and never synchronises the host, so it can be captured in a CUDA graph and replayed; outputs and
-workspaces come from torch's allocator for each call.
+workspaces come from torch's allocator for each call. No gradients are recorded (of the rotation, apply(inverse=True) is one):
+tensors that require them are refused unless gradients are off.
 """
 from __future__ import annotations
 
@@ -106,12 +107,14 @@ class Rotary:
         if (not isinstance(positions, torch.Tensor) or positions.ndim != 1 or positions.shape[0] != tokens
                 or positions.dtype not in (_I64, _I32) or positions.device != device or not positions.is_contiguous()):
             raise ValueError(f"positions must be contiguous int32 or int64 [{tokens}] on {device}")
+        if x.requires_grad:
+            _no_grad(x)
         src = x if tokens == 0 else self._movable(x, out is x)
         if out is None:
             out = torch.empty_like(x, memory_format=torch.contiguous_format)
         elif out is not x:
             src = self._check_out(x, src, out)
-        elif any(st == 0 and n > 1 for n, st in zip(x.shape, x.stride())):
+        elif _folded(x):
             raise ValueError("in place, x must not overlap itself")
         if tokens == 0:
             return out
@@ -137,7 +140,7 @@ class Rotary:
         _rows(out, "out", self.device, (x.dtype,), x.shape[1], x.shape[2])
         if out.shape[0] != x.shape[0]:
             raise ValueError("out must have x's shape")
-        if any(st == 0 and n > 1 for n, st in zip(out.shape, out.stride())):
+        if _folded(out):
             raise ValueError("out must not overlap itself")
         same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()   # the same memory: in place
         if not same and _overlap(x, out):
@@ -166,6 +169,22 @@ class Rotary:
 def _span(t):
     n = t.element_size()
     return t.data_ptr(), t.data_ptr() + n * (1 + sum((s - 1) * st for s, st in zip(t.shape, t.stride())))
+
+
+def _no_grad(*tensors):
+    """The operators record no gradients: a call that autograd would follow is refused, not answered without one."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise ValueError("the attention operators record no gradients: call them under torch.no_grad()")
+
+
+def _folded(t):
+    """Whether two elements of t may share memory."""
+    end = 0
+    for st, n in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1):
+        if st <= end:
+            return True
+        end += (n - 1) * st
+    return False
 
 
 def _overlap(a, b):
@@ -326,6 +345,8 @@ class PagedKVCache:
                 raise ValueError(f"rotary must be a Rotary on {device}")
             if rotary._end > self.key_dim:
                 raise ValueError(f"the rotation ends at {rotary._end}, keys have {self.key_dim} dimensions")
+        if k.requires_grad or v.requires_grad:
+            _no_grad(k, v)
         b = self._batch(batch, tokens)
         if k.stride(2) != 1:
             k = k.contiguous()
@@ -354,8 +375,10 @@ class PagedKVCache:
             raise ValueError("window must be a nonnegative int")
         if scale is None:
             scale = self._scale
-        elif not isinstance(scale, (int, float)) or not 0 <= scale <= 3e38:
+        elif not isinstance(scale, (int, float)) or not 0 <= scale <= 2e38:
             raise ValueError("scale must be a finite nonnegative number")
+        if q.requires_grad:
+            _no_grad(q)
         b = self._batch(batch, tokens)
         st, sh, sd = q.stride()
         if tokens == 1:

@@ -313,8 +313,8 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(At
                         }
                     }
                 }
-                const float ks = kv_scale(cur.ks), vlog = static_cast<float>(static_cast<int>(max(cur.vs, 1u)) - 127);
-                const float iv = __uint_as_float((254u - min(max(cur.vs, 1u), 253u)) << 23);   // 2^-vlog
+                const float ks = kv_scale(cur.ks);
+                const ValueScale vsc = value_scale(cur.vs);
                 const int t0 = cur.tok + 16 * (r8 >> 1) + (r8 & 1);
                 const bool part = cur.tok + KV_PAGE > cur.len - cur.n + 1 || (p.window > 0 && cur.tok < cur.len - p.window);   // not for all rows
                 uint32_t pf[NT][4][2];
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(At
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            float a = sc[g8][e][k] * (ks * c[g8][k & 1]) + vlog;
+                            float a = sc[g8][e][k] * (ks * c[g8][k & 1]) + vsc.e;
                             if (part) {
                                 const int t = t0 + 4 * e + (k & 2);
                                 a = t >= lo[g8][k & 1] && t < hi[g8][k & 1] ? a : -INFINITY;
@@ -362,11 +362,11 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(At
                             w[k] = ex2(sc[g8][e][k] + ref[k & 1]);
                             sum[k & 1] += w[k];
                         }
-                        pf[g8][e][0] = transposed(half2_bits(w[0], w[1]));
-                        pf[g8][e][1] = transposed(half2_bits(w[2], w[3]));
+                        pf[g8][e][0] = transposed(half2_bits(w[0] * vsc.less, w[1] * vsc.less));
+                        pf[g8][e][1] = transposed(half2_bits(w[2] * vsc.less, w[3] * vsc.less));
                     }
-                    l[g8][0] = fmaf(sum[0], iv, l[g8][0]);
-                    l[g8][1] = fmaf(sum[1], iv, l[g8][1]);
+                    l[g8][0] = fmaf(sum[0], vsc.inv, l[g8][0]);
+                    l[g8][1] = fmaf(sum[1], vsc.inv, l[g8][1]);
                 }
                 // tokens of the quad's block; what lies behind the sequence's end may be anything, NaN codes too
                 const int live = cur.len - cur.tok - 16 * quad;
@@ -546,7 +546,7 @@ extern "C" int eva_kv_attend(const EvaKvCache* cache, const EvaKvBatch* batch, c
                              size_t workspace_bytes, void* out, void* stream)
 {
     if (!attend_ok(cache, batch, heads) || (dtype != EVA_DTYPE_F16 && dtype != EVA_DTYPE_BF16) || window < 0 ||
-        !(scale >= 0.0f) || scale > 3.0e38f)
+        !(scale >= 0.0f) || scale > 2.0e38f)   // times log2(e) is finite
         return EVA_ERR_INVALID;
     if (batch->seqs == 0 || batch->tokens == 0 || batch->max_q == 0) return EVA_OK;
     if (!q || !out || !workspace ||
@@ -563,7 +563,7 @@ extern "C" int eva_kv_attend(const EvaKvCache* cache, const EvaKvBatch* batch, c
     p.qh = q_head_stride;
     p.heads = heads;
     p.group = heads / cache->kv_heads;
-    p.window = window;
+    p.window = window < (1 << 30) ? window : 0;   // the longest sequence: no window, and no sum of it passes 32 bits
     p.scale = scale * 1.4426950408889634f;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int64_t rows = shared_rows(*cache, *batch, heads);

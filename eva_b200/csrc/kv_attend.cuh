@@ -9,6 +9,23 @@ namespace eva {
 
 constexpr int COMBINE_THREADS = 512;
 
+// A block's value scale 2^e joins its tokens' exponents as max(e, VALUE_EXP_MIN); what is left of it, 1 but for blocks whose values are
+// all below 448 x 2^VALUE_EXP_MIN = 2^-39, is a factor of the rounded weights alone. So tokens with values of zero (e = -126) count in
+// the sum: with e itself their 2^-e passes 32 bits, or their weights vanish beside those of larger values. The sum holds
+// the tokens down to 2^-40 of the largest as long as no block has e above 35, values up to 2^43.
+constexpr int VALUE_EXP_MIN = -48;
+
+struct ValueScale {
+    float e, inv, less;   // exponent, 2^-e, factor of the weights
+};
+
+__device__ __forceinline__ ValueScale value_scale(uint32_t byte)
+{
+    const int own = static_cast<int>(min(max(byte, 1u), 253u)) - 127, e = max(own, VALUE_EXP_MIN);
+    return {static_cast<float>(e), __uint_as_float(static_cast<uint32_t>(127 - e) << 23),
+            __uint_as_float(static_cast<uint32_t>(127 + own - e) << 23)};
+}
+
 struct AttendArgs {
     EvaKvCache c;
     EvaKvBatch b;

@@ -274,8 +274,8 @@ __device__ __forceinline__ float pr_weights(uint32_t ts, const float4* sc, float
     return l;
 }
 
-// The same two for a step of which a row sees tokens lo .. hi - 1 only, or whose scores lie far from 0, where M must be rounded as
-// t is, else their difference is not small at the largest: 16 columns at a time, since this is seldom run and long code would
+// The same two for a step of which a row sees tokens lo .. hi - 1 only, that has a block of very small values (value_scale), or whose
+// scores lie far from 0, where M must be rounded as t is, else their difference is not small at the largest: 16 columns at a time, since this is seldom run and long code would
 // come from memory.
 __device__ __noinline__ float pr_max_masked(uint32_t ts, const float4* sc, float c, int lo, int hi)
 {
@@ -300,14 +300,14 @@ __device__ __noinline__ float pr_weights_masked(uint32_t ts, const float4* sc, f
         uint32_t r[16], w[8];
         tmem_ld32x32_x16(ts + 16 * x, r);
         const float4 f = sc[x];
-        const float fc = f.x * c;
+        const float fc = f.x * c, less = fabsf(f.w);
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
             const float a = 16 * x + i >= lo && 16 * x + i < hi ? ex2(fmaf(__uint_as_float(r[i]), fc, f.y) + ref) : 0.0f;
             const float b = 16 * x + i + 1 >= lo && 16 * x + i + 1 < hi ? ex2(fmaf(__uint_as_float(r[i + 1]), fc, f.y) + ref) : 0.0f;
             s += a + b;
-            w[i / 2] = half2_bits(a, b);
+            w[i / 2] = half2_bits(a * less, b * less);
         }
         l = fmaf(s, f.z, l);
         tmem_st32x32_x8(ts + 8 * x, w);
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
     using C = PrCfg<DK, DV>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ PrBars B;
-    __shared__ float4 scales[PR_SCALES][4];               // of a step's blocks: key scale, value exponent, 1 / value scale
+    __shared__ float4 scales[PR_SCALES][4];               // of a step's blocks: key scale, value exponent, 2^-exponent, -+ factor of the weights
     __shared__ PrPlace place;
     __shared__ PrSeg segs[PR_SEGS];
     __shared__ float qscale[2][PR_TILE];                  // of a row's query: its power of two times the call's scale
@@ -605,7 +605,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
                 if (m != now) l *= m == -INFINITY ? 1.0f : ex2(m - now);   // (a sum that is not 0 there is NaN, and stays it)
                 m = now;
                 const float ref = PR_BIAS - (m == -INFINITY ? 0.0f : m);
-                if (!part_seen && !__any_sync(0xffffffffu, m != -INFINITY && fabsf(m) > 4096.0f))
+                if (!part_seen && sc[0].w > 0.0f && !__any_sync(0xffffffffu, m != -INFINITY && fabsf(m) > 4096.0f))
                     l += pr_weights(ts, sc, c, ref);
                 else
                     l += pr_weights_masked(ts, sc, c, ref, lo - tok0, hi - tok0);
@@ -803,14 +803,14 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
                     }
                     const int page = __shfl_sync(0xffffffffu, pages, t - pages_at);
                     const int64_t ph = static_cast<int64_t>(max(page, 0)) * p.c.kv_heads + h;
-                    float4 mine = make_float4(1.0f, -INFINITY, 0.0f, 0.0f);   // no page: codes of zero and no weight
+                    float4 mine = make_float4(1.0f, -INFINITY, 0.0f, 1.0f);   // no page: codes of zero and no weight
                     if (lane < 4 && page >= 0) {
                         const uint32_t ks = static_cast<const uint8_t*>(p.c.k_scale)[ph * KV_PAGE_BLOCKS + lane];
                         const uint32_t vs = static_cast<const uint8_t*>(p.c.v_scale)[ph * KV_PAGE_BLOCKS + lane];
-                        const uint32_t ve = min(max(vs, 1u), 253u);
-                        mine = make_float4(kv_scale(ks), static_cast<float>(static_cast<int>(ve) - 127),
-                                           __uint_as_float((254u - ve) << 23), 0.0f);
+                        const ValueScale v = value_scale(vs);
+                        mine = make_float4(kv_scale(ks), v.e, v.inv, v.less);
                     }
+                    if (__any_sync(0xffffffffu, mine.w != 1.0f)) mine.w = -mine.w;   // a step with such a block: pr_weights_masked
                     wait_on(&B.rkempty[rs], par, status);
                     if (page < 0) {
                         for (int i = lane; i < C::RK / 16; i += 32) st_shared16(smem_u32(rawk) + rs * C::RK + i * 16, make_uint4(0, 0, 0, 0));

@@ -259,12 +259,12 @@ def test_append_extremes_of_the_range():
 
 # ---- attention ------------------------------------------------------------------------------------------------
 
-def _check_attention(s, q, out, scale, window=0, rows=None):
+def _check_attention(s, q, out, scale, window=0, lost=0.0):
     """Scores: key_dim products accumulated in 32 bits with truncation, 2^-23 of the sum of their sizes each at most; a query in
     8-bit parts drops 2^-18 of its largest element; weights rounded to 16 bits (2^-11) and the output to its type."""
     ref, mean_abs, size, loud = A.attend(s.host, q.cpu(), s.start, s.lens, s.table, scale, window)
     delta = q.shape[2] * 2.0**-23 * size + 2.0**-18 * loud + 2.0**-20
-    tol = torch.finfo(q.dtype).eps / 2 * ref.abs() + mean_abs * (2.0**-11 + 2 * delta) + torch.finfo(q.dtype).smallest_normal
+    tol = torch.finfo(q.dtype).eps / 2 * ref.abs() + mean_abs * (2.0**-11 + 2 * delta) + torch.finfo(q.dtype).smallest_normal + lost
     got = out.cpu().double()
     n = s.start[-1]
     err = (got - ref)[:n].abs()
@@ -315,6 +315,53 @@ def test_attention_of_very_large_and_small_queries(size, new, lens):
         ref, _, _, _ = A.attend(s.host, q.cpu(), s.start, s.lens, s.table, 0.125)
         # the largest score wins unless two lie within the scores' own error: bound by the values' range
         assert bool(out.isfinite().all()) and float((out.cpu().double() - ref).abs().median()) < 2.0**-8
+
+
+@pytest.mark.parametrize("new,lens", [([1, 1, 1], [64, 200, 1500]), ([100, 40], [100, 700])])
+@pytest.mark.parametrize("kind", ["first", "all", "blocks", "all but one", "tiny", "large"])
+def test_attention_over_values_of_zero_and_of_very_different_sizes(kind, new, lens):
+    """Tokens whose values are zero count in the softmax's sum all the same, wherever they lie. Of a block whose values are all below
+    448 * 2^-48 the weights may round to nothing: then a row is off by no more than that, 2^-39."""
+    dims = (64, 64)
+    s = Setup(dims, 1, new, lens, seed=len(kind)).fill()
+    v, e = s.host["v"].view(torch.uint8), s.host["vs"]
+    for table, n in zip(s.table, lens):
+        for i, page in enumerate(table):
+            for block in range(4):
+                at = 64 * i + 16 * block
+                if kind == "tiny":
+                    e[page, :, block] = (-126, -100, -60, -49, -48, -47, -8, -7)[(at // 16) % 8]
+                elif kind == "large":
+                    e[page, :, block] = (35, -30, 35, -126)[(at // 16) % 4]
+                elif (kind == "all" or (kind == "first" and at < 128) or (kind == "blocks" and at // 16 % 3 != 1)
+                      or (kind == "all but one" and at // 16 != n // 32)):
+                    v[page, :, :, 16 * block:16 * block + 16] = 0
+                    e[page, :, block] = -126
+    s.cache.v.view(torch.uint8).copy_(s.host["v"].view(torch.uint8))
+    s.cache.v_scale.view(torch.uint8).copy_(s.bytes_of("vs"))
+    for heads, size in ((2, 0.1), (24, 2.0)):
+        q = s.rows(heads, 64, BF16, size).to(DEV)
+        _check_attention(s, q, s.cache.attend(q, s.batch), 0.125, lost=2.0**-39)
+
+
+@pytest.mark.parametrize("new,lens", [([1, 3], [70, 200]), ([100, 3], [100, 200]), ([5], [2])])
+def test_attention_extremes_of_its_arguments(new, lens):
+    """A scale of zero (the mean of what a row sees), the longest window, queries of zero."""
+    s = Setup((64, 64), 2, new, lens, seed=1).fill()
+    q = s.rows(8, 64, BF16, 2.0).to(DEV)
+    _check_attention(s, q, s.cache.attend(q, s.batch, scale=0), 0.0)
+    _check_attention(s, q, s.cache.attend(q, s.batch, window=2**31 - 1), 0.125)
+    _check_attention(s, q, s.cache.attend(q, s.batch, window=2**30), 0.125)
+    q[::2] = 0
+    _check_attention(s, q, s.cache.attend(q, s.batch), 0.125)
+
+
+@pytest.mark.parametrize("heads", [17, 24, 64, 300])
+def test_attention_of_many_heads_of_one_key(heads):
+    """Single tokens whose query heads share one key and value are many rows of one sequence."""
+    s = Setup((192, 128), 1, [1, 1, 0, 1], [1, 300, 20, 65], seed=heads).fill()
+    q = s.rows(heads, 192, BF16, 2.0).to(DEV)
+    _check_attention(s, q, s.cache.attend(q, s.batch), 192 ** -0.5)
 
 
 def test_attention_keeps_rows_behind_the_last_sequence():
@@ -591,6 +638,11 @@ def test_refusals():
         lambda: r.apply(q, torch.zeros(2, dtype=torch.int64, device=DEV), out=q[:1].expand(2, 4, 64)),
         lambda: (lambda e: r.apply(e, torch.zeros(2, dtype=torch.int64, device=DEV), out=e))(q[:1].expand(2, 4, 64)),
         lambda: s.cache.attend(q, PagedBatch(s.batch.q_start, s.batch.seq_lens, s.batch.table, 0)),
+        lambda: (lambda e: r.apply(e, torch.zeros(2, dtype=torch.int64, device=DEV), out=e))(q.view(-1).unfold(0, 256, 32)[:2].unflatten(1, (4, 64))),
+        lambda: s.cache.attend(q, s.batch, scale=3e38),
+        lambda: r.apply(q.detach().requires_grad_(), torch.zeros(2, dtype=torch.int64, device=DEV)),
+        lambda: s.cache.attend(q.detach().requires_grad_(), s.batch),
+        lambda: s.cache.append(k, k.detach().requires_grad_(), s.batch),
     ]
     for i, f in enumerate(bad):
         with pytest.raises(ValueError):
