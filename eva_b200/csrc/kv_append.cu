@@ -8,7 +8,10 @@
 // mantissa bits of amax, and dividing by it is exact, so the only roundings are the rotation's (32 bits) and the one to e4m3.
 // A block that already holds tokens keeps max(old e, new e); when that raises it, the older codes are multiplied by
 // 2^(old - new), exact until they reach e4m3's subnormals.
+#include <type_traits>
+
 #include "kv.cuh"
+#include "kv_attend.cuh"
 
 #include <cuda_fp8.h>
 
@@ -76,12 +79,22 @@ __device__ __forceinline__ int2 key_pair(const EvaRotary& r, int i)
     return make_int2(e, e + 1);
 }
 
-template <typename T, int DK, int DV, int KEYS>
-__global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv_append_kernel(AppendArgs p)
+// STAGED: a warp's 16 rows of keys and of values come through shared memory.
+template <typename T, int DK, int DV, int KEYS, bool STAGED>
+__global__ void __launch_bounds__(APPEND_WARPS * 32, STAGED ? (DK == 64 ? 4 : DK == 128 ? 3 : 2) : 4) kv_append_kernel(AppendArgs p)
 {
+    extern __shared__ uint4 stage_raw[];
     constexpr int UNITS = DK / 4, KU = (UNITS + 31) / 32;   // four dimensions each; of a lane
+    __shared__ alignas(8) uint64_t bars[APPEND_WARPS];
     __shared__ float4 turn[KV_BLOCK][UNITS];                // of a token and unit: cosines of both pairs, sines of both
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+    if constexpr (STAGED) {
+        if (lane == 0) {
+            mbar_init(&bars[warp], 1);
+            fence_barrier_init();
+        }
+        __syncwarp();
+    }
     after_previous();
     const int b = blockIdx.x / p.blocks;
     const KvSeq s = kv_seq(p.b, b, p.c.status);
@@ -114,7 +127,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv_append_kernel(AppendA
     }
     // The lane's units; lanes with none repeat the last one, which changes no maximum and spares the loads a branch, and do not store.
     int unit[KU], da[KU][2], db[KU][2];   // KEYS_SINGLE: the unit's dimensions; else da[.][0], db[.][0] begin its two neighbours
-    bool has[KU];
+    bool has[KU], spins[KU];              // a unit of the warp is rotated
 #pragma unroll
     for (int m = 0; m < KU; ++m) {
         has[m] = lane + 32 * m < UNITS;
@@ -125,9 +138,16 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv_append_kernel(AppendA
             da[m][k] = d.x;
             db[m][k] = d.y;
         }
+        const int f = 2 * unit[m] - (p.r.interleaved ? p.r.offset / 2 : 0);   // frequency of its first pair
+        spins[m] = __any_sync(0xffffffffu, f + 1 >= 0 && f < p.r.dim / 2);
     }
     const bool vlane = 4 * lane < DV;
-    for (int h = warp; h < p.c.kv_heads; h += nwarps) {
+    const int slot0 = lo, slot1 = hi;
+    uint32_t phase = 0;
+    // WHOLE: the call fills the block, all loops are of 16
+    auto one_head = [&](auto whole, const int h) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        const int lo = WHOLE ? 0 : slot0, hi = WHOLE ? KV_BLOCK : slot1;
         const int64_t ph = static_cast<int64_t>(page) * p.c.kv_heads + h;
         uint8_t* ks = static_cast<uint8_t*>(p.c.k_scale) + ph * KV_PAGE_BLOCKS + at / KV_BLOCK;
         uint8_t* vs = static_cast<uint8_t*>(p.c.v_scale) + ph * KV_PAGE_BLOCKS + at / KV_BLOCK;
@@ -139,18 +159,36 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv_append_kernel(AppendA
             vbyte = min(max(static_cast<int>(*vs), 1), 253);
         }
         const T* kp = static_cast<const T*>(p.k) + h * p.kh + tok0 * p.kt;
-        const T* vp = static_cast<const T*>(p.v) + h * p.vh + tok0 * p.vt + (vlane ? 4 * lane : 0);
+        const T* vp = static_cast<const T*>(p.v) + h * p.vh + tok0 * p.vt;
+        if constexpr (STAGED) {
+            T* const ring = reinterpret_cast<T*>(stage_raw + warp * (KV_BLOCK * (DK + DV) / 8));
+            // a bulk copy for each row: lanes 0 .. 15 the keys, 16 .. 31 the values
+            __syncwarp();   // every lane is done with the head before
+            const int r = lane % KV_BLOCK;
+            if (lane == 0) mbar_arrive_expect_tx(&bars[warp], (hi - lo) * (DK + DV) * sizeof(T));
+            __syncwarp();
+            if (r >= lo && r < hi) {
+                if (lane < KV_BLOCK) bulk_g2s(ring + r * DK, kp + r * p.kt, DK * sizeof(T), &bars[warp]);
+                else bulk_g2s(ring + KV_BLOCK * DK + r * DV, vp + r * p.vt, DV * sizeof(T), &bars[warp]);
+            }
+            mbar_wait(&bars[warp], phase, p.c.status);
+            phase ^= 1;
+            kp = ring;
+            vp = ring + KV_BLOCK * DK;
+        }
+        if (vlane) vp += 4 * lane;
+        const int64_t kt = STAGED ? DK : p.kt, vt = STAGED ? DV : p.vt;
         // raw elements of token r: values of dimensions 4 lane .. 4 lane + 3; a key unit as (a0, a1), (b0, b1)
         auto values = [&](int r) {
             if constexpr (KEYS != KEYS_SINGLE) {
-                return *reinterpret_cast<const uint2*>(vp + r * p.vt);
+                return *reinterpret_cast<const uint2*>(vp + r * vt);
             } else {
-                const uint16_t* q = reinterpret_cast<const uint16_t*>(vp + r * p.vt);
+                const uint16_t* q = reinterpret_cast<const uint16_t*>(vp + r * vt);
                 return make_uint2(q[0] | static_cast<uint32_t>(q[1]) << 16, q[2] | static_cast<uint32_t>(q[3]) << 16);
             }
         };
         auto keys = [&](int r, int m) {
-            const uint16_t* q = reinterpret_cast<const uint16_t*>(kp + r * p.kt);
+            const uint16_t* q = reinterpret_cast<const uint16_t*>(kp + r * kt);
             if constexpr (KEYS == KEYS_QUADS) {   // a0 b0 a1 b1
                 const uint2 x = *reinterpret_cast<const uint2*>(q + da[m][0]);
                 return make_uint2(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632));
@@ -176,23 +214,36 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv_append_kernel(AppendA
             }
         };
         // largest magnitudes: of the raw elements as integers of 16 bits (NaN above infinity above all), of the rotated keys
-        uint32_t vmax = 0, raw = 0;
+        uint32_t vmax = 0, raw = 0, flat = 0;   // flat: of keys that are not rotated
         float kmax = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
         for (int r = lo; r < hi; ++r) {
             const uint2 v = values(r);
             vmax = __vimax3_u16x2(vmax, v.x & 0x7fff7fffu, v.y & 0x7fff7fffu);
+        }
 #pragma unroll
-            for (int m = 0; m < KU; ++m) {
-                const uint2 w = keys(r, m);
-                float2 ya, yb;
-                rotated(w, r, m, ya, yb);
-                raw = __vimax3_u16x2(raw, w.x & 0x7fff7fffu, w.y & 0x7fff7fffu);
-                kmax = fmaxf(fmaxf(kmax, fmaxf(fabsf(ya.x), fabsf(ya.y))), fmaxf(fabsf(yb.x), fabsf(yb.y)));
+        for (int m = 0; m < KU; ++m) {
+            if (spins[m]) {
+#pragma unroll 4
+                for (int r = lo; r < hi; ++r) {
+                    const uint2 w = keys(r, m);
+                    float2 ya, yb;
+                    rotated(w, r, m, ya, yb);
+                    raw = __vimax3_u16x2(raw, w.x & 0x7fff7fffu, w.y & 0x7fff7fffu);
+                    kmax = fmaxf(fmaxf(kmax, fmaxf(fabsf(ya.x), fabsf(ya.y))), fmaxf(fabsf(yb.x), fabsf(yb.y)));
+                }
+            } else {
+#pragma unroll 8
+                for (int r = lo; r < hi; ++r) {
+                    const uint2 w = keys(r, m);
+                    flat = __vimax3_u16x2(flat, w.x & 0x7fff7fffu, w.y & 0x7fff7fffu);
+                }
             }
         }
+        flat = max(flat & 0xffffu, flat >> 16);
+        kmax = fmaxf(kmax, up2<T>(flat).x);
         vmax = max(vmax & 0xffffu, vmax >> 16);
-        raw = max(raw & 0xffffu, raw >> 16);
+        raw = max(max(raw & 0xffffu, raw >> 16), flat);
         // A token with an element that is not finite has no key of its own, and does not count for the key's scale; of its values the
         // finite ones stay.
         uint32_t bad = 0;
@@ -235,7 +286,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv_append_kernel(AppendA
         }
         // values: 16 tokens of a dimension are 16 bytes
         if (vlane) {
-            const bool grown = lo > 0 && ve > vbyte, merge = lo > 0 || hi < KV_BLOCK;   // the block holds, or may hold, others' bytes
+            const bool grown = lo > 0 && ve > vbyte, merge = !WHOLE && (lo > 0 || hi < KV_BLOCK);   // the block holds, or may hold, others' bytes
             const float moves = vinv * kv_scale(vbyte);
             uint32_t in[4][4];
 #pragma unroll
@@ -270,47 +321,80 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv_append_kernel(AppendA
             for (int j = 0; j < 4; ++j)
                 *reinterpret_cast<uint4*>(vc + static_cast<int64_t>(4 * lane + j) * KV_PAGE) = make_uint4(in[j][0], in[j][1], in[j][2], in[j][3]);
         }
-#pragma unroll 4
-        for (int r = lo; r < hi; ++r) {
-#pragma unroll
-            for (int m = 0; m < KU; ++m) {
-                float2 ya, yb;
-                rotated(keys(r, m), r, m, ya, yb);
-                uint32_t x = e4m3x2(ya.x * kinv, ya.y * kinv), y = e4m3x2(yb.x * kinv, yb.y * kinv);   // (a0, a1), (b0, b1)
-                if (bad >> r & 1) x = y = 0x7f7fu;
-                if (!has[m]) continue;
-                uint8_t* q = kc + r * DK;
-                if constexpr (KEYS == KEYS_SINGLE) {
-                    q[da[m][0]] = static_cast<uint8_t>(x);
-                    q[da[m][1]] = static_cast<uint8_t>(x >> 8);
-                    q[db[m][0]] = static_cast<uint8_t>(y);
-                    q[db[m][1]] = static_cast<uint8_t>(y >> 8);
+        auto put_key = [&](float2 ya, float2 yb, int r, int m) {
+            uint32_t x = e4m3x2(ya.x * kinv, ya.y * kinv), y = e4m3x2(yb.x * kinv, yb.y * kinv);   // (a0, a1), (b0, b1)
+            if (!has[m]) return;
+            uint8_t* q = kc + r * DK;
+            if constexpr (KEYS == KEYS_SINGLE) {
+                q[da[m][0]] = static_cast<uint8_t>(x);
+                q[da[m][1]] = static_cast<uint8_t>(x >> 8);
+                q[db[m][0]] = static_cast<uint8_t>(y);
+                q[db[m][1]] = static_cast<uint8_t>(y >> 8);
+            } else {
+                const uint32_t w = __byte_perm(x, y, 0x5140);   // a0 b0 a1 b1
+                if constexpr (KEYS == KEYS_QUADS) {
+                    *reinterpret_cast<uint32_t*>(q + da[m][0]) = w;
                 } else {
-                    const uint32_t w = __byte_perm(x, y, 0x5140);   // a0 b0 a1 b1
-                    if constexpr (KEYS == KEYS_QUADS) {
-                        *reinterpret_cast<uint32_t*>(q + da[m][0]) = w;
-                    } else {
-                        const bool turned = 2 * unit[m] < p.r.dim / 2;
-                        *reinterpret_cast<uint16_t*>(q + da[m][0]) = static_cast<uint16_t>(turned ? x : w);
-                        *reinterpret_cast<uint16_t*>(q + (turned ? db[m][0] : da[m][1])) = static_cast<uint16_t>(turned ? y : w >> 16);
-                    }
+                    const bool turned = 2 * unit[m] < p.r.dim / 2;
+                    *reinterpret_cast<uint16_t*>(q + da[m][0]) = static_cast<uint16_t>(turned ? x : w);
+                    *reinterpret_cast<uint16_t*>(q + (turned ? db[m][0] : da[m][1])) = static_cast<uint16_t>(turned ? y : w >> 16);
                 }
             }
+        };
+#pragma unroll
+        for (int m = 0; m < KU; ++m) {
+            if (spins[m]) {
+#pragma unroll 4
+                for (int r = lo; r < hi; ++r) {
+                    float2 ya, yb;
+                    rotated(keys(r, m), r, m, ya, yb);
+                    put_key(ya, yb, r, m);
+                }
+            } else {
+#pragma unroll 4
+                for (int r = lo; r < hi; ++r) {
+                    const uint2 w = keys(r, m);
+                    put_key(up2<T>(w.x), up2<T>(w.y), r, m);
+                }
+            }
+        }
+        if (bad) {
+            __syncwarp();   // (after the codes of these rows)
+#pragma unroll 1
+            for (int r = lo; r < hi; ++r)
+                if (bad >> r & 1)
+                    for (int i = lane; i < DK; i += 32) kc[r * DK + i] = 0x7f;
         }
         __syncwarp();   // every lane has read the old scales
         if (lane == 0) {
             *ks = static_cast<uint8_t>(ke);
             *vs = static_cast<uint8_t>(ve);
         }
+    };
+    const bool fills = lo == 0 && hi == KV_BLOCK;
+    for (int h = warp; h < p.c.kv_heads; h += nwarps) {
+        if (fills) one_head(std::true_type{}, h);
+        else one_head(std::false_type{}, h);
     }
 }
 
-template <typename T, int DK, int DV> static cudaError_t append_launch(const AppendArgs& p, int keys, unsigned grid, cudaStream_t st)
+template <typename T, int DK, int DV, int KEYS> static cudaError_t append_staged(const AppendArgs& p, unsigned grid, dim3 threads, cudaStream_t st)
+{
+    static std::atomic<uint64_t> done{0};
+    constexpr int EACH = KV_BLOCK * (DK + DV) * sizeof(T);   // of a warp
+    const auto kernel = &kv_append_kernel<T, DK, DV, KEYS, true>;
+    const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), APPEND_WARPS * EACH, done);
+    if (e != cudaSuccess) return e;
+    return launch_after(*kernel, dim3(grid), threads, static_cast<size_t>(threads.x / 32 * EACH), st, p);
+}
+
+template <typename T, int DK, int DV> static cudaError_t append_launch(const AppendArgs& p, int keys, bool staged, unsigned grid, cudaStream_t st)
 {
     const dim3 threads(32 * (p.c.kv_heads < APPEND_WARPS ? p.c.kv_heads : APPEND_WARPS));
-    if (keys == KEYS_QUADS) return launch_after(kv_append_kernel<T, DK, DV, KEYS_QUADS>, dim3(grid), threads, 0, st, p);
-    if (keys == KEYS_HALVES) return launch_after(kv_append_kernel<T, DK, DV, KEYS_HALVES>, dim3(grid), threads, 0, st, p);
-    return launch_after(kv_append_kernel<T, DK, DV, KEYS_SINGLE>, dim3(grid), threads, 0, st, p);
+    if (staged) return keys == KEYS_QUADS ? append_staged<T, DK, DV, KEYS_QUADS>(p, grid, threads, st) : append_staged<T, DK, DV, KEYS_HALVES>(p, grid, threads, st);
+    if (keys == KEYS_QUADS) return launch_after(kv_append_kernel<T, DK, DV, KEYS_QUADS, false>, dim3(grid), threads, 0, st, p);
+    if (keys == KEYS_HALVES) return launch_after(kv_append_kernel<T, DK, DV, KEYS_HALVES, false>, dim3(grid), threads, 0, st, p);
+    return launch_after(kv_append_kernel<T, DK, DV, KEYS_SINGLE, false>, dim3(grid), threads, 0, st, p);
 }
 
 template <typename T> static cudaError_t append_typed(const AppendArgs& p, cudaStream_t st)
@@ -322,10 +406,11 @@ template <typename T> static cudaError_t append_typed(const AppendArgs& p, cudaS
                          static_cast<uint64_t>(p.kt | p.kh | p.vt | p.vh) * 2;
     const bool quads = p.r.interleaved || p.r.dim == 0;
     const int keys = off % 8 != 0 ? KEYS_SINGLE : quads ? KEYS_QUADS : p.r.dim % 4 == 0 ? KEYS_HALVES : KEYS_SINGLE;
+    const bool staged = off % 16 == 0 && keys != KEYS_SINGLE;
     const unsigned g = static_cast<unsigned>(grid);
-    if (p.c.key_dim == 64) return append_launch<T, 64, 64>(p, keys, g, st);
-    if (p.c.key_dim == 128) return append_launch<T, 128, 128>(p, keys, g, st);
-    return append_launch<T, 192, 128>(p, keys, g, st);
+    if (p.c.key_dim == 64) return append_launch<T, 64, 64>(p, keys, staged, g, st);
+    if (p.c.key_dim == 128) return append_launch<T, 128, 128>(p, keys, staged, g, st);
+    return append_launch<T, 192, 128>(p, keys, staged, g, st);
 }
 
 bool kv_cache_ok(const EvaKvCache* c)
