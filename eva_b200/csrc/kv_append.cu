@@ -105,6 +105,25 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, STAGED ? (DK == 64 ? 4 : DK
     if (page < 0) return;
     const int lo = max(first - base, 0), hi = min(s.len - base, KV_BLOCK), at = base % KV_PAGE;
     const int64_t tok0 = static_cast<int64_t>(s.row0) + base - s.ctx;   // token row of the block's slot 0
+    // A head's rows on their way to shared memory, a bulk copy each, in flight while the angles, or the head before, are worked on
+    T* const staged_k = reinterpret_cast<T*>(stage_raw + warp * (KV_BLOCK * (DK + DV) / 8));
+    T* const staged_v = staged_k + KV_BLOCK * DK;
+    auto stage_keys = [&](int h) {   // and announces the values
+        __syncwarp();                // every lane is done with the keys before
+        if (lane == 0) mbar_arrive_expect_tx(&bars[warp], (hi - lo) * (DK + DV) * sizeof(T));
+        __syncwarp();
+        if (lane >= lo && lane < hi)
+            bulk_g2s(staged_k + lane * DK, static_cast<const T*>(p.k) + h * p.kh + (tok0 + lane) * p.kt, DK * sizeof(T), &bars[warp]);
+    };
+    auto stage_values = [&](int h) {
+        __syncwarp();
+        if (lane >= lo && lane < hi)
+            bulk_g2s(staged_v + lane * DV, static_cast<const T*>(p.v) + h * p.vh + (tok0 + lane) * p.vt, DV * sizeof(T), &bars[warp]);
+    };
+    if constexpr (STAGED) {
+        stage_keys(warp);
+        stage_values(warp);
+    }
     const bool rotates = p.r.dim > 0;
     if (rotates) {
         for (int i = threadIdx.x; i < (hi - lo) * UNITS; i += blockDim.x) {
@@ -161,20 +180,10 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, STAGED ? (DK == 64 ? 4 : DK
         const T* kp = static_cast<const T*>(p.k) + h * p.kh + tok0 * p.kt;
         const T* vp = static_cast<const T*>(p.v) + h * p.vh + tok0 * p.vt;
         if constexpr (STAGED) {
-            T* const ring = reinterpret_cast<T*>(stage_raw + warp * (KV_BLOCK * (DK + DV) / 8));
-            // a bulk copy for each row: lanes 0 .. 15 the keys, 16 .. 31 the values
-            __syncwarp();   // every lane is done with the head before
-            const int r = lane % KV_BLOCK;
-            if (lane == 0) mbar_arrive_expect_tx(&bars[warp], (hi - lo) * (DK + DV) * sizeof(T));
-            __syncwarp();
-            if (r >= lo && r < hi) {
-                if (lane < KV_BLOCK) bulk_g2s(ring + r * DK, kp + r * p.kt, DK * sizeof(T), &bars[warp]);
-                else bulk_g2s(ring + KV_BLOCK * DK + r * DV, vp + r * p.vt, DV * sizeof(T), &bars[warp]);
-            }
             mbar_wait(&bars[warp], phase, p.c.status);
             phase ^= 1;
-            kp = ring;
-            vp = ring + KV_BLOCK * DK;
+            kp = staged_k;
+            vp = staged_v;
         }
         if (vlane) vp += 4 * lane;
         const int64_t kt = STAGED ? DK : p.kt, vt = STAGED ? DV : p.vt;
@@ -284,43 +293,6 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, STAGED ? (DK == 64 ? 4 : DK
                 *q = static_cast<uint16_t>(e4m3_scaled(*q, m));
             }
         }
-        // values: 16 tokens of a dimension are 16 bytes
-        if (vlane) {
-            const bool grown = lo > 0 && ve > vbyte, merge = !WHOLE && (lo > 0 || hi < KV_BLOCK);   // the block holds, or may hold, others' bytes
-            const float moves = vinv * kv_scale(vbyte);
-            uint32_t in[4][4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint4 was = make_uint4(0, 0, 0, 0);
-                if (merge) was = *reinterpret_cast<const uint4*>(vc + static_cast<int64_t>(4 * lane + j) * KV_PAGE);
-                in[j][0] = was.x, in[j][1] = was.y, in[j][2] = was.z, in[j][3] = was.w;
-            }
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {   // tokens 2 t, 2 t + 1
-                const bool fresh0 = 2 * t >= lo && 2 * t < hi, fresh1 = 2 * t + 1 >= lo && 2 * t + 1 < hi;
-                if (merge && !fresh0 && !fresh1 && !(grown && 2 * t < lo)) continue;
-                uint2 v0 = fresh0 ? values(2 * t) : make_uint2(0, 0), v1 = fresh1 ? values(2 * t + 1) : make_uint2(0, 0);
-                if (odd) {
-                    v0 = make_uint2(finite_only(v0.x), finite_only(v0.y));
-                    v1 = make_uint2(finite_only(v1.x), finite_only(v1.y));
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 x = up2<T>(j < 2 ? v0.x : v0.y), y = up2<T>(j < 2 ? v1.x : v1.y);
-                    uint32_t two = e4m3x2((j % 2 ? x.y : x.x) * vinv, (j % 2 ? y.y : y.x) * vinv);
-                    if (merge) {
-                        const uint32_t old = in[j][t / 2] >> (t % 2 * 16) & 0xffffu;
-                        const uint32_t moved = grown ? e4m3_scaled(old, moves) : old;
-                        const uint32_t a = 2 * t < lo ? moved : fresh0 ? two : old, c = 2 * t + 1 < lo ? moved : fresh1 ? two : old;
-                        two = (a & 0xffu) | (c & 0xff00u);
-                    }
-                    in[j][t / 2] = t % 2 ? (in[j][t / 2] & 0xffffu) | two << 16 : (in[j][t / 2] & 0xffff0000u) | two;
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<uint4*>(vc + static_cast<int64_t>(4 * lane + j) * KV_PAGE) = make_uint4(in[j][0], in[j][1], in[j][2], in[j][3]);
-        }
         auto put_key = [&](float2 ya, float2 yb, int r, int m) {
             uint32_t x = e4m3x2(ya.x * kinv, ya.y * kinv), y = e4m3x2(yb.x * kinv, yb.y * kinv);   // (a0, a1), (b0, b1)
             if (!has[m]) return;
@@ -365,6 +337,47 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, STAGED ? (DK == 64 ? 4 : DK
                 if (bad >> r & 1)
                     for (int i = lane; i < DK; i += 32) kc[r * DK + i] = 0x7f;
         }
+        if constexpr (STAGED)
+            if (h + nwarps < p.c.kv_heads) stage_keys(h + nwarps);
+        // values: 16 tokens of a dimension are 16 bytes
+        if (vlane) {
+            const bool grown = lo > 0 && ve > vbyte, merge = !WHOLE && (lo > 0 || hi < KV_BLOCK);   // the block holds, or may hold, others' bytes
+            const float moves = vinv * kv_scale(vbyte);
+            uint32_t in[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint4 was = make_uint4(0, 0, 0, 0);
+                if (merge) was = *reinterpret_cast<const uint4*>(vc + static_cast<int64_t>(4 * lane + j) * KV_PAGE);
+                in[j][0] = was.x, in[j][1] = was.y, in[j][2] = was.z, in[j][3] = was.w;
+            }
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {   // tokens 2 t, 2 t + 1
+                const bool fresh0 = 2 * t >= lo && 2 * t < hi, fresh1 = 2 * t + 1 >= lo && 2 * t + 1 < hi;
+                if (merge && !fresh0 && !fresh1 && !(grown && 2 * t < lo)) continue;
+                uint2 v0 = fresh0 ? values(2 * t) : make_uint2(0, 0), v1 = fresh1 ? values(2 * t + 1) : make_uint2(0, 0);
+                if (odd) {
+                    v0 = make_uint2(finite_only(v0.x), finite_only(v0.y));
+                    v1 = make_uint2(finite_only(v1.x), finite_only(v1.y));
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 x = up2<T>(j < 2 ? v0.x : v0.y), y = up2<T>(j < 2 ? v1.x : v1.y);
+                    uint32_t two = e4m3x2((j % 2 ? x.y : x.x) * vinv, (j % 2 ? y.y : y.x) * vinv);
+                    if (merge) {
+                        const uint32_t old = in[j][t / 2] >> (t % 2 * 16) & 0xffffu;
+                        const uint32_t moved = grown ? e4m3_scaled(old, moves) : old;
+                        const uint32_t a = 2 * t < lo ? moved : fresh0 ? two : old, c = 2 * t + 1 < lo ? moved : fresh1 ? two : old;
+                        two = (a & 0xffu) | (c & 0xff00u);
+                    }
+                    in[j][t / 2] = t % 2 ? (in[j][t / 2] & 0xffffu) | two << 16 : (in[j][t / 2] & 0xffff0000u) | two;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<uint4*>(vc + static_cast<int64_t>(4 * lane + j) * KV_PAGE) = make_uint4(in[j][0], in[j][1], in[j][2], in[j][3]);
+        }
+        if constexpr (STAGED)
+            if (h + nwarps < p.c.kv_heads) stage_values(h + nwarps);
         __syncwarp();   // every lane has read the old scales
         if (lane == 0) {
             *ks = static_cast<uint8_t>(ke);
