@@ -2,10 +2,11 @@
 //
 // At most 16 rows (new tokens x query heads of a group) share each key and value, so the cache's bytes are the cost: every
 // one is read once. The tokens of all sequences and heads, in tiles of a page (64), form one line of work that is cut
-// into equal pieces, one per warp of the GPU, whatever the lengths are; a warp's tiles come through its own
+// into equal pieces, one per warp, whatever the lengths are; a warp's tiles come through its own
 // two-stage ring of bulk copies (a page of a head is contiguous). Scores and outputs are m16n8k16 products with fp32 sums,
 // transposed: keys and values are the 16-row operand and the query rows the 8-column one, so that up to eight rows cost what one
-// does and no product is padding. The codes themselves are multiplied (e4m3 is exact in fp16); their scales stay outside: a
+// does and no product is padding (an accumulator in tensor memory has 128 rows; the tensor pipes are at 19 % here, DRAM is the
+// bound). The codes themselves are multiplied (e4m3 is exact in fp16); their scales stay outside: a
 // token's key scale multiplies its score, its value scale 2^e joins the exponent, t = score + e, and the softmax's running
 // maximum is that of t:
 //   out = sum 2^(t - M) code / sum 2^(t - M) 2^-e.
@@ -15,6 +16,10 @@
 // 16 (r / 2) + 4 e + (0, 2) + r % 2, and lane quad q holds of the values tokens 16 q .. 16 q + 15.
 // An item (sequence and head) whose tiles fall to several warps leaves fp32 partial sums, which
 // kv_combine_kernel joins in their order, so results do not depend on timing.
+//
+// 128 + 128 dimensions, 8 heads of keys: 64 sequences of up to 8192 tokens, 4 rows: 581 MB in 103 us, 5.6 TB/s (0.86 of the 6.5 a
+// copy reaches); two of 131072, 8 rows: 537 MB in 98.5 us, 5.5 TB/s. Smaller calls are latency: 16 sequences of some 3000 tokens
+// within a window of 4096, 4 heads, 16 rows: 54 MB in 38 us, of which a warp's six to eight tiles one behind the other take 20.
 #include <algorithm>
 
 #include "kv.cuh"
@@ -24,7 +29,9 @@
 
 namespace eva {
 
-constexpr int DEC_ROWS = 16, DEC_PIECE = 6;
+constexpr int DEC_ROWS = 16;
+// Tiles of a piece at least, but for calls that this leaves fewer than DEC_SPREAD pieces for each SM: see kv_decode_kernel
+constexpr int DEC_PIECE = 8, DEC_SPREAD = 4;
 constexpr float P_BIAS = 14.0f;   // weights are at most 2^14
 
 template <int DK, int DV> struct DecCfg {
@@ -109,9 +116,11 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(At
     for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
     total *= p.c.kv_heads;
     const int g = warp * gridDim.x + blockIdx.x;
-    // Pieces, none of them empty; of DEC_PIECE tiles at least where that leaves one for each SM, since every piece that cuts an item
-    // leaves partial sums.
-    const int nw = static_cast<int>(min(min(static_cast<int64_t>(C::W * gridDim.x), total), max(static_cast<int64_t>(gridDim.x), total / DEC_PIECE)));
+    // Pieces, none of them empty. Every piece that cuts an item leaves partial sums to be joined, every tile waits for the one before it:
+    // a decode step (rotation and append too) of 24 sequences of up to 3000 tokens takes 42.6 us in pieces of 8 tiles, 45 of 6, 45.7
+    // with one for every warp; but 16 sequences of 2000 tokens and one head 19 us in four pieces for each SM, 25.5 in one.
+    const int64_t most = static_cast<int64_t>(C::W) * gridDim.x, spread = static_cast<int64_t>(DEC_SPREAD) * gridDim.x;
+    const int nw = static_cast<int>(min(min(most, total), max(spread, total / DEC_PIECE)));
     const int64_t begin = g < nw ? total * g / nw : 0;
     int64_t end = g < nw ? total * (g + 1) / nw : 0;
     DecRest lead{}, tail{};   // of an item that began before the piece, and of one that goes on behind it
@@ -511,7 +520,7 @@ template <int DK, int DV, typename T, int NT> static cudaError_t decode_launch(A
 
 template <typename T> static cudaError_t decode_typed(const AttendArgs& p, int pieces, cudaStream_t st)
 {
-    const bool one = p.part_rows <= 8;
+    const bool one = p.part_rows <= 8;   // a group of eight rows or two: 4 rows 103 us, 142 with an empty second group
     if (p.c.key_dim == 64) return one ? decode_launch<64, 64, T, 1>(p, pieces, st) : decode_launch<64, 64, T, 2>(p, pieces, st);
     if (p.c.key_dim == 128) return one ? decode_launch<128, 128, T, 1>(p, pieces, st) : decode_launch<128, 128, T, 2>(p, pieces, st);
     return one ? decode_launch<192, 128, T, 1>(p, pieces, st) : decode_launch<192, 128, T, 2>(p, pieces, st);
@@ -526,7 +535,9 @@ static bool attend_ok(const EvaKvCache* cache, const EvaKvBatch* batch, int32_t 
     return kv_cache_ok(cache) && kv_batch_ok(batch) && heads >= 1 && heads % cache->kv_heads == 0;
 }
 
-// Rows that share a key and value head's tokens, and whether the decode kernel takes them.
+// Rows that share a key and value head's tokens. Up to 16 the decode kernel takes them: 64 sequences of 8000 tokens and 16 rows 61 us,
+// 90 in the prompt kernel, 4 rows 103 against 332 (8 heads); one of 16 x 2000 19 against 23. More rows than two products' columns
+// would reload the queries and halve the decode kernel's warps; 24 rows are 90 us in the prompt kernel, as 16 are.
 static int64_t shared_rows(const EvaKvCache& c, const EvaKvBatch& b, int heads)
 {
     return static_cast<int64_t>(b.max_q) * (heads / c.kv_heads);

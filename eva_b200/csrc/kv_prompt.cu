@@ -1,9 +1,10 @@
 // Attention over the paged 8-bit cache on the tensor cores: many rows per sequence and key/value head (prompts).
 //
 // A CTA holds 256 rows (token, query head of the group) of one sequence and key/value head as two tiles of 128, and walks
-// the sequence's tokens 128 at a time: S = Q K^T (tcgen05.mma, M 128, N 128), softmax, O += P V with P as the A
-// operand in tensor memory. The two tiles alternate: while the tensor cores multiply for one, eight warps (a thread per row)
-// do the softmax of the other. Tensor memory is full: two S of 128 columns (P, 16-bit, overwrites its own S) and two O.
+// the sequence's tokens a page (64) at a step: S = Q K^T (tcgen05.mma, M 128, N 64), softmax, O += P V with P as the A
+// operand in tensor memory. A tile has two S (of even and odd steps; P, 16-bit, overwrites its own S), and four warps for each, a
+// thread per row: scores run two steps ahead, and consecutive steps overlap but for the running maximum M, which
+// the warps of one parity hand to those of the other. Tensor memory is full: four S of 64 columns and two O of value_dim.
 //
 // Bulk copies bring a page's codes as they are; four more warps turn them into fp16 (exact) in the 128-byte swizzled layout: a page's
 // keys are rows of key_dim, its values rows of 64 tokens, so both are K-major operands without a transposition. Converting for
@@ -12,9 +13,18 @@
 // M is raised (and O rescaled in tensor memory) only when a row's maximum has grown by more than 2^12: weights are fp16 up to 2^15,
 // 2^3 at M, so that tokens down to 2^-17 of it keep 11 bits, and 2^-27 is the step below.
 //
-// The (sequence, head, row block, token tile) units of a call form one line that is cut into equal pieces, one per SM, so
+// The (sequence, head, row block, token step) units of a call form one line that is cut into pieces of equal cost, one per SM, so
 // causal rows of different lengths and ragged batches fill the GPU alike; row blocks cut between pieces leave fp32 partial
 // sums that kv_prompt_combine joins in their order.
+//
+// 8192 new tokens, 16 query heads on 4 of 128 + 128 dimensions: 352 us, 275 GFLOP at 780 TFLOP/s (0.47 of the 1679 that a library
+// product reaches); three sequences of up to 700 tokens behind 20000, 16 heads of 192 + 128: 352 us, 730 TFLOP/s. What bounds
+// it is one step's chain: scores, maximum, weights, their product take 1900 clocks of tensor core and 3200 of softmax for each tile
+// and parity, of which two overlap, so 2550 a step; the tensor pipe is 39 % busy, exponentials 39 %, issue 51 %. Steps there
+// (prompt, pieces): one S per tile and 128 tokens a step 835, 625 us; scores read from tensor memory once 646, 494; products issued from
+// rolled loops (straight-line code that one warp runs once a step comes from memory every time) 579, 451; codes by bulk copies
+// 570, 357; two S a tile 548, 351; parities with warps of their own 493, 358; row blocks weighed 355, 352. Slower: 128 tokens a step with
+// a row's scores in registers, two threads a row, one pass with a maximum that lags.
 #include <algorithm>
 
 #include "decode_tc.cuh"
@@ -100,7 +110,7 @@ __device__ __forceinline__ PrItem pr_item(const KvSeq& s, int group, int window,
 __device__ __forceinline__ int pr_blocks(const KvSeq& s, int group) { return (s.n * group + PR_ROWS - 1) / PR_ROWS; }
 
 // Cost of one head of a sequence in steps (whole warp): a row block counts its steps and, before them, PR_BLOCK_COST for the time
-// its query, first scores and output take (15k clocks, against 2.5k of a step).
+// its query, first scores and output take (15k clocks, against 2.5k of a step; without it the 8192 tokens above take 485 us, not 352).
 __device__ __forceinline__ int64_t pr_units(const KvSeq& s, int group, int window)
 {
     int64_t sum = 0;
@@ -117,7 +127,6 @@ struct PrPlace {
     int b, h, qb, off, left, pieces;
     int64_t begin, total;
 };
-
 
 // Consecutive steps of one row block within a piece; t1 == 0 ends the piece.
 struct PrSeg {
@@ -414,7 +423,8 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
     after_previous();
     // this CTA's piece of the line
     const int span = (p.b.seqs + PR_SPANS - 1) / PR_SPANS;
-    if (p.b.seqs < 64) {   // a warp for each sequence's row blocks, or a thread
+    // a warp for each sequence's row blocks where there are few sequences, else a thread: 1000 sequences of one block 57 us, 88 by warps
+    if (p.b.seqs < 64) {
         for (int b = warp; b < p.b.seqs; b += PR_WARPS) {
             const int64_t u = pr_units(kv_seq(p.b, b, status), p.group, p.window);
             if (lane == 0 && u > 0) atomicAdd(&spans[b / span], static_cast<unsigned long long>(u));

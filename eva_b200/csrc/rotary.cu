@@ -5,7 +5,8 @@
 // conversion rounds (1e-7 of a radian). A thread takes one 16-byte unit of a head (for pairs (i, i + dim / 2)
 // the two units that hold both halves), computes its pairs' cosines and sines once and applies them to
 // `hc` heads. The traffic is one read and one write of x; the copied dimensions outside the rotated part
-// go through the same threads, and are left out when x is rotated in place.
+// go through the same threads, and are left out when x is rotated in place. DRAM bounds it: 8192 x 32 heads of 192 bf16, 64 rotated,
+// 45 us, 201 MB at 4.5 TB/s (0.69 of a copy's 6.5; torch's copy of the same tensor takes 35 us). One token: 9 us, the host's.
 #include <algorithm>
 
 #include "kv.cuh"
@@ -67,7 +68,7 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(RotArgs p)
     const int half = p.dim / 2;
     // All of the thread's loads first, then its angles: a load is 1 us away, and so is the position. Copied and rotated units of a
     // warp take one path, so that their loads are under way together, and a thread with all B heads has no branch between them
-    // (8192 x 32 heads of 192 dimensions, 64 rotated: 43 us; with a check of each head 76 us; torch copies as much in 35 us).
+    // (8192 x 32 heads of 192 dimensions, 64 rotated: 45 us; with a check of each head 76 us).
     Vec a[B], b[INTER ? 1 : B];
     const bool full = h1 - h0 == B;
     auto load = [&](int k) {
