@@ -5,15 +5,16 @@
 // conversion rounds (1e-7 of a radian). A thread takes one 16-byte unit of a head (for pairs (i, i + dim / 2)
 // the two units that hold both halves), computes its pairs' cosines and sines once and applies them to
 // `hc` heads. The traffic is one read and one write of x; the copied dimensions outside the rotated part
-// go through the same threads, and are left out when x is rotated in place. DRAM bounds it: 8192 x 32 heads of 192 bf16, 64 rotated,
-// 45 us, 201 MB at 4.5 TB/s (0.69 of a copy's 6.5; torch's copy of the same tensor takes 35 us). One token: 9 us, the host's.
+// go through the same threads, and are left out when x is rotated in place. 8192 x 32 heads of 192 bf16, 64 rotated: interleaved 42
+// us, 201 MB at 4.8 TB/s of a copy's 6.5; bounded by loads, angles and stores in turn with 20 warps an SM (their registers hold
+// eight units). One token: 9 us, the host's.
 #include <algorithm>
 
 #include "kv.cuh"
 
 namespace eva {
 
-constexpr int ROT_THREADS = 256;
+constexpr int ROT_THREADS = 64;   // 256: 48.6 us for the case below, 128: 42; a block's loads, angles and stores follow one another
 
 template <bool INTER> constexpr int ROT_HEADS = INTER ? 8 : 4;   // heads of a thread at most: eight units in flight
 
@@ -42,8 +43,9 @@ template <typename T, int V> struct alignas(sizeof(T) * V) RotVec {
 
 // Units of a head, V elements each (half layout: a rotated unit is V elements of each half):
 // [0, offset / V) copied, then the rotated ones, then the copied rest. V divides every part.
+// Ten blocks an SM for pairs of halves: 62 us, 66 with the registers it would take; interleaved pairs 41.5 and 39.4.
 template <typename T, int V, bool INTER>
-__global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(RotArgs p)
+__global__ void __launch_bounds__(ROT_THREADS, INTER ? 1 : 10) rotary_kernel(RotArgs p)
 {
     using Vec = RotVec<T, V>;
     constexpr int NP = INTER ? V / 2 : V, B = ROT_HEADS<INTER>;
@@ -68,7 +70,7 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(RotArgs p)
     const int half = p.dim / 2;
     // All of the thread's loads first, then its angles: a load is 1 us away, and so is the position. Copied and rotated units of a
     // warp take one path, so that their loads are under way together, and a thread with all B heads has no branch between them
-    // (8192 x 32 heads of 192 dimensions, 64 rotated: 45 us; with a check of each head 76 us).
+    // (with a check of each head such a call took 76 us, not 45).
     Vec a[B], b[INTER ? 1 : B];
     const bool full = h1 - h0 == B;
     auto load = [&](int k) {
