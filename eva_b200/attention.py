@@ -362,7 +362,7 @@ class PagedKVCache:
     def attend(self, q, batch, *, scale=None, window=0, out=None):
         """softmax(scale q k^T) v of q [tokens, heads, key_dim] (BF16 or Half, already rotated) over the batch's sequences,
         new tokens included: a row sees the tokens up to its own position, with window > 0 the last `window` of them.
-        heads is a multiple of kv_heads. Returns [tokens, heads, value_dim] of q's type; rows that see nothing are zero, rows behind
+        heads is a multiple of kv_heads. Values below 2^-39 may count as zero in the output (not in the softmax's sum). Returns [tokens, heads, value_dim] of q's type; rows that see nothing are zero, rows behind
         the last sequence are left as they were (in out; a new tensor has no values there)."""
         device = self.device
         if (not isinstance(q, torch.Tensor) or q.ndim != 3 or q.dtype not in (_BF16, _F16) or q.device != device
