@@ -1,4 +1,4 @@
-"""Plain 64-bit forms of the attention operators (CPU torch, loops): the parity checker of the tests.
+"""Plain 64-bit forms of the attention operators (CPU torch, loops): what the tests compare with.
 
 Rotation, the append into the paged 8-bit cache (one power-of-two scale for each 16 tokens and head, older codes
 rescaled when it grows), and causal attention over the cache, each written from its definition.

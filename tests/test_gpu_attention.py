@@ -230,6 +230,33 @@ def test_append_step_by_step_equals_one_append():
         assert bool(((x - y).abs() <= step).all())
 
 
+@pytest.mark.parametrize("dims", DIMS)
+@pytest.mark.parametrize("layout,rot,offset", [("half", 40, 8), ("half", 22, 2), ("interleaved", 64, 0), (None, 0, 0)])
+@pytest.mark.parametrize("kv_heads", [3, 19])
+def test_append_of_rows_anywhere_in_memory(dims, layout, rot, offset, kv_heads):
+    """The same bytes whether rows lie on 16 bytes (bulk copies), on 8, or on 2; whole and part blocks, more heads than warps."""
+    dk, dv = dims
+    new, lens = [1, 50, 16, 37], [9, 50, 48, 70]
+    rotary = Rotary(rot, layout=layout, offset=offset) if rot else None
+    want = None
+    for shift in (0, 4, 1):
+        s = Setup(dims, kv_heads, new, lens, seed=kv_heads)
+        wide = torch.zeros(s.T, kv_heads * (dk + dv) + 8, dtype=BF16, device=DEV)
+        wide[:, shift:shift + kv_heads * (dk + dv)] = s.rows(kv_heads, dk + dv, BF16).to(DEV).flatten(1)
+        both = wide[:, shift:shift + kv_heads * (dk + dv)].unflatten(1, (kv_heads, dk + dv))
+        s.cache.append(both[..., :dk], both[..., dk:], s.batch, rotary=rotary)
+        assert s.cache.status() == 0
+        got = [getattr(s.cache, n).view(torch.uint8).clone() for n in ("k", "v", "k_scale", "v_scale")]
+        if want is None:
+            want = got
+            if rotary is None:
+                k, v = both[..., :dk].cpu().double(), both[..., dk:].cpu().double()
+                A.append(s.host, k, v, s.start, s.lens, s.table)
+                _same_bytes(s.cache.k, s.host["k"], "k")
+                _same_bytes(s.cache.v, s.host["v"], "v")
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), shift
+
+
 def test_append_of_values_that_are_not_finite():
     """Such a token gets a NaN key; its block's other tokens and scales are as if it were not there, and so are its finite values."""
     s = Setup((64, 64), 2, [40], [70], seed=2)
