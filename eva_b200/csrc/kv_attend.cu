@@ -19,7 +19,7 @@
 //
 // 128 + 128 dimensions, 8 heads of keys: 64 sequences of up to 8192 tokens, 4 rows: 581 MB in 103 us, 5.6 TB/s (0.86 of the 6.5 a
 // copy reaches); two of 131072, 8 rows: 537 MB in 98.5 us, 5.5 TB/s. Smaller calls are latency: 16 sequences of some 3000 tokens
-// within a window of 4096, 4 heads, 16 rows: 54 MB in 38 us, of which a warp's six to eight tiles one behind the other take 20.
+// within a window of 4096, 4 heads, 16 rows: 54 MB in 36.5 us, of which a warp's six to eight tiles one behind the other take 25.
 #include <algorithm>
 
 #include "kv.cuh"
@@ -31,7 +31,7 @@ namespace eva {
 
 constexpr int DEC_ROWS = 16;
 // Tiles of a piece at least, but for calls that this leaves fewer than DEC_SPREAD pieces for each SM: see kv_decode_kernel
-constexpr int DEC_PIECE = 8, DEC_SPREAD = 4;
+constexpr int DEC_PIECE = 8, DEC_SPREAD = 4, DEC_JOIN = 16;   // DEC_JOIN: parts of an item that one warp joins
 constexpr float P_BIAS = 14.0f;   // weights are at most 2^14
 
 template <int DK, int DV> struct DecCfg {
@@ -462,9 +462,10 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(At
     if (lane < DEC_ROWS) count[lane] = 0;
 }
 
-// Joins the partial sums of the items that lie in several pieces. The parts of an item are joined in groups of eight by the warp of
+// Joins the partial sums of the items that lie in several pieces. The parts of an item are joined in groups of 16 by the warp of
 // the group's first piece (and row); where there are more groups, the one that is done last joins the groups, in their
-// order whichever that is, so that an item of a thousand pieces takes as long as three loads, not a hundred.
+// order whichever that is, so that an item of a thousand pieces takes as long as ten loads, not a hundred. A second level costs 5 us,
+// eight more parts one: groups of 8, 16, 32 take 38.5, 36.6, 36.6 us for the drafted tokens above, 99.2, 98.4, 100.2 for the two of 131072.
 template <int DV, typename T>
 __global__ void __launch_bounds__(COMBINE_THREADS) kv_combine_kernel(AttendArgs p, int pieces)
 {
@@ -478,14 +479,14 @@ __global__ void __launch_bounds__(COMBINE_THREADS) kv_combine_kernel(AttendArgs 
     for (int slot = 0; slot < 2; ++slot) {
         const DecRest rest = rests[2 * g + slot];
         const int i = g - rest.first;   // this piece's part of the item
-        if (rest.first < 0 || i % 8 != 0 || r >= rest.n * p.group) continue;
+        if (rest.first < 0 || i % DEC_JOIN != 0 || r >= rest.n * p.group) continue;
         // part k of the item: its first piece, slot 1, then the next pieces, slot 0
         float* base = p.part + static_cast<int64_t>(rest.first) * 2 * step;
         auto part = [&](int k) { return base + (k == 0 ? step : static_cast<int64_t>(k) * 2 * step); };
-        const int parts = rest.last - rest.first + 1, groups = (parts + 7) / 8, tok = r / p.group;
+        const int parts = rest.last - rest.first + 1, groups = (parts + DEC_JOIN - 1) / DEC_JOIN, tok = r / p.group;
         T* out = static_cast<T*>(p.out) + ((static_cast<int64_t>(rest.row0) + tok) * p.heads + rest.h * p.group + (r - tok * p.group)) * DV;
         float m, l, o[4];
-        join_parts<DV>([&](int k) { return part(i + k); }, min(8, parts - i), r, R + r, 2 * R + r * DV, lane, m, l, o);
+        join_parts<DV>([&](int k) { return part(i + k); }, min(DEC_JOIN, parts - i), r, R + r, 2 * R + r * DV, lane, m, l, o);
         if (groups > 1) {
             float* own = part(i);   // no other warp reads this row of it
             __syncwarp();
@@ -500,7 +501,7 @@ __global__ void __launch_bounds__(COMBINE_THREADS) kv_combine_kernel(AttendArgs 
             if (lane == 0) before = atomicAdd(counts + rest.first * DEC_ROWS + r, 1);
             if (__shfl_sync(0xffffffffu, before, 0) != groups - 1) continue;
             __threadfence();
-            join_parts<DV>([&](int k) { return part(8 * k); }, groups, r, R + r, 2 * R + r * DV, lane, m, l, o);
+            join_parts<DV>([&](int k) { return part(DEC_JOIN * k); }, groups, r, R + r, 2 * R + r * DV, lane, m, l, o);
         }
         put_row<DV, T>(out, l, o, lane);
     }
