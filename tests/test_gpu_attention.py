@@ -465,6 +465,50 @@ def test_attention_of_one_long_sequence_and_head():
         assert torch.equal(out, s.cache.attend(q, s.batch))
 
 
+@pytest.mark.parametrize("new", [1, 3, 100])
+def test_pages_beyond_32_bit_offsets(new):
+    """The last pages of a cache of 4.6 GB of keys give what its first ones do, through a table that is a slice of a wider one."""
+    pages, heads = 70000, 8
+    assert pages * heads * 64 * 128 > 2**32
+    cache = PagedKVCache(pages, heads, 128)
+    g = torch.Generator().manual_seed(new)
+    k, v = (torch.randn(130, heads, 128, generator=g).to(BF16).to(DEV) for _ in range(2))
+    q = torch.randn(new, 2 * heads, 128, generator=g).to(BF16).to(DEV)
+    int32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)   # noqa: E731
+    rotary, outs = Rotary(128, layout="half"), []
+    for ids in ([0, 2, 1], [pages - 1, pages - 3, pages - 2]):
+        table = int32([[-1] + ids + [-1, -1]])[:, 1:4]
+        cache.append(k, v, PagedBatch(int32([0, 130]), int32([130]), table, 130), rotary=rotary)
+        outs.append(cache.attend(q, PagedBatch(int32([0, new]), int32([130]), table, new)))
+    first, last = torch.tensor([0, 2, 1], device=DEV), torch.tensor([pages - 1, pages - 3, pages - 2], device=DEV)
+    for t in (cache.k, cache.v, cache.k_scale, cache.v_scale):
+        assert torch.equal(t.view(torch.uint8)[first], t.view(torch.uint8)[last])
+    assert torch.equal(*outs) and bool(outs[0].float().abs().sum() > 0)
+    assert not cache.k.view(torch.uint8)[3:pages - 3:997].any() and cache.status() == 0
+
+
+def test_two_layers_in_one_graph_and_two_graphs_in_turn():
+    """Graphs that share a memory pool, replayed in turn, each with the other's contents in between."""
+    s = Setup((128, 128), 2, [1, 1, 1], [65, 300, 1], seed=3).fill()
+    big = Setup((128, 128), 2, [40, 3], [140, 90], seed=4).fill()
+    qs, qb = s.rows(8, 128, BF16, 2.0).to(DEV), big.rows(8, 128, BF16, 2.0).to(DEV)
+    want = [s.cache.attend(qs, s.batch), big.cache.attend(qb, big.batch)]
+    stream, pool, graphs, outs = torch.cuda.Stream(), torch.cuda.graph_pool_handle(), [], []
+    stream.wait_stream(torch.cuda.current_stream())
+    for setup, q in ((s, qs), (big, qb)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool, stream=stream):
+            outs.append([setup.cache.attend(q, setup.batch) for _ in range(2)])
+        graphs.append(graph)
+    for _ in range(3):
+        for graph, pair, w in zip(graphs, outs, want):
+            for o in pair:
+                o.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(o, w) for o in pair)
+
+
 # ---- the three together, streams, graphs, refusals ------------------------------------------------------------
 
 @pytest.mark.parametrize("dims,layout", [((128, 128), "half"), ((192, 128), "interleaved")])
