@@ -34,7 +34,7 @@ struct AttendArgs {
     int64_t qt, qh;        // strides of q, elements
     int heads, group, window;
     float scale;           // times log2(e): the softmax's exponentials are powers of two
-    int part_rows;         // rows of a partial sum: of a call of few rows all of them, else PR_ROWS
+    int part_rows;         // rows of a partial sum (few rows: all that share a key)
     int4* heads_of;        // [pieces]: what a piece leaves unfinished (each kernel's own record)
     float* part;           // [pieces][2] partial sums
 };

@@ -942,7 +942,6 @@ size_t prompt_workspace(int dv)
 
 cudaError_t launch_prompt(AttendArgs p, void* workspace, bool bf16, cudaStream_t st)
 {
-    p.part_rows = PR_ROWS;
     p.heads_of = static_cast<int4*>(workspace);
     p.part = reinterpret_cast<float*>(p.heads_of + num_sms());
     const int dk = p.c.key_dim;
