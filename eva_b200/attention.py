@@ -245,7 +245,7 @@ class PagedBatch:
     The tensors stay the caller's: a captured step is replayed with new contents in them (max_q and the table's width
     bound what they may hold). A padding sequence has length 0 (its rows come out zero, nothing is appended). What does
     not fit (page ids outside the cache, lengths beyond the table, rows out of order) sets STATUS_BAD_BATCH in the cache's
-    status and is left out. A page that stands twice among those that one call appends to (of two sequences, or of one) is the
+    status and is left out. To a sequence without rows an append does nothing: its pages may be another's. A page that stands twice among those that one call appends to (of two sequences, or of one) is the
     caller's error: its contents are then undefined."""
 
     def __init__(self, q_start, seq_lens, table, max_q):

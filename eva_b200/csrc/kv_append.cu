@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, STAGED ? (DK == 64 ? 4 : DK
     const KvSeq s = kv_seq(p.b, b, p.c.status);
     const int first = max(s.ctx, 0);
     const int base = (first / KV_BLOCK + static_cast<int>(blockIdx.x - b * p.blocks)) * KV_BLOCK;
-    if (base >= s.len) return;
+    if (s.n == 0 || base >= s.len) return;   // (a sequence without new rows may share its last page with one that appends)
     const int page = kv_page(p.c, p.b, b, base / KV_PAGE, p.c.status);
     if (page < 0) return;
     const int lo = max(first - base, 0), hi = min(s.len - base, KV_BLOCK), at = base % KV_PAGE;

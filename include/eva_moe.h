@@ -353,7 +353,7 @@ typedef struct EvaKvBatch {
  * the pages. A block of 16 tokens has the smallest power of two that brings all its values into e4m3's range;
  * when a later token raises it, the block's older codes are rescaled. A token of whose key or value an element
  * is not finite gets a NaN key (its values: 0 there), so that exactly the rows that see it become NaN. Everything
- * but the blocks' codes and scales stays as it was. No page may stand twice among those that a call appends to
+ * but the blocks' codes and scales stays as it was; a sequence without rows has no such block. No page may stand twice among those that a call appends to
  * (its contents would be undefined).
  * k: [tokens][kv_heads][key_dim], v: [tokens][kv_heads][value_dim], F16 or BF16, strides in elements. */
 int eva_kv_append(const EvaKvCache* cache, const EvaKvBatch* batch, const EvaRotary* rotary, const void* k,

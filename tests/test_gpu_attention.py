@@ -257,6 +257,27 @@ def test_append_of_rows_anywhere_in_memory(dims, layout, rot, offset, kv_heads):
         assert all(torch.equal(a, b) for a, b in zip(got, want)), shift
 
 
+@pytest.mark.parametrize("dims", DIMS)
+@pytest.mark.parametrize("size", [0.02, 200.0])
+def test_append_beside_sequences_without_new_rows(dims, size):
+    """Sequences that bring no row of their own touch nothing: many of them share the part-full page that one appends to (a forked
+    prefix), one has no page at all, and the bytes are those of the append alone; at the larger size its scales grow."""
+    idle, n, new = 60, 37, 3
+    s = Setup(dims, 3, [new], [n + new], seed=9).fill()
+    k, v = s.rows(3, dims[0], BF16, size), s.rows(3, dims[1], BF16, size)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)   # noqa: E731
+    page = s.table[0][0]
+    start = [0] * (idle + 1) + [new] * (idle + 2)
+    lens = [n] * idle + [n + new] + [n] * idle + [n]
+    table = [[page]] * (2 * idle + 1) + [[-1]]
+    s.cache.append(k.to(DEV), v.to(DEV), PagedBatch(i32(start), i32(lens), i32(table), 64))
+    A.append(s.host, k.double(), v.double(), s.start, s.lens, s.table)
+    for name in ("k", "v"):
+        _same_bytes(getattr(s.cache, name), s.host[name], name)
+        assert torch.equal(getattr(s.cache, name + "_scale").view(torch.uint8), s.bytes_of(name + "s"))
+    assert s.cache.status() == 0
+
+
 def test_append_of_values_that_are_not_finite():
     """Such a token gets a NaN key; its block's other tokens and scales are as if it were not there, and so are its finite values."""
     s = Setup((64, 64), 2, [40], [70], seed=2)
