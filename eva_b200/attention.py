@@ -449,7 +449,8 @@ class PagedAttention:
 
     def forward(self, h, batch, positions, *, out_f32=None):
         """h: BF16 [tokens, hidden], the batch's new tokens; positions: int32 or int64 [tokens], each token's place in its
-        sequence. Returns BF16 [tokens, hidden], in FP32 into out_f32 where that is given."""
+        sequence. Returns BF16 [tokens, hidden], in FP32 into out_f32 where that is given. Rows of no sequence (behind the last one,
+        or of one that does not fit the batch) are zero."""
         c = self.cache
         if h.ndim != 2 or h.shape[1] != self.hidden or h.dtype != _BF16 or h.device != c.device:
             raise ValueError(f"h must be BF16 [tokens, {self.hidden}] on {c.device}")
@@ -461,7 +462,8 @@ class PagedAttention:
         if self.rotary is not None:
             q = self.rotary.apply(q, positions, out=q)
         c.append(k, v, batch, rotary=self.rotary)
-        y = c.attend(q, batch, scale=self.scale, window=self.window).flatten(1) @ self.wo.T
+        o = q.new_zeros((h.shape[0], self.heads, c.value_dim))   # attend leaves rows of no sequence as they were
+        y = c.attend(q, batch, scale=self.scale, window=self.window, out=o).flatten(1) @ self.wo.T
         return y if out_f32 is None else out_f32.copy_(y)
 
     __call__ = forward

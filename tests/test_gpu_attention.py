@@ -703,6 +703,76 @@ def test_layer_stack_with_attention(oracle):
         MoEStack(stack.layers, norms, attention=att)
 
 
+def _leave_in_memory(value, *shapes):
+    """Freed blocks full of `value` where the next tensors of these shapes are likely to lie."""
+    blocks = [torch.full(shape, value, dtype=BF16, device=DEV) for shape in shapes for _ in range(40)]
+    torch.cuda.synchronize()
+    del blocks
+
+
+@pytest.mark.parametrize("new,lens", [([1, 1, 1], [30, 70, 5]), ([40, 3, 1], [60, 70, 5])])
+def test_attention_half_gives_zeros_to_rows_of_no_sequence(new, lens):
+    """Rows behind the last sequence, and those of a sequence that does not fit its batch, come out of the layer half as
+    zeros whatever the memory held before; the other rows' bits do not depend on it."""
+    from eva_b200.attention import make_attention
+    heads, dv, T = 4, 128, sum(new) + 5
+    half = make_attention(1, 256, heads, 2, 128, dv, 8, seed=1)[0]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)   # noqa: E731
+    start = [0, new[0], new[0] + new[1], sum(new)]
+    batch = PagedBatch(i32(start), i32(lens), i32([[0, 1], [2, 3], [77, 77]]), max(new))
+    h = torch.randn(T, 256, generator=torch.Generator().manual_seed(2)).to(BF16).to(DEV)
+    positions = torch.zeros(T, dtype=torch.int64, device=DEV)
+    batch.seq_lens[2] = 129   # longer than its pages
+    seen = []
+    for value in (math.nan, 3.0, 0.0):
+        _leave_in_memory(value, (T, heads, dv), (T, 256), (T, heads * 128 + 512))
+        out32 = torch.empty(T, 256, device=DEV)
+        seen.append((half.forward(h, batch, positions), half.forward(h, batch, positions, out_f32=out32).clone()))
+        assert half.cache.status() == _lib.STATUS_BAD_BATCH
+        half.cache.clear_status()
+        for y in seen[-1]:
+            assert bool(y.isfinite().all()) and not y[start[2]:].any() and bool(y[:start[2]].any(1).all())
+    for other in seen[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(seen[0], other))
+
+
+def test_layer_stack_of_a_padded_step():
+    """A step of three rows of which two belong to sequences, captured and replayed with the third left over: what memory held before
+    reaches no row."""
+    from eva_b200 import config as C
+    from eva_b200.attention import make_attention
+    from eva_b200.experts import make_layer
+    from eva_b200.runner import EvaMoE
+    from eva_b200.stack import MoEStack, make_norms
+    cfg = C.MoEConfig("small", hidden=512, inter=256, n_experts=16, topk=4, router="sigmoid", n_group=4, topk_group=2,
+                      route_scale=2.5, norm_topk=True, shared_inter=384, bits=3, shared_bits=4)
+    att = make_attention(2, cfg.hidden, 4, 2, 128, 128, 6, seed=3)
+    norms, anorms = make_norms(2, cfg.hidden, DEV, seed=4), make_norms(2, cfg.hidden, DEV, seed=5)[:2]
+    stack = MoEStack([EvaMoE(make_layer(cfg, "cpu", seed=50 + i).to(DEV), max_rows=16) for i in range(2)], norms,
+                     attention=att, attention_norms=anorms)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)   # noqa: E731
+    batch, pos = PagedBatch(i32([0, 1, 2, 3]), i32([7, 9, 1]), i32([[4], [1], [2]]), 1), torch.zeros(3, dtype=torch.int64, device=DEV)
+    x = torch.randn(3, cfg.hidden, generator=torch.Generator().manual_seed(1)).to(BF16).to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        stack.forward(x, batch=batch, positions=pos)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = stack.forward(x, batch=batch, positions=pos)
+    outs = []
+    for third in (math.nan, 1.0):
+        batch.q_start.copy_(i32([0, 1, 2, 3]))
+        x[2] = third
+        graph.replay()   # the third row's sequence is there: its contents stay in the graph's memory
+        batch.q_start.copy_(i32([0, 1, 2, 2]))
+        x[2] = 0.5
+        graph.replay()
+        outs.append(out.clone())
+    assert bool(outs[0].isfinite().all()) and torch.equal(*outs)
+
+
 def test_refusals():
     s = Setup((64, 64), 2, [1, 1], [10, 20]).fill()
     q, k = s.rows(4, 64, BF16).to(DEV), s.rows(2, 64, BF16).to(DEV)
