@@ -416,7 +416,7 @@ class PagedKVCache:
         return k, v.transpose(2, 3)
 
     def status(self) -> int:
-        """The device status bits (reads them back: synchronises the host)."""
+        """The device status bits (reads them back: synchronises the host). They stay until clear_status(), whatever later calls do."""
         return int(self._status.item())
 
     def clear_status(self) -> None:

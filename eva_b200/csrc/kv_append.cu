@@ -188,7 +188,10 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, STAGED ? (DK == 64 ? 4 : DK
         const T* kp = static_cast<const T*>(p.k) + h * p.kh + tok0 * p.kt;
         const T* vp = static_cast<const T*>(p.v) + h * p.vh + tok0 * p.vt;
         if constexpr (STAGED) {
-            mbar_wait(&bars[warp], phase, p.c.status);
+            if (!copies_arrived(&bars[warp], phase, p.c.status)) {   // the block's older tokens stay as they were
+                copies_late(&bars[warp], phase, p.c.status);
+                return false;
+            }
             phase ^= 1;
             kp = staged_k;
             vp = staged_v;
@@ -391,12 +394,11 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, STAGED ? (DK == 64 ? 4 : DK
             *ks = static_cast<uint8_t>(ke);
             *vs = static_cast<uint8_t>(ve);
         }
+        return true;
     };
     const bool fills = lo == 0 && hi == KV_BLOCK;
-    for (int h = warp; h < p.c.kv_heads; h += nwarps) {
-        if (fills) one_head(std::true_type{}, h);
-        else one_head(std::false_type{}, h);
-    }
+    for (int h = warp; h < p.c.kv_heads; h += nwarps)
+        if (!(fills ? one_head(std::true_type{}, h) : one_head(std::false_type{}, h))) return;
 }
 
 template <typename T, int DK, int DV, int KEYS> static cudaError_t append_staged(const AppendArgs& p, unsigned grid, dim3 threads, cudaStream_t st)

@@ -299,7 +299,11 @@ __global__ void __launch_bounds__(DecCfg<DK, DV>::W * 32, 1) kv_decode_kernel(At
             if (cur.tok >= 0) {
                 const uint8_t* K = ring + slot * C::STAGE;
                 const uint8_t* V = K + C::KB;
-                mbar_wait(&bars[warp][slot], phase >> slot & 1, p.c.status);
+                if (!copies_arrived(&bars[warp][slot], phase >> slot & 1, p.c.status)) {
+                    copies_late(&bars[warp][slot], phase >> slot & 1, p.c.status);
+                    if (at + 1 < end && nxt.tok >= 0) copies_late(&bars[warp][slot ^ 1], phase >> (slot ^ 1) & 1, p.c.status);
+                    break;   // the item stays unfinished
+                }
                 phase ^= 1u << slot;
                 float sc[NT][4][4];   // product e: tokens t0 + 4 e + (0, 0, 2, 2), rows 2 quad + (0, 1, 0, 1)
 #pragma unroll

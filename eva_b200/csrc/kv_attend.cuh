@@ -86,6 +86,33 @@ __device__ __forceinline__ float ex2(float x)
     return y;
 }
 
+// Bounded wait for bulk copies that have not arrived yet; sets EVA_STATUS_TIMEOUT where it gives up. The status word is the cache's and
+// outlives the launch: a bit that is there already does not end the wait as in mbar_wait, but makes the limit 20 ms, a
+// thousand times what a copy takes, so that a launch of many waves does not spend the whole limit in each.
+static __device__ __noinline__ bool copies_late(uint64_t* bar, uint32_t parity, int* status)
+{
+    const uint64_t t0 = globaltimer();
+    uint64_t limit = 0;
+    for (uint32_t i = 1;; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 31) != 0) continue;
+        if (limit == 0) limit = ld_volatile(status) & ST_TIMEOUT ? WAIT_LIMIT_NS / 100 : WAIT_LIMIT_NS;
+        if (globaltimer() - t0 > limit) {
+            atomicOr(status, ST_TIMEOUT);
+            return false;
+        }
+    }
+}
+
+// Whether a warp's copies arrived (the whole warp asks and gets one answer). If not, the caller stores nothing that comes from them, waits
+// once more for what it has in flight, and leaves.
+__device__ __forceinline__ bool copies_arrived(uint64_t* bar, uint32_t parity, int* status)
+{
+    bool ok = mbar_try_wait(bar, parity);
+    if (!ok) ok = copies_late(bar, parity, status);
+    return __all_sync(0xffffffffu, ok);
+}
+
 // Joins a row's partial sums, by a warp, eight at a time (their loads do not wait for one another): maximum at part(k)[im], sum at
 // part(k)[is], output from part(k) + io; every lane gets the joint maximum and sum, and of the output dimensions
 // 4 lane .. 4 lane + 3 (modulo DV).

@@ -293,7 +293,9 @@ int eva_rmsnorm_residual(int32_t H, int32_t M, float* resid, const float* add, c
 /* ---- attention between the MoE layers: rotary positions, paged 8-bit key/value cache ------------------
  * The reference's attention half of a layer (runtime/ds41/model.py:566-937 `Attention`, rotary tails
  * runtime/ds41/attn_cuda.py:22) keeps its cache in 4 bits behind an index; these operators give the
- * layer stack plain causal attention over a paged 8-bit cache. Nothing here synchronises the host. */
+ * layer stack plain causal attention over a paged 8-bit cache. Nothing here synchronises the host.
+ * EVA_STATUS_TIMEOUT in the cache's status: a call gave up waiting for its own copies. Its outputs, or the blocks that it appended to, are not
+ * complete (what an append had not got to stays as it was). The bit stays until it is cleared, and does not change what later calls do. */
 
 /* element types of activations (EVA_DTYPE_F16 and _BF16 are the values of x_is_bf16 above) */
 #define EVA_DTYPE_F16 0

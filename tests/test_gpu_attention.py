@@ -613,6 +613,25 @@ def test_two_streams_at_once():
         assert all(torch.equal(g, want[i]) for g in got[i])
 
 
+@pytest.mark.parametrize("new,lens", [([1] * 40, [3000 + 50 * i for i in range(40)])])
+def test_a_timeout_of_an_earlier_call_does_not_spoil_later_ones(new, lens):
+    """The status word keeps a timeout until it is cleared; calls in between give what they give without it (more pages than any cache
+    level near the SMs holds, so that waits take their time), and leave the bit alone."""
+    s = Setup((128, 128), 8, new, lens, seed=2).fill()
+    k, v, q = (t.to(DEV) for t in (s.rows(8, 128, BF16), s.rows(8, 128, BF16), s.rows(32, 128, BF16, 2.0)))
+    names = ("k", "v", "k_scale", "v_scale")
+    before = [getattr(s.cache, n).view(torch.uint8).clone() for n in names]
+    seen = []
+    for bits in (0, _lib.STATUS_TIMEOUT):
+        for n, b in zip(names, before):
+            getattr(s.cache, n).view(torch.uint8).copy_(b)
+        s.cache._status.fill_(bits)
+        s.cache.append(k, v, s.batch)
+        seen.append([s.cache.attend(q, s.batch) for _ in range(3)] + [getattr(s.cache, n).view(torch.uint8).clone() for n in names])
+        assert s.cache.status() == bits
+    assert all(torch.equal(a, b) for a, b in zip(*seen))
+
+
 @pytest.mark.parametrize("new,lens", [([1, 1], [100, 200]), ([70, 40], [100, 200])])
 def test_a_batch_that_does_not_fit_is_flagged_and_left_out(new, lens):
     """Page ids outside the cache, lengths beyond the table and row starts beyond the rows are bounded before any access
