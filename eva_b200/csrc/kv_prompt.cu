@@ -59,12 +59,16 @@ struct PrBars {
     uint64_t sready[2][2], pready[2][2], pvdone[2][2], qfull[2];   // [tile][step & 1]
     uint64_t mready[2][4][2];                                   // [tile][warp][step & 1]
     uint64_t scfull[PR_SCALES], segfull[PR_SEGS], segempty[PR_SEGS];
-    uint32_t tmem;
+    uint64_t pair[2][4];                                        // [tile][warp]: both parities' warps are here
+    uint64_t mmadone[2];                                        // [tile], of a CTA that gave up
+    uint32_t tmem, copied_k, copied_v;                          // steps whose codes the copying warp has asked for
+    int gave_up;
 };
 
 // mbar_wait that sleeps in the barrier unit for up to 100 us a try: many warps wait here at any time, and short tries would
 // fill the queue to shared memory, exponentials and tensor memory that the others work through. The loop for a wait
-// that is not over by then stays out of line.
+// that is not over by then stays out of line. A wait of the CTA that gives up ends the others of that CTA, and no more: the status
+// word is the cache's, and a bit that an earlier launch left in it says nothing of this one.
 __device__ __forceinline__ bool try_wait_long(uint64_t* bar, uint32_t parity)
 {
     uint32_t ok;
@@ -76,19 +80,24 @@ __device__ __forceinline__ bool try_wait_long(uint64_t* bar, uint32_t parity)
     return ok != 0;
 }
 
-__device__ __noinline__ void wait_more(uint64_t* bar, uint32_t parity, int* status)
+__device__ __noinline__ bool wait_more(uint64_t* bar, uint32_t parity, int* gave_up, int* status, uint64_t limit)
 {
     const uint64_t t0 = globaltimer();
-    while (!try_wait_long(bar, parity))
-        if (globaltimer() - t0 > WAIT_LIMIT_NS || (ld_volatile(status) & ST_TIMEOUT)) {
+    while (ld_volatile(gave_up) == 0) {
+        if (try_wait_long(bar, parity)) return true;
+        if (globaltimer() - t0 > limit) {
+            *static_cast<volatile int*>(gave_up) = 1;
             atomicOr(status, ST_TIMEOUT);
-            return;
         }
+    }
+    return false;
 }
 
-__device__ __forceinline__ void wait_on(uint64_t* bar, uint32_t parity, int* status)
+// Before a CTA that gave up leaves: what it has in flight, whatever the others do.
+__device__ __noinline__ void wait_for_own(uint64_t* bar, uint32_t parity)
 {
-    if (!try_wait_long(bar, parity)) wait_more(bar, parity, status);
+    const uint64_t t0 = globaltimer();
+    while (!try_wait_long(bar, parity) && globaltimer() - t0 <= WAIT_LIMIT_NS) {}
 }
 
 // Row block qb of a sequence: its rows' tokens, the token range they see and the steps over it.
@@ -409,12 +418,15 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
                 for (int k = 0; k < 4; ++k) mbar_init(&B.mready[i][k][j], 1);
             }
             mbar_init(&B.qfull[i], 8);
+            mbar_init(&B.mmadone[i], 1);
+            for (int k = 0; k < 4; ++k) mbar_init(&B.pair[i][k], 2);
         }
         for (int i = 0; i < PR_SCALES; ++i) mbar_init(&B.scfull[i], 1);
         for (int i = 0; i < PR_SEGS; ++i) {
             mbar_init(&B.segfull[i], 1);
             mbar_init(&B.segempty[i], PR_SOFT + PR_CONV + 3);
         }
+        B.gave_up = 0;
         fence_barrier_init();
     }
     if (warp == PR_MMA) tmem_alloc(&B.tmem, 512);
@@ -494,9 +506,16 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = B.tmem;
-    // Segment i of the piece, for every lane of a warp (or the one thread that calls)
+    // ok: no wait of the thread has given up. What a wait was for is garbage then, but harmless: warps vote on ok once a step, before
+    // anything leaves the CTA, and end.
+    bool ok = true;
+    auto wait_on = [&](uint64_t* bar, uint32_t parity) {
+        if (!try_wait_long(bar, parity)) ok &= wait_more(bar, parity, &B.gave_up, status, WAIT_LIMIT_NS);
+    };
+    auto all_ok = [&] { return __all_sync(0xffffffffu, ok) != 0; };
+    // Segment i of the piece, for every lane of a warp
     auto segment = [&](uint32_t i) -> const PrSeg& {
-        wait_on(&B.segfull[i % PR_SEGS], (i / PR_SEGS) & 1, status);
+        wait_on(&B.segfull[i % PR_SEGS], (i / PR_SEGS) & 1);
         return segs[i % PR_SEGS];
     };
 
@@ -506,12 +525,17 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
         const int tile = warp >> 3, odd_steps = (warp >> 2) & 1, quad = warp & 3, row = quad * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
         const uint32_t ts = tmem + lanes + tile * PR_TILE + odd_steps * PR_STEP, to = tmem + lanes + 2 * PR_TILE + tile * DV;
-        uint32_t it = 0;                      // steps so far
+        uint32_t it = 0, met = 0;             // steps so far; meetings with the other parity's warp
+        auto meet = [&] {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&B.pair[tile][quad]);
+            wait_on(&B.pair[tile][quad], met++ & 1);
+        };
         if (threadIdx.x == 0) p.heads_of[blockIdx.x] = make_int4(-1, 0, 0, 0);
         for (uint32_t seg = 0;; ++seg) {
             const PrSeg& g = segment(seg);
             const int t0 = g.t0, t1 = g.t1;
-            if (t1 == 0) break;
+            if (!all_ok() || t1 == 0) break;
             const int qb = g.qb, h = g.h, rows = g.s.n, row0 = g.s.row0;
             const int r = qb * PR_ROWS + tile * PR_TILE + row, tok = r / p.group, qh = h * p.group + (r - tok * p.group);
             const bool in = tok < rows, whole = g.first && g.after == 0;
@@ -582,7 +606,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&B.qfull[tile]);
             }
-            asm volatile("bar.sync %0, 64;" ::"r"(1 + tile * 4 + quad) : "memory");
+            meet();
             const float c = qscale[tile][row];
             const int all_hi = __reduce_min_sync(0xffffffffu, hi), all_lo = __reduce_max_sync(0xffffffffu, lo);
             const uint32_t first = it, end = it + (t1 - t0);
@@ -592,13 +616,13 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
                 const float4* sc = scales[it % PR_SCALES];
                 const int tok0 = (t0 + static_cast<int>(it - first)) * PR_STEP;
                 const bool part_seen = tok0 + PR_STEP > all_hi || tok0 < all_lo;
-                wait_on(&B.scfull[it % PR_SCALES], (it / PR_SCALES) & 1, status);
-                wait_on(&B.sready[tile][odd_steps], (it >> 1) & 1, status);
+                wait_on(&B.scfull[it % PR_SCALES], (it / PR_SCALES) & 1);
+                wait_on(&B.sready[tile][odd_steps], (it >> 1) & 1);
                 tc_fence_after();
                 const float mx = part_seen ? pr_max_masked(ts, sc, c, lo - tok0, hi - tok0) : pr_max(ts, sc, c);
                 float was = -INFINITY;
                 if (it > first) {
-                    wait_on(&B.mready[tile][quad][odd_steps ^ 1], ((it - 1) >> 1) & 1, status);
+                    wait_on(&B.mready[tile][quad][odd_steps ^ 1], ((it - 1) >> 1) & 1);
                     was = top[tile][row];
                 }
                 const bool grow = mx > was + PR_SLACK || (was == -INFINITY && mx > was);
@@ -608,7 +632,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
                 if (lane == 0) mbar_arrive(&B.mready[tile][quad][odd_steps]);
                 if (it > first && __any_sync(0xffffffffu, grow)) {
                     const float fall = grow ? ex2(was - now) : 1.0f;
-                    wait_on(&B.pvdone[tile][odd_steps ^ 1], ((it - 1) >> 1) & 1, status);
+                    wait_on(&B.pvdone[tile][odd_steps ^ 1], ((it - 1) >> 1) & 1);
                     tc_fence_after();
                     pr_rescale<DV>(to, fall);
                 }
@@ -623,16 +647,18 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&B.pready[tile][odd_steps]);
+                if (!all_ok()) break;
             }
             it = end;
             // both parities' sums, then half of the output each
             sums[tile][odd_steps][row] = make_float2(m, l);
-            asm volatile("bar.sync %0, 64;" ::"r"(1 + tile * 4 + quad) : "memory");
+            meet();
             const float2 s0 = sums[tile][0][row], s1 = sums[tile][1][row];
             m = fmaxf(s0.x, s1.x);
             l = s0.y * (s0.x == -INFINITY ? 1.0f : ex2(s0.x - m)) + s1.y * (s1.x == -INFINITY ? 1.0f : ex2(s1.x - m));
-            wait_on(&B.pvdone[tile][(it - 1) & 1], ((it - 1) >> 1) & 1, status);
+            wait_on(&B.pvdone[tile][(it - 1) & 1], ((it - 1) >> 1) & 1);
             tc_fence_after();
+            if (!all_ok()) break;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const int pr = tile * PR_TILE + row;
             if (!whole && in && odd_steps == 0) {
@@ -672,14 +698,14 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
         for (uint32_t seg = 0;; ++seg) {
             const PrSeg& g = segment(seg);
             const int t0 = g.t0, t1 = g.t1, len = g.s.len;
-            if (t1 == 0) break;
+            if (!all_ok() || t1 == 0) break;
             __syncwarp();
             if (lane == 0) mbar_arrive(&B.segempty[seg % PR_SEGS]);
 #pragma unroll 1
             for (int t = t0; t < t1; ++t, ++it) {
                 const uint32_t ks = it % C::KST, vs = it % C::VST, rs = it % C::RST;
-                wait_on(&B.rkfull[rs], (it / C::RST) & 1, status);
-                wait_on(&B.kempty[ks], ((it / C::KST) & 1) ^ 1, status);
+                wait_on(&B.rkfull[rs], (it / C::RST) & 1);
+                wait_on(&B.kempty[ks], ((it / C::KST) & 1) ^ 1);
                 {
                     const uint32_t src = smem_u32(rawk) + rs * C::RK + sub * DK + unit * 16, dst = sk + ks * C::K;
                     uint4 c[C::KC][2];
@@ -703,8 +729,8 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
                     mbar_arrive(&B.kfull[ks]);
                     mbar_arrive(&B.rkempty[rs]);
                 }
-                wait_on(&B.rvfull[rs], (it / C::RST) & 1, status);
-                wait_on(&B.vempty[vs], ((it / C::VST) & 1) ^ 1, status);
+                wait_on(&B.rvfull[rs], (it / C::RST) & 1);
+                wait_on(&B.vempty[vs], ((it / C::VST) & 1) ^ 1);
                 {
                     const uint32_t src = smem_u32(rawv) + rs * C::RV + sub * KV_PAGE + unit * 16, dst = sv + vs * C::V;
                     uint4 c[DV / 32];
@@ -741,6 +767,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
                     mbar_arrive(&B.vfull[vs]);
                     mbar_arrive(&B.rvempty[rs]);
                 }
+                if (!all_ok()) break;
             }
         }
     } else {
@@ -757,17 +784,17 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
             for (uint32_t seg = 0;; ++seg) {
                 const PrSeg& g = segment(seg);
                 const int n = g.t1 - g.t0;
-                if (g.t1 == 0) break;
+                if (!all_ok() || g.t1 == 0) break;
                 __syncwarp();
                 if (lead) mbar_arrive(&B.segempty[seg % PR_SEGS]);
-                wait_on(&B.qfull[tile], seg & 1, status);
+                wait_on(&B.qfull[tile], seg & 1);
                 // scores run two steps ahead of the weights' products
                 it -= 2;
 #pragma unroll 1
                 for (int j = -2; j < n; ++j, ++it) {
                     if (j >= 0) {
-                        wait_on(&B.vfull[it % C::VST], (it / C::VST) & 1, status);
-                        wait_on(&B.pready[tile][it & 1], (it >> 1) & 1, status);
+                        wait_on(&B.vfull[it % C::VST], (it / C::VST) & 1);
+                        wait_on(&B.pready[tile][it & 1], (it >> 1) & 1);
                         tc_fence_after();
                         uint64_t b = umma_desc_sw128(sv + (it % C::VST) * C::V);
                         uint32_t a = ts + (it & 1) * PR_STEP;
@@ -778,7 +805,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
                     }
                     if (j + 2 < n) {
                         const uint32_t ahead = it + 2, ks = ahead % C::KST;
-                        wait_on(&B.kfull[ks], (ahead / C::KST) & 1, status);
+                        wait_on(&B.kfull[ks], (ahead / C::KST) & 1);
                         tc_fence_after();
                         uint64_t a = dq, b = umma_desc_sw128(sk + ks * C::K);
 #pragma unroll 1
@@ -790,16 +817,17 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
                         umma_commit_if(lead, &B.sready[tile][it & 1]);
                         umma_commit_if(lead, &B.kempty[ks]);
                     }
+                    if (!all_ok()) break;
                 }
             }
         } else if (warp == PR_MMA + 2) {
             // ---- copies: a step's page into shared memory as it is, and its blocks' scales
             int pages = -1, pages_at = -64, pages_b = -1;   // lane l: page pages_at + l of sequence pages_b
-            uint32_t it = 0;
+            uint32_t it = 0, half = 0;
             for (uint32_t seg = 0;; ++seg) {
                 const PrSeg& g = segment(seg);
                 const int b = g.b, h = g.h, t0 = g.t0, t1 = g.t1, len = g.s.len;
-                if (t1 == 0) break;
+                if (!all_ok() || t1 == 0) break;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&B.segempty[seg % PR_SEGS]);
 #pragma unroll 1
@@ -821,7 +849,8 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
                         mine = make_float4(kv_scale(ks), v.e, v.inv, v.less);
                     }
                     if (__any_sync(0xffffffffu, mine.w != 1.0f)) mine.w = -mine.w;   // a step with such a block: pr_weights_masked
-                    wait_on(&B.rkempty[rs], par, status);
+                    wait_on(&B.rkempty[rs], par);
+                    if (!all_ok()) break;   // the stage is not free: nothing is copied into it
                     if (page < 0) {
                         for (int i = lane; i < C::RK / 16; i += 32) st_shared16(smem_u32(rawk) + rs * C::RK + i * 16, make_uint4(0, 0, 0, 0));
                         __syncwarp();
@@ -830,7 +859,11 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
                         mbar_arrive_expect_tx(&B.rkfull[rs], page >= 0 ? C::RK : 0);
                         if (page >= 0) bulk_g2s(rawk + rs * C::RK, static_cast<const uint8_t*>(p.c.k) + ph * C::RK, C::RK, &B.rkfull[rs]);
                     }
-                    wait_on(&B.rvempty[rs], par, status);
+                    wait_on(&B.rvempty[rs], par);
+                    if (!all_ok()) {
+                        half = 1;
+                        break;
+                    }
                     if (page < 0)
                         for (int i = lane; i < C::RV / 16; i += 32) st_shared16(smem_u32(rawv) + rs * C::RV + i * 16, make_uint4(0, 0, 0, 0));
                     if (lane < 4) scales[it % PR_SCALES][lane] = mine;
@@ -843,12 +876,16 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
                     __syncwarp();
                 }
             }
+            if (lane == 0) B.copied_k = it + half, B.copied_v = it;
         } else if (warp == PR_MMA + 1 && lane == 0) {
             // ---- the segments of the piece
             int b = place.b, h = place.h, qb = place.qb, off = place.off, left = place.left, done = 0;
             KvSeq s = left > 0 ? kv_seq(p.b, b, status) : KvSeq{0, 0, 0, 0};
             for (uint32_t i = 0;; ++i) {
-                wait_on(&B.segempty[i % PR_SEGS], ((i / PR_SEGS) & 1) ^ 1, status);
+                // (the others may be a whole segment's steps away)
+                if (!try_wait_long(&B.segempty[i % PR_SEGS], ((i / PR_SEGS) & 1) ^ 1) &&
+                    !wait_more(&B.segempty[i % PR_SEGS], ((i / PR_SEGS) & 1) ^ 1, &B.gave_up, status, WAIT_LIMIT_NS + 20000ull * done))
+                    break;
                 PrSeg& g = segs[i % PR_SEGS];
                 PrItem item{};
                 int n = 0, lo = 0, hi = 0, after = 0;
@@ -896,6 +933,20 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if (B.gave_up) {   // (what this needs is kept in shared memory: values held in registers until here cost the loops above 7 %)
+        if (warp == PR_MMA || warp == PR_MMA + 3) {
+            uint64_t* const bar = &B.mmadone[warp == PR_MMA ? 0 : 1];
+            umma_commit_if(elect_one(), bar);   // the same lane as before
+            wait_for_own(bar, 0);
+        } else if (warp == PR_MMA + 2) {
+            const uint32_t k = B.copied_k, v = B.copied_v;
+            for (uint32_t i = 1; i <= C::RST; ++i) {
+                if (k >= i) wait_for_own(&B.rkfull[(k - i) % C::RST], ((k - i) / C::RST) & 1);
+                if (v >= i) wait_for_own(&B.rvfull[(v - i) % C::RST], ((v - i) / C::RST) & 1);
+            }
+        }
+        __syncthreads();
+    }
     if (warp == PR_MMA) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);

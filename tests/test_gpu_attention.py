@@ -613,7 +613,7 @@ def test_two_streams_at_once():
         assert all(torch.equal(g, want[i]) for g in got[i])
 
 
-@pytest.mark.parametrize("new,lens", [([1] * 40, [3000 + 50 * i for i in range(40)])])
+@pytest.mark.parametrize("new,lens", [([1] * 40, [3000 + 50 * i for i in range(40)]), ([300, 70], [2000, 5000])])
 def test_a_timeout_of_an_earlier_call_does_not_spoil_later_ones(new, lens):
     """The status word keeps a timeout until it is cleared; calls in between give what they give without it (more pages than any cache
     level near the SMs holds, so that waits take their time), and leave the bit alone."""
