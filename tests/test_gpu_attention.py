@@ -365,6 +365,93 @@ def test_attention_of_very_large_and_small_queries(size, new, lens):
         assert bool(out.isfinite().all()) and float((out.cpu().double() - ref).abs().median()) < 2.0**-8
 
 
+def _tokens(s, b, h):
+    """Keys and values of sequence b and head h as the cache's codes and scales give them, float64 [length, dim]."""
+    two = lambda e: torch.exp2(e.double()).repeat_interleave(A.BLOCK, -1)   # noqa: E731
+    pages = torch.tensor(s.table[b])
+    K = s.host["k"][pages, h].double() * two(s.host["ks"][pages, h])[..., None]
+    V = s.host["v"][pages, h].double() * two(s.host["vs"][pages, h])[:, None, :]
+    return K.flatten(0, 1)[:s.lens[b]], V.transpose(1, 2).flatten(0, 1)[:s.lens[b]]
+
+
+@pytest.mark.parametrize("new,lens", [([1, 1], [500, 70]), ([100], [100]), ([70, 60], [800, 300])])
+@pytest.mark.parametrize("size", [1e4, 1e30])
+def test_rows_of_large_scores_are_the_value_of_the_largest(size, new, lens):
+    """A score is off by key_dim * 2^-23 of the sum of its products' sizes at most, and by 2^-25 of the query's largest element times the
+    sum of the key's (its rounding to 16 bits). A row whose largest score leads by twice that and 20 more has all its weight on one
+    token, but for 2e-9 of each other one: its value to half a step of the output's type and 2^-11 (the weight's 16 bits)."""
+    s = Setup((64, 64), 2, new, lens, seed=4).fill()
+    q = s.rows(4, 64, BF16, size)
+    out = s.cache.attend(q.to(DEV), s.batch).cpu().double()
+    clear = 0
+    for b, n in enumerate(lens):
+        for h in range(4):
+            K, V = _tokens(s, b, h // 2)
+            for i in range(new[b]):
+                pos, row = n - new[b] + i, s.start[b] + i
+                Q = q[row, h].double()
+                x = 0.125 * K[:pos + 1] @ Q
+                off = 0.125 * (64 * 2.0**-23 * (K[:pos + 1].abs() @ Q.abs()).max()
+                               + 2.0**-25 * Q.abs().max() * K[:pos + 1].abs().sum(1).max())
+                top = x.topk(min(2, pos + 1)).values
+                if pos and float(top[0] - top[1]) <= 2 * float(off) + 20:
+                    continue
+                clear += 1
+                want = V[int(x.argmax())]
+                tol = want.abs() * (2.0**-9 + 2.0**-11 + 2.0**-20) + (pos + 1) * 2.1e-9 * V.abs().max()
+                assert bool(((out[row, h] - want).abs() <= tol).all()), (b, h, i)
+    assert clear >= 0.9 * 4 * sum(new)
+
+
+@pytest.mark.parametrize("dims", [(64, 64), (128, 128)])
+@pytest.mark.parametrize("new,lens", [([1, 3], [200, 700]), ([100, 40], [400, 700])])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_small_differences_of_large_scores(dims, new, lens, dtype):
+    """Scores near +-20000, 5000 and 1000 that differ by a few units: one dimension of the keys is 448 throughout, another a whole number,
+    the queries 2^10, 2^8 or 2^6 times the one and once the other, so that a product's sum has at most 19 bits and is exact.
+    What is rounded is the exponent t of a weight, below 2^15 times log2(e): half a step is 2^-10 (the largest is rounded
+    as t is, and cancels), ln 2 of it of each weight, in numerator and sum; then the weight's 16 bits, the output's products
+    in 32 bits, and the output."""
+    s = Setup(dims, 1, new, lens, seed=12).fill()
+    g = torch.Generator().manual_seed(5)
+    s.host["k"].view(torch.uint8).zero_()
+    codes = s.host["k"]
+    small = (torch.randn(codes.shape[:3], generator=g) * 20).round().clamp(-60, 60)
+    codes.view(torch.uint8)[..., 3] = 0x7e   # 448
+    codes.view(torch.uint8)[..., dims[0] - 2] = small.to(A.E4M3).view(torch.uint8)
+    s.host["ks"].fill_(-7)
+    for name, b in (("k", codes.view(torch.uint8)), ("k_scale", s.bytes_of("ks"))):
+        getattr(s.cache, name).view(torch.uint8).copy_(b)
+    q = torch.zeros(s.T, 6, dims[0], dtype=dtype)
+    q[..., dims[0] - 2] = 1.0
+    for h, big in enumerate((2.0**10, -2.0**10, 2.0**8, -2.0**8, 2.0**6, -2.0**6)):
+        q[:, h, 3] = big
+    scale = 5.5   # 448 * 2^10 * 2^-7 * 5.5 = 19712
+    out = s.cache.attend(q.to(DEV), s.batch, scale=scale).cpu().double()
+    ref, mean_abs, _, _ = A.attend(s.host, q, s.start, s.lens, s.table, scale)
+    tol = torch.finfo(dtype).eps / 2 * ref.abs() + torch.finfo(dtype).smallest_normal \
+        + mean_abs * (2.0**-11 + 2 * math.log(2) * 2.0**-10 + max(lens) * 2.0**-23)
+    assert bool(((out - ref).abs() <= tol).all()), float(((out - ref).abs() - tol).max())
+
+
+@pytest.mark.parametrize("dims", DIMS)
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (15, 3)])
+@pytest.mark.parametrize("new,lens", [([1, 1, 1], [16, 65, 1500]), ([5, 0, 33], [5, 70, 130]), ([130, 2], [700, 2000])])
+def test_attention_within_the_rounding_of_its_operands(dims, heads, kv_heads, new, lens):
+    """As above, with what the query's rounding to 16 bits can take at most, 2^-25 of its largest element, and half a step of a weight of
+    16 bits (2^-28 of the largest) for each token whose own step that is."""
+    s = Setup(dims, kv_heads, new, lens, seed=heads).fill()
+    q = s.rows(heads, dims[0], BF16 if heads % 2 else F16, 2.0)
+    q[:, :, ::7] *= 2.0**-9   # elements whose 16 bits end before the type's
+    scale = dims[0] ** -0.5
+    out = s.cache.attend(q.to(DEV), s.batch).cpu().double()
+    ref, mean_abs, size, loud = A.attend(s.host, q, s.start, s.lens, s.table, scale)
+    delta = dims[0] * 2.0**-23 * size + 2.0**-25 * loud + 2.0**-20
+    tol = torch.finfo(q.dtype).eps / 2 * ref.abs() + torch.finfo(q.dtype).smallest_normal \
+        + mean_abs * (2.0**-11 + 2 * delta) + max(lens) * 2.0**-28 * 448 * 2.0**-6
+    assert bool(((out - ref).abs() <= tol).all()), float(((out - ref).abs() - tol).max())
+
+
 @pytest.mark.parametrize("new,lens", [([1, 1, 1], [64, 200, 1500]), ([100, 40], [100, 700])])
 @pytest.mark.parametrize("kind", ["first", "all", "blocks", "all but one", "tiny", "large"])
 def test_attention_over_values_of_zero_and_of_very_different_sizes(kind, new, lens):
