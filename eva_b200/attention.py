@@ -10,7 +10,7 @@ The reference's attention (runtime/ds41/model.py:566-937 `Attention`) reads a 4-
 this is plain causal attention, for layers of DeepSeek shape without that index. Everything runs on the caller's current
 CUDA stream and never synchronises the host, so it can be captured in a CUDA graph and replayed; outputs and
 workspaces come from torch's allocator for each call. No gradients are recorded (of the rotation, apply(inverse=True) is one):
-tensors that require them are refused unless gradients are off.
+tensors that require them are refused unless gradients are off, and so are dual tensors of forward-mode differentiation.
 """
 from __future__ import annotations
 
@@ -19,6 +19,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad as _forward
 
 from . import _lib
 
@@ -107,7 +108,7 @@ class Rotary:
         if (not isinstance(positions, torch.Tensor) or positions.ndim != 1 or positions.shape[0] != tokens
                 or positions.dtype not in (_I64, _I32) or positions.device != device or not positions.is_contiguous()):
             raise ValueError(f"positions must be contiguous int32 or int64 [{tokens}] on {device}")
-        if x.requires_grad:
+        if x.requires_grad or _forward._current_level >= 0:
             _no_grad(x)
         src = x if tokens == 0 else self._movable(x, out is x)
         if out is None:
@@ -172,9 +173,12 @@ def _span(t):
 
 
 def _no_grad(*tensors):
-    """The operators record no gradients: a call that autograd would follow is refused, not answered without one."""
+    """The operators record no gradients: a call that autograd would follow is refused, not answered without one. Tangents of
+    forward mode are followed under no_grad too."""
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise ValueError("the attention operators record no gradients: call them under torch.no_grad()")
+    if _forward._current_level >= 0 and any(_forward.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError("the attention operators have no forward-mode derivatives: unpack dual tensors first")
 
 
 def _folded(t):
@@ -345,7 +349,7 @@ class PagedKVCache:
                 raise ValueError(f"rotary must be a Rotary on {device}")
             if rotary._end > self.key_dim:
                 raise ValueError(f"the rotation ends at {rotary._end}, keys have {self.key_dim} dimensions")
-        if k.requires_grad or v.requires_grad:
+        if k.requires_grad or v.requires_grad or _forward._current_level >= 0:
             _no_grad(k, v)
         b = self._batch(batch, tokens)
         if k.stride(2) != 1:
@@ -377,7 +381,7 @@ class PagedKVCache:
             scale = self._scale
         elif not isinstance(scale, (int, float)) or not 0 <= scale <= 2e38:
             raise ValueError("scale must be a finite nonnegative number")
-        if q.requires_grad:
+        if q.requires_grad or _forward._current_level >= 0:
             _no_grad(q)
         b = self._batch(batch, tokens)
         st, sh, sd = q.stride()

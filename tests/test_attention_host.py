@@ -66,6 +66,20 @@ def test_no_cpu_fallback():
         T.PagedBatch(i32, i32[:1], i32[None, :1], 1)
 
 
+def test_tensors_that_forward_mode_follows_are_refused():
+    """Dual tensors, with gradients off too; plain ones within a level are not."""
+    from torch.autograd import forward_ad
+    x = torch.ones(3)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(3))
+        T._no_grad(x, x)
+        with pytest.raises(ValueError, match="forward-mode"):
+            T._no_grad(x, dual)
+        with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+            T._no_grad(dual * 2)
+    T._no_grad(x)
+
+
 def _cache(**kw):
     a = 1 << 20
     d = dict(pages=8, kv_heads=2, key_dim=128, value_dim=128, k=a, v=a, k_scale=a, v_scale=a, status=a)

@@ -879,6 +879,23 @@ def test_layer_stack_of_a_padded_step():
     assert bool(outs[0].isfinite().all()) and torch.equal(*outs)
 
 
+def test_dual_tensors_are_refused():
+    """No tangent is dropped in silence; the same calls with plain tensors go on within the level."""
+    from torch.autograd import forward_ad
+    s = Setup((64, 64), 2, [1, 1], [10, 20]).fill()
+    q, k, pos = s.rows(4, 64, BF16).to(DEV), s.rows(2, 64, BF16).to(DEV), torch.zeros(2, dtype=torch.int64, device=DEV)
+    r = Rotary(64, layout="half")
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))   # noqa: E731
+        for f in (lambda: r.apply(dual(q), pos), lambda: s.cache.attend(dual(q), s.batch), lambda: s.cache.append(dual(k), k, s.batch),
+                  lambda: s.cache.append(k, dual(k), s.batch)):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="forward-mode"):
+                    f()
+        s.cache.append(k, k, s.batch)
+        assert s.cache.attend(r.apply(q, pos), s.batch).shape == q.shape
+
+
 def test_refusals():
     s = Setup((64, 64), 2, [1, 1], [10, 20]).fill()
     q, k = s.rows(4, 64, BF16).to(DEV), s.rows(2, 64, BF16).to(DEV)
