@@ -141,6 +141,8 @@ class Rotary:
         _rows(out, "out", self.device, (x.dtype,), x.shape[1], x.shape[2])
         if out.shape[0] != x.shape[0]:
             raise ValueError("out must have x's shape")
+        if out.requires_grad or _forward._current_level >= 0:
+            _no_grad(out)
         if _folded(out):
             raise ValueError("out must not overlap itself")
         same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()   # the same memory: in place
@@ -397,8 +399,11 @@ class PagedKVCache:
         elif (not isinstance(out, torch.Tensor) or out.device != device or out.dtype != q.dtype or not out.is_contiguous()
               or out.shape != (tokens, heads, self.value_dim) or out.data_ptr() % 16):
             raise ValueError(f"out must be a contiguous {q.dtype} [{tokens}, {heads}, {self.value_dim}] on {device}, 16-byte aligned")
-        elif _overlap(q, out):
-            raise ValueError("out must not overlap q")
+        else:
+            if _overlap(q, out):
+                raise ValueError("out must not overlap q")
+            if out.requires_grad or _forward._current_level >= 0:
+                _no_grad(out)
         n = self._sizes.get((heads, batch.max_q))
         with _on(device):
             if n is None:

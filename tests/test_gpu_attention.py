@@ -879,6 +879,20 @@ def test_layer_stack_of_a_padded_step():
     assert bool(outs[0].isfinite().all()) and torch.equal(*outs)
 
 
+def test_outputs_that_autograd_follows_are_refused():
+    """A result written into a tensor with a history would keep that history's gradient."""
+    s = Setup((64, 64), 2, [1, 1], [10, 20]).fill()
+    q, pos = s.rows(4, 64, BF16).to(DEV), torch.zeros(2, dtype=torch.int64, device=DEV)
+    r, w = Rotary(64, layout="half"), torch.ones(2, 4, 64, dtype=BF16, device=DEV, requires_grad=True)
+    for out in (w, w * 2):
+        with pytest.raises(ValueError, match="no gradients"):
+            r.apply(q, pos, out=out)
+        with pytest.raises(ValueError, match="no gradients"):
+            s.cache.attend(q, s.batch, out=out)
+    with torch.no_grad():
+        assert r.apply(q, pos, out=w) is w and s.cache.attend(q, s.batch, out=w) is w
+
+
 def test_dual_tensors_are_refused():
     """No tangent is dropped in silence; the same calls with plain tensors go on within the level."""
     from torch.autograd import forward_ad
