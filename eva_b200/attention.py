@@ -179,8 +179,12 @@ def _no_grad(*tensors):
     forward mode are followed under no_grad too."""
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise ValueError("the attention operators record no gradients: call them under torch.no_grad()")
-    if _forward._current_level >= 0 and any(_forward.unpack_dual(t).tangent is not None for t in tensors):
+    if any(_dual(t) for t in tensors):
         raise ValueError("the attention operators have no forward-mode derivatives: unpack dual tensors first")
+
+
+def _dual(t):
+    return _forward._current_level >= 0 and _forward.unpack_dual(t).tangent is not None
 
 
 def _folded(t):
@@ -458,11 +462,13 @@ class PagedAttention:
 
     def forward(self, h, batch, positions, *, out_f32=None):
         """h: BF16 [tokens, hidden], the batch's new tokens; positions: int32 or int64 [tokens], each token's place in its
-        sequence. Returns BF16 [tokens, hidden], in FP32 into out_f32 where that is given. Rows of no sequence (behind the last one,
+        sequence. Returns BF16 [tokens, hidden], or FP32 in out_f32 where that is given, not rounded to BF16 in between. Rows of no sequence (behind the last one,
         or of one that does not fit the batch) are zero."""
         c = self.cache
         if h.ndim != 2 or h.shape[1] != self.hidden or h.dtype != _BF16 or h.device != c.device:
             raise ValueError(f"h must be BF16 [tokens, {self.hidden}] on {c.device}")
+        if out_f32 is not None and (out_f32.shape != h.shape or out_f32.dtype != _F32 or out_f32.device != c.device):
+            raise ValueError(f"out_f32 must be FP32 {list(h.shape)} on {c.device}")
         rows = h @ self.wqkv.T
         nq, nk = self.heads * c.key_dim, c.kv_heads * c.key_dim
         q = rows[:, :nq].unflatten(1, (self.heads, c.key_dim))
@@ -472,8 +478,12 @@ class PagedAttention:
             q = self.rotary.apply(q, positions, out=q)
         c.append(k, v, batch, rotary=self.rotary)
         o = q.new_zeros((h.shape[0], self.heads, c.value_dim))   # attend leaves rows of no sequence as they were
-        y = c.attend(q, batch, scale=self.scale, window=self.window, out=o).flatten(1) @ self.wo.T
-        return y if out_f32 is None else out_f32.copy_(y)
+        o = c.attend(q, batch, scale=self.scale, window=self.window, out=o).flatten(1)
+        if out_f32 is None:
+            return o @ self.wo.T
+        if (self.wo.requires_grad and torch.is_grad_enabled()) or _dual(self.wo):
+            return out_f32.copy_(o @ self.wo.T)   # torch has no derivative of the product below
+        return torch.mm(o, self.wo.T, out_dtype=_F32, out=out_f32)
 
     __call__ = forward
 

@@ -842,6 +842,33 @@ def test_attention_half_gives_zeros_to_rows_of_no_sequence(new, lens):
         assert all(torch.equal(a, b) for a, b in zip(seen[0], other))
 
 
+@pytest.mark.parametrize("new,lens", [([1, 1], [1, 1]), ([40, 3], [40, 3])])
+def test_attention_half_keeps_32_bits_where_they_are_asked_for(new, lens):
+    """out_f32 is the product of the attention's BF16 output and wo with nothing rounded but its 32-bit sums: 64 terms, each within
+    2^-23 of the terms' sizes (a BF16 result is off by up to 2^-9 of the sum)."""
+    from eva_b200.attention import make_attention
+    half = make_attention(1, 96, 1, 1, 64, 64, 4, seed=1)[0]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)   # noqa: E731
+    T = sum(new)
+    batch, pos = PagedBatch(i32([0, new[0], T]), i32(lens), i32([[0], [1]]), max(new)), torch.zeros(T, dtype=torch.int64, device=DEV)
+    h = torch.randn(T, 96, generator=torch.Generator().manual_seed(2)).to(BF16).to(DEV)
+    wide = torch.empty(T, 200, device=DEV)
+    out = half.forward(h, batch, pos, out_f32=wide[:, :96])
+    assert out.data_ptr() == wide.data_ptr() and out.shape == (T, 96)
+    o = half.cache.attend((h @ half.wqkv.T)[:, None, :64], batch).flatten(1).double()
+    ref, size = o @ half.wo.T.double(), o.abs() @ half.wo.T.double().abs()
+    assert bool(((out.double() - ref).abs() <= 64 * 2.0**-23 * size).all())
+    y = half.forward(h, batch, pos)
+    assert y.dtype == BF16 and bool(((y.double() - ref).abs() <= 64 * 2.0**-23 * size + 2.0**-8 * ref.abs() + 1e-38).all())
+    half.wo.requires_grad_()
+    half.forward(h, batch, pos, out_f32=torch.empty(T, 96, device=DEV)).sum().backward()
+    want = o.sum(0)   # of the sum over the output: every row of wo has it, rounded to BF16
+    assert bool(((half.wo.grad.double() - want).abs() <= 2.0**-7 * o.abs().sum(0)).all())
+    for bad in (torch.empty(T, 95, device=DEV), torch.empty(T, 96, device=DEV, dtype=BF16), torch.empty(T, 96)):
+        with pytest.raises(ValueError):
+            half.forward(h, batch, pos, out_f32=bad)
+
+
 def test_layer_stack_of_a_padded_step():
     """A step of three rows of which two belong to sequences, captured and replayed with the third left over: what memory held before
     reaches no row."""
