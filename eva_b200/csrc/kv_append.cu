@@ -64,7 +64,7 @@ __device__ __forceinline__ float inv_scale(int byte) { return __uint_as_float(st
 
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// two 16-bit elements as floats; exponent bits of an element that is not finite; exponent bits above which a rotation might not be
+// two 16-bit elements as floats; exponent bits of an element that is not finite
 template <typename T> __device__ __forceinline__ float2 up2(uint32_t v);
 template <> __device__ __forceinline__ float2 up2<__nv_bfloat16>(uint32_t v)
 {
@@ -74,8 +74,6 @@ template <> __device__ __forceinline__ float2 up2<__half>(uint32_t v) { return _
 template <typename T> constexpr uint32_t INF_BITS = 0;
 template <> constexpr uint32_t INF_BITS<__nv_bfloat16> = 0x7f80u;
 template <> constexpr uint32_t INF_BITS<__half> = 0x7c00u;
-template <typename T> constexpr uint32_t LOUD_BITS = INF_BITS<T>;
-template <> constexpr uint32_t LOUD_BITS<__nv_bfloat16> = 0x7e00u;
 
 // Dimensions of pair i of a key: the rotated ones as the layout pairs them, the others as neighbours.
 __device__ __forceinline__ int2 key_pair(const EvaRotary& r, int i)
@@ -265,14 +263,15 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, STAGED ? (DK == 64 ? 4 : DK
         vmax = max(vmax & 0xffffu, vmax >> 16);
         raw = max(max(raw & 0xffffu, raw >> 16), flat);
         // A token with an element that is not finite has no key of its own, and does not count for the key's scale; of its values the
-        // finite ones stay.
+        // finite ones stay. (A rotated key's overflow is an infinity in one of its pair at least, never a NaN: the products are
+        // summed unrounded.)
         uint32_t bad = 0;
         auto finite_only = [&](uint32_t w) {
             if ((w & 0x7fffu) >= INF_BITS<T>) w &= 0xffff0000u;
             if ((w >> 16 & 0x7fffu) >= INF_BITS<T>) w &= 0xffffu;
             return w;
         };
-        const bool odd = __any_sync(0xffffffffu, vmax >= INF_BITS<T> || raw >= LOUD_BITS<T>);
+        const bool odd = __any_sync(0xffffffffu, vmax >= INF_BITS<T> || raw >= INF_BITS<T> || !finite(kmax));
         if (odd) {
             vmax = 0;
             kmax = 0.0f;

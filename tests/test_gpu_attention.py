@@ -292,6 +292,24 @@ def test_append_of_values_that_are_not_finite():
     assert bool(nan[s.table[0][0], 0, 30 + 3].all()) and bool(nan[s.table[0][0], 1, 30 + 9].all())
 
 
+@pytest.mark.parametrize("dtype,big,mscale", [(BF16, 2.0**124, 64.0), (F16, 1000.0, 2.0**120)])
+@pytest.mark.parametrize("layout,rot,offset", [("half", 64, 0), ("interleaved", 20, 44), ("half", 22, 2)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_append_of_keys_that_the_rotation_takes_out_of_range(dtype, big, mscale, layout, rot, offset, shift):
+    """A finite key that is not finite once rotated and scaled (|y| of a pair (a, a) is |a| mscale at least in one of the two) is
+    treated as one that was not finite before: the same bytes."""
+    r, got = Rotary(rot, layout=layout, offset=offset, mscale=mscale), []
+    for value in (big, math.nan):
+        s = Setup((64, 64), 3, [40, 3], [70, 23], seed=2)
+        k, v = s.rows(3, 64, dtype), s.rows(3, 64, dtype)
+        k[3, 0], k[11, 2], k[41, 1], k[42, 1] = value, value, value, value
+        wide = torch.zeros(s.T, 3, 64 + 8, dtype=dtype, device=DEV)
+        wide[:, :, shift:shift + 64] = k.to(DEV)
+        s.cache.append(wide[:, :, shift:shift + 64], v.to(DEV), s.batch, rotary=r)
+        got.append([getattr(s.cache, n).view(torch.uint8).clone() for n in ("k", "v", "k_scale", "v_scale")])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 def test_append_extremes_of_the_range():
     """Zero blocks, the smallest and the largest values of the input types."""
     for dtype, big, tiny in ((BF16, 3.0e38, 1e-38), (F16, 65504.0, 6e-8)):
