@@ -29,6 +29,7 @@ _DTYPE = {_F16: _lib.DTYPE_F16, _BF16: _lib.DTYPE_BF16, _F32: _lib.DTYPE_F32}
 PAGE, BLOCK = _lib.KV_PAGE, _lib.KV_BLOCK
 HEAD_DIMS = ((64, 64), (128, 128), (192, 128))
 _INT32_MAX = 2**31 - 1
+_DECODE_ROWS = 16   # of the library: rows that share a key and value, up to which the decode kernel takes a call
 
 
 def _device(device) -> torch.device:
@@ -322,7 +323,7 @@ class PagedKVCache:
         self._c = _lib.EvaKvCache(pages, kv_heads, key_dim, value_dim, self.k.data_ptr(), self.v.data_ptr(),
                                   self.k_scale.data_ptr(), self.v_scale.data_ptr(), self._status.data_ptr())
         self._ref = ctypes.byref(self._c)
-        self._scale, self._sizes = key_dim ** -0.5, {}   # default scale; workspace bytes by (heads, max_q)
+        self._scale, self._sizes = key_dim ** -0.5, {}   # default scale; workspace bytes by rows that share a key
 
     def _buffer(self, t, shape, dtype, name):
         if t is None:
@@ -408,13 +409,14 @@ class PagedKVCache:
                 raise ValueError("out must not overlap q")
             if out.requires_grad or _forward._current_level >= 0:
                 _no_grad(out)
-        n = self._sizes.get((heads, batch.max_q))
+        rows = min(batch.max_q * (heads // self.kv_heads), _DECODE_ROWS + 1)   # above them the size is the same
+        n = self._sizes.get(rows)
         with _on(device):
             if n is None:
                 n = self.lib.eva_kv_attend_workspace(self._ref, b, heads)
                 if n == 0:
                     raise ValueError("unsupported batch")
-                self._sizes[heads, batch.max_q] = n
+                self._sizes[rows] = n
             ws = q.new_empty((n,), dtype=_U8)
             rc = self.lib.eva_kv_attend(self._ref, b, q.data_ptr(), _DTYPE[q.dtype], heads, st, sh, scale, window, ws.data_ptr(), n,
                                         out.data_ptr(), _stream(device))

@@ -550,6 +550,24 @@ def test_queries_that_are_not_finite_stay_in_their_rows(new, lens):
     assert int(out.isnan().sum()) == 2 * 64
 
 
+def test_workspace_sizes_kept_for_many_prompt_lengths():
+    """A cache that sees many lengths and head counts keeps few sizes, each what the library asks for."""
+    import ctypes
+    s = Setup((64, 64), 2, [1], [100]).fill()
+    for heads in (2, 8, 34):
+        q = s.rows(heads, 64, BF16).to(DEV)
+        for max_q in [*range(1, 40), 300, 5000, 1 << 28]:
+            batch = PagedBatch(s.batch.q_start, s.batch.seq_lens, s.batch.table, max_q)
+            rows = min(max_q * heads // 2, 17)
+            if max_q in (1, 2, 17, 1 << 28):
+                _check_attention(s, q, s.cache.attend(q, batch), 0.125)
+            else:
+                s.cache.attend(q[:0], batch)
+            want = s.cache.lib.eva_kv_attend_workspace(ctypes.byref(s.cache._c), ctypes.byref(batch._c), heads)
+            assert s.cache._sizes[rows] == want
+    assert len(s.cache._sizes) <= 18 and s.cache.status() == 0
+
+
 def test_attention_strided_queries():
     s = Setup((128, 128), 2, [20, 1], [100, 30]).fill()
     wide = torch.randn(s.T, 900, device=DEV).to(BF16)
