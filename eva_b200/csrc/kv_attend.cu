@@ -2,7 +2,7 @@
 //
 // At most 16 rows (new tokens x query heads of a group) share each key and value, so the cache's bytes are the cost: every
 // one is read once. The tokens of all sequences and heads, in tiles of a page (64), form one line of work that is cut
-// into equal pieces, one per warp, whatever the lengths are; a warp's tiles come through its own
+// into equal pieces whatever the lengths are, one per warp of the GPU or, in short lines, fewer (DEC_PIECE, DEC_SPREAD); a warp's tiles come through its own
 // two-stage ring of bulk copies (a page of a head is contiguous). Scores and outputs are m16n8k16 products with fp32 sums,
 // transposed: keys and values are the 16-row operand and the query rows the 8-column one, so that up to eight rows cost what one
 // does and no product is padding (an accumulator in tensor memory has 128 rows; the tensor pipes are at 19 % here, DRAM is the

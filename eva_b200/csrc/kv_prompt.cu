@@ -51,7 +51,6 @@ template <int DK, int DV> struct PrCfg {
     static constexpr int RK = PR_STEP * DK, RV = PR_STEP * DV;   // a step's codes as they are in the cache
     static constexpr int KST = DK == 192 ? 2 : 3, VST = KST, RST = 2;   // stages
     static constexpr int SMEM = Q + KST * K + VST * V + RST * (RK + RV) + 1024;
-    static_assert(SMEM <= 227 * 1024 - 7168, "shared memory");
 };
 
 struct PrBars {
@@ -391,6 +390,9 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 1) kv_prompt_kernel(AttendArgs 
     __shared__ float qscale[2][PR_TILE];                  // of a row's query: its power of two times the call's scale
     __shared__ float top[2][PR_TILE];                     // the running M of a tile's rows
     __shared__ float2 sums[2][2][PR_TILE];                // [tile][step & 1]: M and sum of a row as its steps left them
+    static_assert(C::SMEM + sizeof(B) + sizeof(scales) + sizeof(place) + sizeof(segs) + sizeof(qscale) + sizeof(top) + sizeof(sums) + 7 * 16 <=
+                      227 * 1024,
+                  "shared memory, each array at a multiple of 16");
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform for the compiler
     uint8_t* smem = align1024(smem_raw);
     const uint32_t sq = smem_u32(smem), sk = sq + C::Q, sv = sk + C::KST * C::K;
