@@ -36,7 +36,7 @@ struct AppendArgs {
     const void* k;
     const void* v;
     int64_t kt, kh, vt, vh;
-    int blocks;   // blocks one sequence's max_q rows can touch
+    int blocks;   // blocks that one sequence's rows can touch
 };
 
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi)
@@ -482,7 +482,8 @@ extern "C" int eva_kv_append(const EvaKvCache* cache, const EvaKvBatch* batch, c
     p.kh = k_head_stride;
     p.vt = v_token_stride;
     p.vh = v_head_stride;
-    p.blocks = (batch->max_q + KV_BLOCK - 2) / KV_BLOCK + 1;
+    const int most = batch->max_q < batch->tokens ? batch->max_q : batch->tokens;   // rows of a sequence
+    p.blocks = (most + KV_BLOCK - 2) / KV_BLOCK + 1;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const cudaError_t e = dtype == EVA_DTYPE_BF16 ? append_typed<__nv_bfloat16>(p, st) : append_typed<__half>(p, st);
     return e == cudaSuccess ? EVA_OK : EVA_ERR_CUDA;

@@ -257,6 +257,19 @@ def test_append_of_rows_anywhere_in_memory(dims, layout, rot, offset, kv_heads):
         assert all(torch.equal(a, b) for a, b in zip(got, want)), shift
 
 
+@pytest.mark.parametrize("seqs,new,max_q", [(200, 1, 1 << 28), (3, 21, 1 << 28), (150, 2, 5000)])
+def test_append_of_far_fewer_rows_than_max_q(seqs, new, max_q):
+    """max_q only bounds the rows of a sequence: any one appends the same bytes."""
+    got = []
+    for bound in (new, max_q):
+        s = Setup((64, 64), 2, [new] * seqs, [new + 7 * i for i in range(seqs)], seed=1)
+        k, v = s.rows(2, 64, BF16).to(DEV), s.rows(2, 64, BF16).to(DEV)
+        s.cache.append(k, v, PagedBatch(s.batch.q_start, s.batch.seq_lens, s.batch.table, bound))
+        assert s.cache.status() == 0
+        got.append([getattr(s.cache, n).view(torch.uint8).clone() for n in ("k", "v", "k_scale", "v_scale")])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 @pytest.mark.parametrize("dims", DIMS)
 @pytest.mark.parametrize("size", [0.02, 200.0])
 def test_append_beside_sequences_without_new_rows(dims, size):
