@@ -64,13 +64,7 @@ __device__ __forceinline__ float inv_scale(int byte) { return __uint_as_float(st
 
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// two 16-bit elements as floats; exponent bits of an element that is not finite
-template <typename T> __device__ __forceinline__ float2 up2(uint32_t v);
-template <> __device__ __forceinline__ float2 up2<__nv_bfloat16>(uint32_t v)
-{
-    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-}
-template <> __device__ __forceinline__ float2 up2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+// exponent bits of an element that is not finite
 template <typename T> constexpr uint32_t INF_BITS = 0;
 template <> constexpr uint32_t INF_BITS<__nv_bfloat16> = 0x7f80u;
 template <> constexpr uint32_t INF_BITS<__half> = 0x7c00u;
@@ -221,7 +215,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, STAGED ? (DK == 64 ? 4 : DK
             }
         };
         auto rotated = [&](uint2 w, int r, int m, float2& ya, float2& yb) {
-            const float2 a = up2<T>(w.x), c = up2<T>(w.y);
+            const float2 a = two_floats<T>(w.x), c = two_floats<T>(w.y);
             ya = a;
             yb = c;
             if (rotates) {
@@ -259,7 +253,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, STAGED ? (DK == 64 ? 4 : DK
             }
         }
         flat = max(flat & 0xffffu, flat >> 16);
-        kmax = fmaxf(kmax, up2<T>(flat).x);
+        kmax = fmaxf(kmax, two_floats<T>(flat).x);
         vmax = max(vmax & 0xffffu, vmax >> 16);
         raw = max(max(raw & 0xffffu, raw >> 16), flat);
         // A token with an element that is not finite has no key of its own, and does not count for the key's scale; of its values the
@@ -293,7 +287,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, STAGED ? (DK == 64 ? 4 : DK
                 else kmax = fmaxf(kmax, top);
             }
         }
-        const int ve = max(scale_byte(__float_as_uint(up2<T>(__reduce_max_sync(0xffffffffu, vmax)).x)), vbyte);
+        const int ve = max(scale_byte(__float_as_uint(two_floats<T>(__reduce_max_sync(0xffffffffu, vmax)).x)), vbyte);
         const int ke = max(scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(kmax))), kbyte);
         const float vinv = inv_scale(ve), kinv = inv_scale(ke);
         if (lo > 0 && ke > kbyte) {   // the older keys: lo rows of DK bytes, contiguous
@@ -336,7 +330,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, STAGED ? (DK == 64 ? 4 : DK
 #pragma unroll 4
                 for (int r = lo; r < hi; ++r) {
                     const uint2 w = keys(r, m);
-                    put_key(up2<T>(w.x), up2<T>(w.y), r, m);
+                    put_key(two_floats<T>(w.x), two_floats<T>(w.y), r, m);
                 }
             }
         }
@@ -371,7 +365,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, STAGED ? (DK == 64 ? 4 : DK
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float2 x = up2<T>(j < 2 ? v0.x : v0.y), y = up2<T>(j < 2 ? v1.x : v1.y);
+                    const float2 x = two_floats<T>(j < 2 ? v0.x : v0.y), y = two_floats<T>(j < 2 ? v1.x : v1.y);
                     uint32_t two = e4m3x2((j % 2 ? x.y : x.x) * vinv, (j % 2 ? y.y : y.x) * vinv);
                     if (merge) {
                         const uint32_t old = in[j][t / 2] >> (t % 2 * 16) & 0xffffu;

@@ -25,8 +25,6 @@
 #include "kv.cuh"
 #include "kv_attend.cuh"
 
-#include <cuda_fp8.h>
-
 namespace eva {
 
 constexpr int DEC_ROWS = 16;

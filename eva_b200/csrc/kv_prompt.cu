@@ -31,8 +31,6 @@
 #include "kv_attend.cuh"
 #include "tc.cuh"
 
-#include <cuda_fp8.h>
-
 namespace eva {
 
 constexpr int PR_TILE = 128, PR_ROWS = 2 * PR_TILE;       // rows of a tile, of a CTA
