@@ -304,7 +304,8 @@ class PagedKVCache:
     and head. (key_dim, value_dim) is (64, 64), (128, 128) or (192, 128).
 
     k [pages, kv_heads, 64, key_dim], v [pages, kv_heads, value_dim, 64] (a dimension's tokens side by side), k_scale and
-    v_scale [pages, kv_heads, 4]; existing contiguous tensors may be given (float8 or uint8; scale bytes 1 .. 253)."""
+    v_scale [pages, kv_heads, 4]; existing contiguous tensors may be given (float8 or uint8; scale bytes 1 .. 253, and no NaN among the
+    value codes of a sequence's tokens: it would reach rows that do not see its token; an append writes none)."""
 
     def __init__(self, pages, kv_heads, key_dim, value_dim=None, *, device="cuda", k=None, v=None, k_scale=None, v_scale=None):
         value_dim = key_dim if value_dim is None else value_dim
@@ -342,7 +343,7 @@ class PagedKVCache:
         """Write the batch's new tokens: k [tokens, kv_heads, key_dim] rotated by each token's position in its sequence, and
         v [tokens, kv_heads, value_dim] (BF16 or Half, any token and head strides), quantised. A block's scale is the smallest
         power of two that fits its tokens; one that a later token raises has its older codes rescaled. A token with a
-        non-finite element gets a NaN key: the rows that see it become NaN, and no others."""
+        non-finite element (of the rotated key too) gets a NaN key: the rows that see it become NaN, and no others."""
         device = self.device
         if (not isinstance(k, torch.Tensor) or k.ndim != 3 or k.dtype not in (_BF16, _F16) or k.device != device
                 or k.shape[1] != self.kv_heads or k.shape[2] != self.key_dim):
@@ -373,8 +374,12 @@ class PagedKVCache:
     def attend(self, q, batch, *, scale=None, window=0, out=None):
         """softmax(scale q k^T) v of q [tokens, heads, key_dim] (BF16 or Half, already rotated) over the batch's sequences,
         new tokens included: a row sees the tokens up to its own position, with window > 0 the last `window` of them.
-        heads is a multiple of kv_heads. Values below 2^-39 may count as zero in the output (not in the softmax's sum). Returns [tokens, heads, value_dim] of q's type; rows that see nothing are zero, rows behind
-        the last sequence are left as they were (in out; a new tensor has no values there)."""
+        heads is a multiple of kv_heads. Returns [tokens, heads, value_dim] of q's type; rows that see nothing are zero, rows behind
+        the last sequence, and of one that does not fit, are left as they were (in out; a new tensor has no values there).
+
+        Values below 2^-39, and weights (times their block's value scale) below 2^-28 of a row's largest, may count as zero in the
+        output (not in the softmax's sum); with values above 2^43 beside much smaller ones the sum may lose tokens. Scores count as 32-bit floats: one above
+        their range makes its row NaN, one below has no weight."""
         device = self.device
         if (not isinstance(q, torch.Tensor) or q.ndim != 3 or q.dtype not in (_BF16, _F16) or q.device != device
                 or q.shape[2] != self.key_dim):

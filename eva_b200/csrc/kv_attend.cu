@@ -10,15 +10,16 @@
 // token's key scale multiplies its score, its value scale 2^e joins the exponent, t = score + e, and the softmax's running
 // maximum is that of t:
 //   out = sum 2^(t - M) code / sum 2^(t - M) 2^-e.
-// Weights are rounded to fp16 with 2^14 as the largest, so that tokens down to 2^-28 of the largest keep 11 bits.
+// Weights are rounded to fp16, the operand's type, with 2^14 as the largest, so that tokens down to 2^-28 of the largest keep 11 bits; their sum
+// is of the unrounded ones.
 // The order of a tile's tokens within a product is free, and chosen so that both operands are 16-byte shared-memory loads and
 // the weights need no exchange but movmatrix: product e of a tile has, in its rows r and r + 8, tokens
 // 16 (r / 2) + 4 e + (0, 2) + r % 2, and lane quad q holds of the values tokens 16 q .. 16 q + 15.
 // An item (sequence and head) whose tiles fall to several warps leaves fp32 partial sums, which
 // kv_combine_kernel joins in their order, so results do not depend on timing.
 //
-// 128 + 128 dimensions, 8 heads of keys: 64 sequences of up to 8192 tokens, 4 rows: 581 MB in 103 us, 5.6 TB/s (0.86 of the 6.5 a
-// copy reaches); two of 131072, 8 rows: 537 MB in 98.5 us, 5.5 TB/s. Smaller calls are latency: 16 sequences of some 3000 tokens
+// 128 + 128 dimensions, 8 heads of keys: 64 sequences of up to 8192 tokens, 4 rows: 581 MB in 106 us, 5.5 TB/s (0.84 of the 6.5 a
+// copy reaches); two of 131072, 8 rows: 537 MB in 101 us, 5.3 TB/s; 16 heads of 192 + 128, one row each: 1365 MB in 236 us, 5.8 TB/s. Smaller calls are latency: 16 sequences of some 3000 tokens
 // within a window of 4096, 4 heads, 16 rows: 54 MB in 36.5 us, of which a warp's six to eight tiles one behind the other take 25.
 #include <algorithm>
 

@@ -17,7 +17,7 @@
 // causal rows of different lengths and ragged batches fill the GPU alike; row blocks cut between pieces leave fp32 partial
 // sums that kv_prompt_combine joins in their order.
 //
-// 8192 new tokens, 16 query heads on 4 of 128 + 128 dimensions: 352 us, 275 GFLOP at 780 TFLOP/s (0.47 of the 1679 that a library
+// 8192 new tokens, 16 query heads on 4 of 128 + 128 dimensions: 355 us, 275 GFLOP at 775 TFLOP/s (0.46 of the 1679 that a library
 // product reaches); three sequences of up to 700 tokens behind 20000, 16 heads of 192 + 128: 352 us, 730 TFLOP/s. What bounds
 // it is one step's chain: scores, maximum, weights, their product take 1900 clocks of tensor core and 3200 of softmax for each tile
 // and parity, of which two overlap, so 2550 a step; the tensor pipe is 39 % busy, exponentials 39 %, issue 51 %. Steps there

@@ -6,7 +6,7 @@
 // the two units that hold both halves), computes its pairs' cosines and sines once and applies them to
 // `hc` heads. The traffic is one read and one write of x; the copied dimensions outside the rotated part
 // go through the same threads, and are left out when x is rotated in place. 8192 x 32 heads of 192 bf16, 64 rotated: interleaved 42
-// us, 201 MB at 4.8 TB/s of a copy's 6.5; bounded by loads, angles and stores in turn with 20 warps an SM (their registers hold
+// us, 201 MB at 4.8 TB/s of a copy's 6.5; half layout 59, each thread's angles serving four heads; bounded by loads, angles and stores in turn with 20 warps an SM (their registers hold
 // eight units). One token: 9 us, the host's.
 #include <algorithm>
 
@@ -43,7 +43,8 @@ template <typename T, int V> struct alignas(sizeof(T) * V) RotVec {
 
 // Units of a head, V elements each (half layout: a rotated unit is V elements of each half):
 // [0, offset / V) copied, then the rotated ones, then the copied rest. V divides every part.
-// Ten blocks an SM for pairs of halves: 62 us, 66 with the registers it would take; interleaved pairs 41.5 and 39.4.
+// Blocks an SM, 8192 x 32 heads of 192 bf16, the last 64 rotated: pairs of halves 59 us with ten, 63 with the registers that they would take;
+// interleaved pairs 42 with those, 38.5 with ten. (All of 128 dimensions: 33 either way, 28.3 and 26.3.)
 template <typename T, int V, bool INTER>
 __global__ void __launch_bounds__(ROT_THREADS, INTER ? 1 : 10) rotary_kernel(RotArgs p)
 {

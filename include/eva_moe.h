@@ -366,9 +366,10 @@ int eva_kv_append(const EvaKvCache* cache, const EvaKvBatch* batch, const EvaRot
  * only the last `window` of them; out = softmax(scale q k^T) v, zero where nothing is seen. q: [tokens][heads]
  * [key_dim], heads a multiple of kv_heads (query head h reads head h / (heads / kv_heads)); out: contiguous
  * [tokens][heads][value_dim] of q's type (F16 or BF16). Rows behind the last sequence stay as they were.
- * Scores count as 32-bit floats (beyond their range a row is NaN). Values of a block that are all below 2^-39 may count
- * as zero in the output, never in the softmax's sum, which holds tokens down to 2^-40 of the largest while values are
- * below 2^43.
+ * Scores count as 32-bit floats: one above their range makes its row NaN, one below has no weight (a row of none but such is zero).
+ * Weights (times their block's value scale) below 2^-28 of a row's largest, and values of a block that are all below 2^-39, may count as zero in
+ * the output, never in the softmax's sum, which holds tokens down to 2^-40 of the largest while values are below 2^43. Value codes must be
+ * finite, as an append writes them.
  * workspace: eva_kv_attend_workspace() bytes, 16-byte aligned, not shared by calls that may overlap. */
 size_t eva_kv_attend_workspace(const EvaKvCache* cache, const EvaKvBatch* batch, int32_t heads);
 int eva_kv_attend(const EvaKvCache* cache, const EvaKvBatch* batch, const void* q, int32_t dtype, int32_t heads,

@@ -465,6 +465,31 @@ def test_small_differences_of_large_scores(dims, new, lens, dtype):
     assert bool(((out - ref).abs() <= tol).all()), float(((out - ref).abs() - tol).max())
 
 
+@pytest.mark.parametrize("new,lens", [([1, 1], [200, 700]), ([100, 40], [400, 700])])
+def test_scores_beyond_32_bits(new, lens):
+    """Above the range a row is NaN; below it a score has no weight, and a row of none but such is zero; the rows beside are right."""
+    s = Setup((64, 64), 1, new, lens, seed=3).fill()
+    s.host["k"].view(torch.uint8).fill_(0x7e)   # 448
+    s.host["ks"].fill_(100)
+    for b, n in enumerate(lens):   # every third token's keys are zero, but in the last sequence
+        for t in range(0, n if b == 0 else 0, 3):
+            s.host["k"].view(torch.uint8)[s.table[b][t // 64], 0, t % 64] = 0
+    s.cache.k.view(torch.uint8).copy_(s.host["k"].view(torch.uint8))
+    s.cache.k_scale.view(torch.uint8).copy_(s.bytes_of("ks"))
+    q = torch.zeros(s.T, 4, 64, dtype=BF16)
+    q[:, 0], q[:, 1], q[:, 2] = -2.0**30, 2.0**30, 2.0**-120   # scores -+2^141 and, of the others, 2^-8 and 0
+    out = s.cache.attend(q.to(DEV), s.batch)
+    ref, mean_abs, _, _ = A.attend(s.host, q, s.start, s.lens, s.table, 0.125)
+    for h in (0, 2, 3):
+        want = ref[:, h].clone()
+        if h == 0:
+            want[s.start[1]:] = 0.0
+        tol = 2.0**-9 * want.abs() + mean_abs[:, h] * (2.0**-11 + 2.0**-12)
+        assert bool(((out[:, h].cpu().double() - want).abs() <= tol).all()), h
+    first = [s.start[b] + i for b in range(2) for i in range(new[b])]
+    assert bool(out[first, 1].isnan().all())
+
+
 @pytest.mark.parametrize("dims", DIMS)
 @pytest.mark.parametrize("heads,kv_heads", [(4, 2), (15, 3)])
 @pytest.mark.parametrize("new,lens", [([1, 1, 1], [16, 65, 1500]), ([5, 0, 33], [5, 70, 130]), ([130, 2], [700, 2000])])
